@@ -253,6 +253,50 @@ int mirec_topk_ordered(const float* Q, int64_t nq, const float* Y, int64_t ni, i
                        size_t ws_bytes, mirec_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Drawing items from rows of scores: the stochastic counterpart of mirec_topk, over
+ * its ranked lists (`ids` given) or over dense rows of scores of any model
+ * (recommenders/als_recommender.py:181-186 and hybrid_docker/inference.py:156-197
+ * always serve the best items; a service that explores, or a trainer that samples
+ * negatives, draws them).  Per row, with s the scores that are not excluded:
+ *   w_i = exp((s_i - max s) / temperature), in the order (score descending, index
+ *   ascending); top_k keeps the first top_k items (0: all), top_p the shortest prefix
+ *   of those that holds top_p of their mass (an item stays if the mass before it is
+ *   below top_p; 1: all; at least one item stays), min_p the items with
+ *   w_i >= min_p * max w; a temperature below 1e-37 keeps the best item;
+ *   draw d takes the first index i whose running sum of kept weights, in ascending
+ *   index order, exceeds uniforms[row, d] * total.
+ * replacement = 0: a drawn item leaves the row before its next draw.
+ * out_ids int32[n, draws]: the item (ids[row, i] where ids are given, else i), or -1
+ * where nothing is left; out_logprob fp32[n, draws]: the natural logarithm of the
+ * probability the item was drawn with (-inf with id -1).
+ * Excluded are scores that are NaN or not above the lowest finite value of their type
+ * (what mirec_topk gives filtered items and empty slots), items of the row's filter
+ * (mask_indptr / mask_indices as in mirec_topk, in any order; dense rows only, at most
+ * MIREC_SAMPLE_MAX_MASKED_ITEMS items) and list positions with a negative id.
+ * Weights are fixed-point numbers of S = min(51, 62 - ceil(log2 m)) fraction bits, so
+ * the result does not depend on any order of summation; an item less likely than
+ * 2^-(S+1) of the best one is never drawn.
+ *   scores       [n, m] of `dtype` (MIREC_F32 / F16 / BF16), row r at r * row_stride elements
+ *   ids          int32 [n, m], row r at r * ids_stride elements, or null
+ *   uniforms     fp32 [n, draws] in [0, 1); values outside are moved to its ends, NaN to 0
+ *   row_*        per-row parameters (null: the one value for all rows).  In rows: a
+ *                temperature that is not >= 1e-37 is greedy, top_k <= 0, top_p not
+ *                below 1 and min_p not above 0 do not cut, min_p above 1 counts as 1.
+ * ws: mirec_sample_workspace_bytes(...) bytes of device scratch, 256-byte aligned (null if
+ * 0); two calls that overlap in time need one each. */
+#define MIREC_F32 0
+#define MIREC_F16 1
+#define MIREC_BF16 2
+#define MIREC_SAMPLE_MAX_DRAWS 1024
+#define MIREC_SAMPLE_MAX_MASKED_ITEMS 524288
+size_t mirec_sample_workspace_bytes(int64_t n, int64_t m, int dtype, int draws);
+int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m, int64_t row_stride, const int32_t* ids,
+                 int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
+                 int draws, int replacement, double temperature, const float* row_temperature, int32_t top_k,
+                 const int32_t* row_top_k, double top_p, const float* row_top_p, double min_p, const float* row_min_p,
+                 int32_t* out_ids, float* out_logprob, void* ws, size_t ws_bytes, mirec_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * LightFM representations (lightfm `compute_representation`, reached from
  * `model.predict` at hybrid_docker/inference.py:159-165,188-194):
  *   out[r, emb_col + j] = sum_k (w_k * scale) * E[indices[k], j]   (j < nc)

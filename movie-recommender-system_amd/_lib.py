@@ -53,6 +53,9 @@ SIGNATURES = {
     "mirec_topk_ordered": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _sz, _vp]),
     "mirec_topk_small_workspace_bytes": (_sz, [_i64, _i64, _int]),
     "mirec_topk_small": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _sz, _vp]),
+    "mirec_sample_workspace_bytes": (_sz, [_i64, _i64, _int, _int]),
+    "mirec_sample": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _int, _int, _c.c_double, _vp, _i32, _vp,
+                            _c.c_double, _vp, _c.c_double, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mirec_lightfm_repr": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _f32, _int, _vp, _int, _int, _int, _int, _vp]),
     "mirec_lightfm_predict": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _vp, _vp]),
     "mirec_events_to_csr_workspace_bytes": (_sz, [_i64, _i64]),
@@ -88,7 +91,9 @@ def load(path: str = LIB_PATH):
                 raise MirecError(f"{path} is version {have}, this package binds version {ABI_VERSION}: rebuild it "
                                  "with `python __graft_entry__.py`")
             for name, (res, args) in SIGNATURES.items():
-                fn = getattr(lib, name)
+                fn = getattr(lib, name, None)
+                if fn is None:
+                    raise MirecError(f"{path} has no entry point {name}: rebuild it with `python __graft_entry__.py`")
                 fn.restype = res
                 fn.argtypes = args
             _lib = lib

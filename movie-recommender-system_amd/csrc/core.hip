@@ -16,7 +16,8 @@ void set_error(const char* fmt, ...) {
 
 // 101: cg_steps = MIREC_SOLVE_EXACT (and conf_max in mirec_als_half_sweep: a change of signature)
 // 102: y_absmax in mirec_gram, mirec_gram_static and mirec_als_half_sweep (a change of signature); mirec_topk_small
-extern "C" int mirec_version(void) { return 102; }
+// 103: mirec_sample, mirec_distill_* (new entry points; the signatures of 102 are unchanged)
+extern "C" int mirec_version(void) { return 103; }
 
 extern "C" const char* mirec_last_error(void) { return mirec::g_error; }
 

@@ -501,6 +501,86 @@ def norm_order(Y: torch.Tensor, n_items: Optional[int] = None) -> torch.Tensor:
     return torch.argsort(Y[:ni].norm(dim=1), descending=True, stable=True).to(torch.int32)
 
 
+_SCORE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # MIREC_F32, MIREC_F16, MIREC_BF16
+
+
+def _row_parameter(name: str, v, n: int, dtype: torch.dtype, dev: torch.device):
+    """(one value, tensor or None) of a parameter given as one number or as one number per row."""
+    if not isinstance(v, torch.Tensor):
+        return v, None
+    if v.shape != (n,) or v.dtype != dtype or v.device != dev or not v.is_contiguous():
+        raise ValueError(f"{name} must be one number or a contiguous {dtype} tensor of one value per row on {dev}")
+    return 0, v
+
+
+def sample_scores(scores: torch.Tensor, uniforms: torch.Tensor, ids: Optional[torch.Tensor] = None,
+                  mask: Optional[DeviceCSR] = None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  replacement: bool = True, ws: Optional[torch.Tensor] = None,
+                  out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+    """Draw items from every row of ``scores`` [n, m] (fp32, fp16 or bf16; rows may be strided): softmax at
+    ``temperature`` (0: the best item), cut to the ``top_k`` best (0: all), then to the shortest best-first prefix
+    that holds ``top_p`` of what is left, then to the items at least ``min_p`` times as likely as the best; one draw
+    per column of ``uniforms`` (fp32 [n, draws], numbers in [0, 1)) by inverse look-up in ascending index order.
+    Ties rank by ascending index.  The four parameters are numbers, or tensors of one value per row (fp32; int32
+    for ``top_k``).
+
+    ``ids`` (int32 [n, m]): the rows are ranked lists as ``topk`` returns them, the drawn list entries' ids come
+    back and entries with a negative id or the score -FLT_MAX are never drawn; without it the rows are dense and
+    ``mask`` may hold one row of filtered items per row, as in ``topk``.  ``replacement=False``: an item is drawn
+    at most once per row.
+
+    Returns (ids int32 [n, draws], logprob fp32 [n, draws]): the items and the logarithms of the probabilities they
+    were drawn with; (-1, -inf) where nothing is left to draw.  The same inputs give the same bits on every call."""
+    lib = _lib.require()
+    if scores.dim() != 2 or scores.dtype not in _SCORE_TYPES:
+        raise ValueError("scores must be a 2-D fp32, fp16 or bf16 tensor")
+    n, m = scores.shape
+    dev = scores.device
+    if dev.type != "cuda":
+        raise _lib.MirecError(f"device {dev} is not a HIP device")
+
+    def strided(t, what):
+        if m > 1 and t.stride(1) != 1:
+            raise ValueError(f"the entries of a row of {what} must be adjacent in memory")
+        return int(t.stride(0)) if n > 1 else m
+
+    stride = strided(scores, "scores")
+    if uniforms.dim() != 2 or uniforms.shape[0] != n or uniforms.dtype != torch.float32 or uniforms.device != dev \
+            or not uniforms.is_contiguous():
+        raise ValueError("uniforms must be a contiguous fp32 tensor [rows, draws] on the device of the scores")
+    draws = int(uniforms.shape[1])
+    ids_stride = 0
+    if ids is not None:
+        if mask is not None:
+            raise ValueError("Can't specify both ids and mask")
+        if ids.shape != scores.shape or ids.dtype != torch.int32 or ids.device != dev:
+            raise ValueError("ids must be an int32 tensor of the shape of the scores, on their device")
+        ids_stride = strided(ids, "ids")
+    if mask is not None and (mask.shape != (n, m) or mask.indptr.device != dev):
+        raise ValueError("the filter needs one row per row of the scores, the same number of items and their device")
+    t1, t_rows = _row_parameter("temperature", temperature, n, torch.float32, dev)
+    k1, k_rows = _row_parameter("top_k", top_k, n, torch.int32, dev)
+    p1, p_rows = _row_parameter("top_p", top_p, n, torch.float32, dev)
+    q1, q_rows = _row_parameter("min_p", min_p, n, torch.float32, dev)
+    if out is None:
+        out = (torch.empty((n, draws), dtype=torch.int32, device=dev),
+               torch.empty((n, draws), dtype=torch.float32, device=dev))
+    elif any(o.shape != (n, draws) or o.dtype != t or o.device != dev or not o.is_contiguous()
+             for o, t in zip(out, (torch.int32, torch.float32))):
+        raise ValueError("out must be contiguous tensors [rows, draws] of int32 and fp32 on the device of the scores")
+    need = int(lib.mirec_sample_workspace_bytes(n, m, _SCORE_TYPES[scores.dtype], draws))
+    if need and (ws is None or ws.numel() * ws.element_size() < need or ws.device != dev):
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(lib.mirec_sample(_ptr(scores), _SCORE_TYPES[scores.dtype], n, m, stride, _ptr(ids), ids_stride,
+                                    _ptr(None if mask is None else mask.indptr),
+                                    _ptr(None if mask is None else mask.indices), _ptr(uniforms), draws,
+                                    int(bool(replacement)), float(t1), _ptr(t_rows), min(int(k1), (1 << 31) - 1),
+                                    _ptr(k_rows), float(p1), _ptr(p_rows), float(q1), _ptr(q_rows), _ptr(out[0]),
+                                    _ptr(out[1]), _ptr(ws), need, _stream_ptr()), "mirec_sample")
+    return out
+
+
 class ChunkedDownload:
     """Results of a scoring pass over many queries, brought to host memory while the pass is still running.
 
