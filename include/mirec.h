@@ -297,6 +297,35 @@ int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m, int64_t ro
                  int32_t* out_ids, float* out_logprob, void* ws, size_t ws_bytes, mirec_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Distillation of a factor model from a teacher's ranked lists (a larger ALS model's
+ * `recommend` output, recommenders/als_recommender.py:181-186; the reference trains
+ * every model it serves from the interactions alone).  X [n, f] are the student's
+ * factors of the rows of a step, Y [m, f] its item factors, `ids` / `scores` [n, k] the
+ * teacher's lists as mirec_topk writes them.  With z_bj = x_b . y_j / T:
+ *   q_b = softmax(z_b) over all m items, p_b = softmax(scores_b / T) over the list;
+ *   loss_b = T^2 sum_list p (log p - log q).
+ * teacher_lse (fp32 [n] or null): log sum exp of ALL the teacher's scores over T; then
+ * p = exp(scores / T - teacher_lse), and what the list leaves of both distributions is
+ * one class more in the sum (the student's share of it is taken to be at least 2^-24).
+ * List entries with an id outside 0 .. m-1 or a score that is NaN or not above -FLT_MAX
+ * are left out; entries that name the same item add up; a row without entries has loss
+ * and gradient zero.
+ * mirec_distill_grad writes the gradients of sum_b grad[b] * loss[b]: dX [n, f], dY
+ * [m, f] (either may be null).  It reads what mirec_distill_loss with
+ * with_grad != 0 left in `ws` for the same X, Y, lists and sizes, as often as needed.
+ * f as in the ALS kernels (mirec_factor_width(f, 0)), k <= MIREC_DISTILL_MAX_LIST.
+ * Sums and statistics are fp32 or wider.  The same inputs give the same bits.
+ * ws: mirec_distill_workspace_bytes(n, m, f, k) bytes, 256-byte aligned; calls that
+ * overlap in time need one each. */
+#define MIREC_DISTILL_MAX_LIST 256
+size_t mirec_distill_workspace_bytes(int64_t n, int64_t m, int f, int k);
+int mirec_distill_loss(const float* X, int64_t n, const float* Y, int64_t m, int f, const int32_t* ids,
+                       const float* scores, int k, float temperature, const float* teacher_lse, int with_grad,
+                       float* loss, void* ws, size_t ws_bytes, mirec_stream_t stream);
+int mirec_distill_grad(const float* X, int64_t n, const float* Y, int64_t m, int f, int k, float temperature,
+                       const float* grad, float* dX, float* dY, void* ws, size_t ws_bytes, mirec_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * LightFM representations (lightfm `compute_representation`, reached from
  * `model.predict` at hybrid_docker/inference.py:159-165,188-194):
  *   out[r, emb_col + j] = sum_k (w_k * scale) * E[indices[k], j]   (j < nc)

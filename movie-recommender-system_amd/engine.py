@@ -581,6 +581,101 @@ def sample_scores(scores: torch.Tensor, uniforms: torch.Tensor, ids: Optional[to
     return out
 
 
+def _distill_inputs(X, Y, ids, scores, teacher_lse):
+    n, f = X.shape if X.dim() == 2 else (-1, -1)
+    dev = X.device
+    if dev.type != "cuda":
+        raise _lib.MirecError(f"device {dev} is not a HIP device")
+    if n < 0 or Y.dim() != 2 or Y.shape[1] != f or X.dtype != torch.float32 or Y.dtype != torch.float32:
+        raise ValueError("X and Y must be fp32 factor matrices of the same width")
+    if ids.dim() != 2 or ids.shape[0] != n or ids.shape != scores.shape or ids.dtype != torch.int32 or scores.dtype != torch.float32:
+        raise ValueError("ids (int32) and scores (fp32) must hold one list per row of X")
+    if teacher_lse is not None and (teacher_lse.shape != (n,) or teacher_lse.dtype != torch.float32):
+        raise ValueError("teacher_lse must hold one fp32 number per row of X")
+    for t in (X, Y, ids, scores) + (() if teacher_lse is None else (teacher_lse,)):
+        if t.device != dev or not t.is_contiguous():
+            raise ValueError("factors, lists and teacher_lse must be contiguous and on one device")
+
+
+def _distill_loss(X, Y, ids, scores, temperature, teacher_lse, with_grad, ws=None):
+    """(loss [n], workspace that _distill_grad reads)."""
+    lib = _lib.require()
+    n, f = X.shape
+    m, k = int(Y.shape[0]), int(ids.shape[1])
+    loss = torch.empty(n, dtype=torch.float32, device=X.device)
+    need = int(lib.mirec_distill_workspace_bytes(n, m, f, k))
+    if ws is None or ws.numel() * ws.element_size() < need or ws.device != X.device:
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=X.device)
+    with torch.cuda.device(X.device):
+        _lib.check(lib.mirec_distill_loss(_ptr(X), n, _ptr(Y), m, f, _ptr(ids), _ptr(scores), k, float(temperature),
+                                          _ptr(teacher_lse), int(with_grad), _ptr(loss), _ptr(ws),
+                                          ws.numel() * ws.element_size(), _stream_ptr()), "mirec_distill_loss")
+    return loss, ws
+
+
+def _distill_grad(X, Y, k, temperature, grad, ws, need_x=True, need_y=True):
+    lib = _lib.require()
+    n, f = X.shape
+    dX = torch.empty_like(X) if need_x else None
+    dY = torch.empty_like(Y) if need_y else None
+    with torch.cuda.device(X.device):
+        _lib.check(lib.mirec_distill_grad(_ptr(X), n, _ptr(Y), int(Y.shape[0]), f, int(k), float(temperature), _ptr(grad),
+                                          _ptr(dX), _ptr(dY), _ptr(ws), ws.numel() * ws.element_size(), _stream_ptr()),
+                   "mirec_distill_grad")
+    return dX, dY
+
+
+def distill(X: torch.Tensor, Y: torch.Tensor, ids: torch.Tensor, scores: torch.Tensor, temperature: float = 1.0,
+            teacher_lse: Optional[torch.Tensor] = None, grad: Optional[torch.Tensor] = None,
+            ws: Optional[torch.Tensor] = None):
+    """One distillation step of a factor model: the loss of every row of ``X`` [n, f] against a teacher's ranked
+    lists ``ids`` / ``scores`` [n, k] (what ``topk`` returns) over the items ``Y`` [m, f], and its gradients.
+
+    With z = X Y^T / ``temperature``, q = softmax(z) over all items and p = softmax(scores / temperature) over the
+    row's list, loss = temperature^2 * KL(p || q).  With ``teacher_lse`` (fp32 [n]: log sum exp of all the teacher's
+    scores / temperature) p keeps its mass outside the list, which both sides hold as one class more.  Entries with
+    an id that is no item, a NaN or the score -FLT_MAX are left out, entries of the same item add up, a row without
+    entries has loss and gradient zero.  ``f`` is a width of the ALS kernels (``factor_width``, zero-padded), k at
+    most 256.
+
+    Returns (loss [n], dX [n, f], dY [m, f]), the gradients of sum(grad * loss) (``grad`` fp32 [n]; None: ones).
+    The matrix of scores is never written.  ``ws`` lets a caller that takes many steps reuse its workspace."""
+    _distill_inputs(X, Y, ids, scores, teacher_lse)
+    if grad is None:
+        grad = torch.ones(X.shape[0], dtype=torch.float32, device=X.device)
+    elif grad.shape != (X.shape[0],) or grad.dtype != torch.float32 or grad.device != X.device or not grad.is_contiguous():
+        raise ValueError("grad must hold one fp32 number per row of X")
+    loss, ws = _distill_loss(X, Y, ids, scores, temperature, teacher_lse, True, ws)
+    return (loss,) + _distill_grad(X, Y, ids.shape[1], temperature, grad, ws)
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, X, Y, ids, scores, temperature, teacher_lse):
+        need = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        loss, ws = _distill_loss(X, Y, ids, scores, temperature, teacher_lse, need)
+        if need:
+            ctx.save_for_backward(X, Y, ws)
+            ctx.k, ctx.temperature = int(ids.shape[1]), float(temperature)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        X, Y, ws = ctx.saved_tensors
+        dX, dY = _distill_grad(X, Y, ctx.k, ctx.temperature, grad.contiguous(), ws, ctx.needs_input_grad[0],
+                               ctx.needs_input_grad[1])
+        return dX, dY, None, None, None, None
+
+
+def distill_loss(X: torch.Tensor, Y: torch.Tensor, ids: torch.Tensor, scores: torch.Tensor, temperature: float = 1.0,
+                 teacher_lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The loss of ``distill`` [n] as a differentiable function of ``X`` and ``Y`` (once; the lists and
+    ``teacher_lse`` are constants)."""
+    _distill_inputs(X, Y, ids, scores, teacher_lse)
+    return _Distill.apply(X, Y, ids, scores, temperature, teacher_lse)
+
+
 class ChunkedDownload:
     """Results of a scoring pass over many queries, brought to host memory while the pass is still running.
 
