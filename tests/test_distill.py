@@ -3,7 +3,10 @@
 Tolerances.  A logit is a sum of f products of fp32 values carried to at least 22 bits: with S = max sum |x y| / T it is
 off by at most dz = (8 sqrt(f) 2^-24 + 2 * 2^-22) S, eight standard deviations of f roundings of half a step and both
 operands' truncation.  A probability is then off by a factor 1 + 2 dz + 8 * 2^-24 (the logit's and the log-sum's error,
-exponential and division), and a sum of m (or n) such terms by 8 sqrt(m) 2^-24 of the sum of their magnitudes on top."""
+exponential and division), and a sum of m (or n) such terms by 8 sqrt(m) 2^-24 of the sum of their magnitudes on top.
+The weights of the sums are held as two fp16 numbers: the smallest step of fp16 is 2^-24, so each is off by 2^-25 at
+most where it is too small for its 22 bits.  With the largest weight grad_b T scaled to at least 2^14 that is 2^-39 of it
+per row of dY; with a row's largest probability scaled to at least 2^7 it is 2^-32 of that probability per item of dX."""
 
 import math
 
@@ -70,8 +73,10 @@ def tolerances(X, Y, T, G, has, tlse, loss, grad):
     rel = 2 * dz + 16 * HALF
     if tlse is not None:
         rel = rel * 4 + 1e-6   # p_r / q_r: both are differences from one
-    tx = (rel + 8 * math.sqrt(m) * HALF) * (mag @ Y.abs()) + 1e-30
-    ty = (rel + 8 * math.sqrt(n) * HALF) * (mag.T @ X.abs()) + 1e-30
+    w = torch.ones(n, dtype=torch.float64) if grad is None else grad.double().cpu().abs()
+    tx = (rel + 8 * math.sqrt(m) * HALF) * (mag @ Y.abs())
+    tx = tx + m * 2.0 ** -32 * (T * w * has * q.amax(1))[:, None] * Y.abs().amax()
+    ty = (rel + 8 * math.sqrt(n) * HALF) * (mag.T @ X.abs()) + n * 2.0 ** -39 * T * w.max() * X.abs().amax()
     tl = T * T * (2 * dz + 64 * HALF) * (1 + loss.abs() / (T * T)) * (4 if tlse is not None else 1) + 4 * HALF * loss.abs()
     return tl, tx, ty
 
@@ -123,7 +128,7 @@ def c_call(entry, X=256, n=4, Y=256, m=8, f=32, ids=256, scores=256, k=3, T=1.0,
     ({"T": -1.0}, -1, "temperature"), ({"T": float("nan")}, -1, "temperature"), ({"T": float("inf")}, -1, "temperature"),
     ({"m": 0}, -1, "empty"), ({"X": None}, -1, "null"), ({"Y": None}, -1, "null"), ({"X": 260}, -1, "aligned"),
     ({"Y": 264}, -1, "aligned"), ({"ws": None}, -2, "workspace"), ({"ws": 320}, -2, "workspace"), ({"ws_bytes": 100}, -2, "workspace"),
-    ({"n": 1 << 31}, -4, "2^31"), ({"m": 1 << 31}, -4, "2^31"),
+    ({"n": (1 << 28) + 1}, -4, "2^28"), ({"m": (1 << 28) + 1}, -4, "2^28"),
 ])
 def test_the_c_entries_refuse(entry, change, code, text):
     rc, msg = c_call(entry, **change)
