@@ -32,11 +32,15 @@
 
 namespace mirec {
 
-constexpr int DI_LIST = MIREC_DISTILL_MAX_LIST;   // longest list; one thread per entry in distill_list_kernel
+constexpr int DI_LIST = MIREC_DISTILL_MAX_LIST;   // longest list
+constexpr int64_t DI_MANY_ROWS = 2048;            // from here on a wavefront per row in distill_list_kernel
 constexpr int DI_THREADS = 256;
 constexpr int DI_NW = 8;                          // wavefronts of a workgroup of the two passes
 constexpr int DI_OWN = 32 * DI_NW;                // rows it owns
 constexpr int DI_PARTS = 256;                     // partial maxima of a matrix
+constexpr int DI_MAX_THREADS = 1024;              // of the workgroups that find them
+constexpr int DI_GROUP_THREADS = 1024;
+constexpr int DI_BINS = 4096;                     // item tiles that distill_group_kernel counts at a time
 constexpr int DI_CUS = 256;                       // workgroups that run at once
 constexpr float DI_HEADROOM = 7.f;                // log2 of a probability's scale when its row's reference is current
 
@@ -60,10 +64,11 @@ struct DistillTile {
 
 // Workspace of a call pair (host side): what mirec_distill_loss leaves for mirec_distill_grad, and scratch.
 struct DistillWorkspace {
-    size_t max_off, ref_off, mass_off, a_off, count_off, id_off, val_off, start_off, base_off, ximg_off, yimg_off, pref_off,
+    size_t max_off, ref_off, mass_off, a_off, count_off, id_off, val_off, start_off, place_off, gval_off, row_off, base_off, ximg_off, yimg_off, pref_off,
         pmass_off, part_off, bytes;
     int64_t xtiles, ytiles;
-    int splits_x, splits_y;   // ranges the streamed side is cut into: of Y in the forward pass, of X in the backward
+    int splits_x;      // ranges that Y is cut into in the forward pass
+    int64_t runs;      // workgroups of the backward pass
 };
 
 // Into how many ranges to cut the streamed tiles: the fewest rounds of 256 workgroups, each paying for its start (four
@@ -94,7 +99,7 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.ytiles = (m + 31) / 32;
     const int64_t xblocks = (n + DI_OWN - 1) / DI_OWN, yblocks = (m + DI_OWN - 1) / DI_OWN;
     w.splits_x = distill_splits(xblocks, w.ytiles);
-    w.splits_y = distill_splits(yblocks, w.xtiles);
+    w.runs = yblocks * w.xtiles < DI_CUS ? yblocks * w.xtiles : DI_CUS;
     w.max_off = take(3 * DI_PARTS * 4);       // partial maxima of |X|, |Y|, |grad|
     w.ref_off = take((size_t)n * 4);          // M_b: log2 reference of a row's mass
     w.mass_off = take((size_t)n * 4);         // sum_j 2^(z_bj log2 e - M_b)
@@ -102,57 +107,46 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.count_off = take((size_t)n * 4);        // entries of the merged list
     w.id_off = take((size_t)n * k * 4);       // merged list, ascending ids
     w.val_off = take((size_t)n * k * 4);      // q - p of those
-    w.start_off = take((size_t)n * (w.ytiles + 1) * 2);   // where the entries of an item tile begin in the list
+    // the same by (row tile, item tile): where a group begins, the entries' places in their 32 x 32 block, q - p
+    w.start_off = take((size_t)w.xtiles * (w.ytiles + 1) * 2);
+    w.place_off = take((size_t)n * k * 2);
+    w.gval_off = take((size_t)n * k * 4);
+    w.row_off = take((size_t)n * 16);         // what a row brings to the backward pass
     w.base_off = take((size_t)n * f * 4);     // dX_b / (grad_b T)
     w.ximg_off = take((size_t)w.xtiles * 256 * f);
     w.yimg_off = take((size_t)w.ytiles * 256 * f);
     w.pref_off = take((size_t)w.splits_x * n * 4);
     w.pmass_off = take((size_t)w.splits_x * n * 4);
-    const size_t px = (size_t)w.splits_x * n * f * 4, py = w.splits_y > 1 ? (size_t)w.splits_y * m * f * 4 : 0;
-    w.part_off = take(px > py ? px : py);     // partial means, later partial dY
+    const size_t px = (size_t)w.splits_x * n * f * 4, py = (size_t)w.runs * 2 * DI_OWN * f * 4;
+    w.part_off = take(px > py ? px : py);     // partial means, later parts of dY
     w.bytes = at;
     return w;
-}
-
-__device__ __forceinline__ float di_block_max(float v, float* part) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    for (int w = 0; w < DI_THREADS / 64; ++w) v = fmaxf(v, part[w]);
-    return v;
-}
-
-__device__ __forceinline__ double di_block_sum(double v, double* part) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < DI_THREADS / 64; ++w) v += part[w];
-    return v;
 }
 
 // ------------------------------------------------------------------------------------------------ operand images
 
 // Largest magnitude of up to two arrays (blockIdx.y), as DI_PARTS partial maxima of bit patterns each (a NaN's is
 // above every number's).
-__global__ __launch_bounds__(DI_THREADS) void distill_absmax_kernel(const float* __restrict__ a, int64_t na,
+__global__ __launch_bounds__(DI_MAX_THREADS) void distill_absmax_kernel(const float* __restrict__ a, int64_t na,
                                                                     const float* __restrict__ b, int64_t nb,
                                                                     uint32_t* __restrict__ parts) {
-    __shared__ uint32_t part[DI_THREADS / 64];
+    __shared__ uint32_t part[DI_MAX_THREADS / 64];
     const float* v = blockIdx.y ? b : a;
     const int64_t cnt = blockIdx.y ? nb : na;
     uint32_t top = 0;
-    for (int64_t e = ((int64_t)blockIdx.x * DI_THREADS + threadIdx.x) * 4; e < cnt; e += (int64_t)DI_PARTS * DI_THREADS * 4) {
-        const f32x4 q = *reinterpret_cast<const f32x4*>(v + e);   // the widths are multiples of 32: no tail
+    constexpr int64_t step = (int64_t)DI_PARTS * DI_MAX_THREADS * 4;
+    // (the widths are multiples of 32: no tail; a thread past the end reads its first value again)
+    for (int64_t e = ((int64_t)blockIdx.x * DI_MAX_THREADS + threadIdx.x) * 4; e < cnt; e += 4 * step) {
+        f32x4 q[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t u = __float_as_uint(q[i]) & 0x7fffffffu;
-            top = u > top ? u : top;
-        }
+        for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const f32x4*>(v + (e + u * step < cnt ? e + u * step : e));
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t b = __float_as_uint(q[u][i]) & 0x7fffffffu;
+                top = b > top ? b : top;
+            }
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -162,7 +156,7 @@ __global__ __launch_bounds__(DI_THREADS) void distill_absmax_kernel(const float*
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < DI_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
+        for (int w = 1; w < DI_MAX_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
         parts[blockIdx.y * DI_PARTS + blockIdx.x] = top;
     }
 }
@@ -336,7 +330,7 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
     typedef DistillTile<F> D;
     constexpr int FETCH = GRAD ? D::BYTES : 2 * D::PLANE;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int64_t work = di_work_index();
     const int64_t range = work / blocks, block = work % blocks;
     const int64_t t0 = range * tiles_per_range;
@@ -404,250 +398,385 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
     }
 }
 
-// Items [32 w, 32 w + 32) of the block per wavefront against a range of row tiles: their gradient from those rows.
+// First of the steps that workgroup w of `runs` takes.
+__host__ __device__ __forceinline__ int64_t di_run_begin(int64_t w, int64_t steps, int64_t runs) { return w * steps / runs; }
+
+// The gradients of the items: 32 of them per wavefront, 256 per workgroup, against all tiles of rows.  The steps (block of
+// items, row tile) are numbered block by block and cut into equal runs, one per workgroup, whatever the number of
+// blocks: 106 or 782 blocks are 0.4 and 3.05 rounds of 256 workgroups.  A workgroup writes a block that it
+// sees whole to its place, and what it has of a block at an end of its run to a slot of its own, which
+// distill_join_kernel adds up in the order of the rows.
 template <int F>
 __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
-    const char* __restrict__ yimg, int64_t m, int64_t blocks, const char* __restrict__ ximg, int64_t n, int64_t xtiles,
-    int64_t tiles_per_range, float step, float temperature, const uint32_t* __restrict__ parts, const float* __restrict__ ref,
-    const float* __restrict__ mass, const float* __restrict__ a, const float* __restrict__ grad,
-    const uint16_t* __restrict__ start, int64_t ytiles, const int32_t* __restrict__ list_id,
-    const float* __restrict__ list_val, int k, float* __restrict__ out) {
+    const char* __restrict__ yimg, int64_t m, int64_t steps, const char* __restrict__ ximg, int64_t n, int64_t xtiles,
+    float step, float temperature, const uint32_t* __restrict__ parts, const f32x4* __restrict__ row_const,
+    const uint16_t* __restrict__ start, int64_t ytiles, const uint16_t* __restrict__ place, const float* __restrict__ gval,
+    int k, float* __restrict__ dY, float* __restrict__ slots) {
     typedef DistillTile<F> D;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     __shared__ __attribute__((aligned(16))) float row_off[2][32], row_w[2][32], row_v[2][32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-    const int64_t work = di_work_index();
-    const int64_t range = work / blocks, block = work % blocks;
-    const int64_t t0 = range * tiles_per_range;
-    const int64_t t1 = t0 + tiles_per_range < xtiles ? t0 + tiles_per_range : xtiles;
-    const int64_t own0 = block * DI_OWN + wave * 32, jt = own0 / 32;
-    const bool active = own0 < m;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const int64_t run0 = di_run_begin(blockIdx.x, steps, gridDim.x), run1 = di_run_begin(blockIdx.x + 1, steps, gridDim.x);
     const int sx = di_scale_exponent(parts), sy = di_scale_exponent(parts + DI_PARTS);
     const int sg = di_scale_exponent(parts + 2 * DI_PARTS);   // the weights of the rows; |q - p| and |A q| are at most 1
     const float c = ldexpf(step, -sx - sy);
 
-    // what a row brings besides its factors: the reference of its logits, the weight of a probability, that of a list entry
-    float p_ref = 0.f, p_w = 0.f, p_v = 0.f;
+    const float back = ldexpf(temperature, -sx - sg);
+
+    f32x4 p_row = {0.f, 0.f, 0.f, 0.f};
     auto fetch_rows = [&](int64_t t) {
         if (tid < 32) {
             const int64_t b = t * 32 + tid;
-            const float w = b < n ? ldexpf(grad[b], sg) : 0.f;
-            p_ref = b < n ? -ref[b] : 0.f;
-            p_v = w;
-            p_w = b < n ? w * a[b] / mass[b] : 0.f;
+            p_row = b < n ? row_const[b] : f32x4{0.f, 0.f, 0.f, 0.f};
         }
     };
-    auto store_rows = [&](int64_t t) {
+    int cur = 0;   // the buffer of the current step
+    auto store_rows = [&]() {
         if (tid < 32) {
-            row_off[(t - t0) & 1][tid] = p_ref;
-            row_w[(t - t0) & 1][tid] = p_w;
-            row_v[(t - t0) & 1][tid] = p_v;
+            row_off[cur][tid] = p_row[0];
+            row_w[cur][tid] = ldexpf(p_row[1], sg);
+            row_v[cur][tid] = ldexpf(p_row[2], sg);
         }
     };
-    // a lane's row (of the tile) on the lists: where the entries of this wavefront's items begin and end
+    // The list entries that fall on this wavefront's items and a tile's rows.  Where they begin and end is asked for
+    // two steps ahead, the first 64 of them (one per lane) one step ahead.
+    struct Step {
+        int block, t;
+    };
+    const int xt = (int)xtiles;
+    auto after = [&](Step p) { return p.t + 1 < xt ? Step{p.block, p.t + 1} : Step{p.block + 1, 0}; };
     int e0 = 0, e1 = 0;
-    auto fetch_list = [&](int64_t t) {
-        const int64_t b = t * 32 + (lane & 31);
+    auto fetch_extent = [&](Step p) {
+        const int64_t jt = (int64_t)p.block * DI_NW + wave;
         e0 = e1 = 0;
-        if (active && b < n) {
-            e0 = start[b * (ytiles + 1) + jt];
-            e1 = start[b * (ytiles + 1) + jt + 1];
-            e1 = e1 < k ? e1 : k;   // whatever the workspace holds, the list is not left
+        if (jt < ytiles) {
+            const uint16_t* at = start + p.t * (ytiles + 1) + jt;
+            e0 = at[0];
+            e1 = at[1];
+            // whatever the workspace holds, the tile's entries are not left
+            const int64_t have = (n - p.t * 32 < 32 ? n - p.t * 32 : 32) * k;
+            e1 = e1 < have ? e1 : (int)have;
         }
     };
-    di_fetch(ximg + t0 * D::BYTES, lds, D::BYTES);
-    fetch_rows(t0);
-    fetch_list(t0);
-    u32x4 own[2][F / 16];
-    if (active) di_load_own<F>(yimg + jt * D::BYTES, own);
-    f32x16 acc[F / 32] = {};
-    for (int64_t t = t0; t < t1; ++t) {
-        const int cur = (int)((t - t0) & 1);
-        const char* tile = lds + cur * D::BYTES;
-        store_rows(t);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        // the first entry of each row's part of the list
-        const int f0 = e0, f1 = e1;
-        const int64_t lrow = (t * 32 + (lane & 31)) * k;
-        int32_t id = 0;
-        float val = 0.f;
-        if (f1 > f0) {
-            id = list_id[lrow + f0];
-            val = list_val[lrow + f0];
+    int entries = 0, spot = 0;
+    float val = 0.f;
+    int64_t list0 = 0;
+    auto fetch_entries = [&](Step p) {
+        entries = __builtin_amdgcn_readfirstlane(e1 - e0);
+        list0 = (int64_t)p.t * 32 * k + __builtin_amdgcn_readfirstlane(e0);
+        if (lane < entries) {
+            spot = place[list0 + lane] & 1023;
+            val = gval[list0 + lane];
         }
-        if (t + 1 < t1) {
-            di_fetch(ximg + (t + 1) * D::BYTES, lds + (cur ^ 1) * D::BYTES, D::BYTES);
-            fetch_rows(t + 1);
-            fetch_list(t + 1);
-        }
-        if (!active) continue;
-        f32x16 z = di_logits<F>(tile, own);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 o = *reinterpret_cast<const f32x4*>(&row_off[cur][8 * g + 4 * half]);
-            const f32x4 w = *reinterpret_cast<const f32x4*>(&row_w[cur][8 * g + 4 * half]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + i], c, o[i])) * w[i];
-        }
-        // where an item is on a row's list, its gradient is not A q but q - p
-        uint32_t rows = (uint32_t)__ballot(half == 0 && f1 > f0);
-        while (rows) {
-            const int r = __builtin_ctz(rows);
-            rows &= rows - 1;
-            const int n_e = __builtin_amdgcn_readlane(f1 - f0, r);
-            int32_t item = __builtin_amdgcn_readlane(id, r);
-            float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(val), r));
-            const int first = __builtin_amdgcn_readlane(f0, r);
-            for (int e = 0;;) {
-                const bool here = lane == (int)(item - own0) + 32 * ((r >> 2) & 1);
-                const float gv = v * row_v[cur][r];
-                const int reg = 4 * (r >> 3) + (r & 3);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (i == reg) z[i] = here ? gv : z[i];
-                if (++e >= n_e) break;
-                item = list_id[(t * 32 + r) * k + first + e];
-                v = list_val[(t * 32 + r) * k + first + e];
+    };
+    // Their values on the way to the lanes and registers that hold their places: 16 values per lane (rows of 20: 16-byte
+    // reads of neighbouring lanes fall into distinct banks) and a bit for each that is there.
+    float* fix = reinterpret_cast<float*>(lds + 2 * D::BYTES) + wave * (64 * 20 + 64);
+    uint32_t* fix_bits = reinterpret_cast<uint32_t*>(fix + 64 * 20);
+    fix_bits[lane] = 0;
+    Step now = {(int)(run0 / xtiles), (int)(run0 % xtiles)};
+    di_fetch(ximg + (int64_t)now.t * D::BYTES, lds, D::BYTES);
+    fetch_rows(now.t);
+    fetch_extent(now);
+    fetch_entries(now);
+    Step next = after(now);
+    fetch_extent(next);
+    bool first = true;
+    for (int64_t left = run1 - run0; left > 0;) {   // block by block
+        const int t0 = now.t, t1 = left < xt - t0 ? t0 + (int)left : xt;
+        const int64_t block = now.block;
+        const int64_t own0 = block * DI_OWN + wave * 32;
+        const bool active = own0 < m;
+        u32x4 own[2][F / 16];
+        if (active) di_load_own<F>(yimg + own0 / 32 * D::BYTES, own);
+        f32x16 acc[F / 32] = {};
+        for (int t = t0; t < t1; ++t, cur ^= 1) {
+            const char* tile = lds + cur * D::BYTES;
+            store_rows();
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int have = entries;
+            for (int done = 0; done < have; done += 64) {
+                if (done > 0 && lane < have - done) {
+                    spot = place[list0 + done + lane] & 1023;
+                    val = gval[list0 + done + lane];
+                }
+                if (lane < have - done) {
+                    const int r = spot >> 5, to = (spot & 31) + 32 * ((r >> 2) & 1), reg = 4 * (r >> 3) + (r & 3);
+                    fix[to * 20 + reg] = val * row_v[cur][r];
+                    atomicOr(&fix_bits[to], 1u << reg);
+                }
             }
+            now = next;
+            next = after(next);
+            if (--left > 0) {
+                di_fetch(ximg + (int64_t)now.t * D::BYTES, lds + (cur ^ 1) * D::BYTES, D::BYTES);
+                fetch_rows(now.t);
+                fetch_entries(now);
+                fetch_extent(next);   // (behind the run's last step: read, not used)
+            }
+            if (!active) continue;
+            f32x16 z = di_logits<F>(tile, own);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 o = *reinterpret_cast<const f32x4*>(&row_off[cur][8 * g + 4 * half]);
+                const f32x4 w = *reinterpret_cast<const f32x4*>(&row_w[cur][8 * g + 4 * half]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    z[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + i], c, o[i])) * w[i];
+            }
+            // where an item is on a row's list, its gradient is not A q but q - p
+            if (have > 0) {
+                asm volatile("" ::: "memory");   // written by other lanes of this wavefront, in order
+                const uint32_t bits = fix_bits[lane];
+                fix_bits[lane] = 0;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(fix + lane * 20 + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[4 * g + i] = (bits >> (4 * g + i)) & 1u ? v[i] : z[4 * g + i];
+                }
+            }
+            di_accumulate<F>(tile, z, acc);
         }
-        di_accumulate<F>(tile, z, acc);
+        const int64_t item = own0 + (lane & 31);
+        if (active && item < m) {
+            // a part of a block goes to slot 0 where the run begins with it, else to slot 1
+            float* out = t0 == 0 && t1 == xt ? dY + item * F
+                                                 : slots + ((2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * DI_OWN + wave * 32 + (lane & 31)) * F;
+#pragma unroll
+            for (int u = 0; u < F / 32; ++u)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 q = {acc[u][4 * g] * back, acc[u][4 * g + 1] * back, acc[u][4 * g + 2] * back, acc[u][4 * g + 3] * back};
+                    *reinterpret_cast<f32x4*>(out + 32 * u + 8 * g + 4 * half) = q;
+                }
+        }
+        first = false;
     }
-    const int64_t item = own0 + (lane & 31);
-    if (!active || item >= m) return;
-    const float back = ldexpf(temperature, -sx - sg);
-#pragma unroll
-    for (int u = 0; u < F / 32; ++u)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 q = {acc[u][4 * g] * back, acc[u][4 * g + 1] * back, acc[u][4 * g + 2] * back, acc[u][4 * g + 3] * back};
-            *reinterpret_cast<f32x4*>(out + (range * m + item) * F + 32 * u + 8 * g + 4 * half) = q;
-        }
 }
 
-// The sum of the ranges' partial gradients, in their order.
-__global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* __restrict__ part, int ranges, int64_t cnt,
-                                                                  float* __restrict__ out) {
-    for (int64_t e = ((int64_t)blockIdx.x * DI_THREADS + threadIdx.x) * 4; e < cnt; e += (int64_t)gridDim.x * DI_THREADS * 4) {
-        f32x4 v = *reinterpret_cast<const f32x4*>(part + e);
-        for (int r = 1; r < ranges; ++r) v += *reinterpret_cast<const f32x4*>(part + r * cnt + e);
-        *reinterpret_cast<f32x4*>(out + e) = v;
+// The blocks that no workgroup saw whole: the sum of their parts, in the order of the rows.  One workgroup column per
+// run; it takes the block that its run begins inside of, if no run before it does.
+__global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* __restrict__ slots, int64_t steps, int64_t runs,
+                                                                  int64_t xtiles, int64_t m, int f, float* __restrict__ dY) {
+    const int64_t begin = di_run_begin(blockIdx.x + 1, steps, runs), block = begin / xtiles, s0 = block * xtiles, s1 = s0 + xtiles;
+    const int64_t w0 = blockIdx.x, before = di_run_begin(w0, steps, runs);   // the run that ends inside the block
+    if (begin == s0 || before > s0) return;
+    int64_t w1 = w0 + 1;   // one past the last run with a part of the block
+    while (w1 < runs && di_run_begin(w1, steps, runs) < s1) ++w1;
+    const int first_slot = before == s0 ? 0 : 1;
+    const int64_t rows = m - block * DI_OWN < DI_OWN ? m - block * DI_OWN : DI_OWN;
+    for (int64_t e = ((int64_t)blockIdx.y * DI_THREADS + threadIdx.x) * 4; e < rows * f; e += (int64_t)gridDim.y * DI_THREADS * 4) {
+        f32x4 v = *reinterpret_cast<const f32x4*>(slots + (2 * w0 + first_slot) * DI_OWN * f + e);
+        for (int64_t w = w0 + 1; w < w1; ++w) v += *reinterpret_cast<const f32x4*>(slots + 2 * w * DI_OWN * f + e);
+        *reinterpret_cast<f32x4*>(dY + block * DI_OWN * f + e) = v;
     }
 }
 
 // ------------------------------------------------------------------------------------------------------- the lists
 
-// One workgroup per row, one thread per list entry: joins the row's partial results; the list without its excluded
-// entries, ordered by item, entries that name the same item merged (their probabilities add), and where the entries of
-// every item tile begin in it; the row's loss; its dX but for the weight.
-__global__ __launch_bounds__(DI_LIST) void distill_list_kernel(
-    const float* __restrict__ X, int64_t n, const float* __restrict__ Y, int64_t m, int f, const int32_t* __restrict__ ids,
+// One workgroup per row: joins the row's partial results; the list without its excluded entries, entries that name the
+// same item merged (their probabilities add); the row's loss; its dX but for the weight.  Latency, not bandwidth, is
+// what a row costs (a chain of a dozen dependent steps): factor rows are read by sixteen lanes each, four rows of a
+// group of lanes in flight, and what does not depend on each other is asked for at once.  NT threads: 256 finish a row
+// soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) many rows: DI_MANY_ROWS.
+template <int F, int NT>
+__global__ __launch_bounds__(NT) void distill_list_kernel(
+    const float* __restrict__ X, int64_t n, const float* __restrict__ Y, int64_t m, const int32_t* __restrict__ ids,
     const float* __restrict__ scores, int k, float temperature, const float* __restrict__ teacher_lse, int ranges,
     const float* __restrict__ pref, const float* __restrict__ pmass, const float* __restrict__ psum,
     const uint32_t* __restrict__ parts, float* __restrict__ loss, float* __restrict__ ref_out, float* __restrict__ mass_out,
     float* __restrict__ a_out, int32_t* __restrict__ count_out, int32_t* __restrict__ id_out, float* __restrict__ val_out,
-    uint16_t* __restrict__ start_out, float* __restrict__ base) {
-    __shared__ uint64_t key[DI_LIST];
-    __shared__ int32_t sid[DI_LIST];     // by ascending item
-    __shared__ float st[DI_LIST];        // log p, then the coefficient of y in dX
-    __shared__ float sp[DI_LIST];        // p
-    __shared__ int32_t mid[DI_LIST];     // merged
-    __shared__ float mlogp[DI_LIST], mp[DI_LIST], mz[DI_LIST];
-    __shared__ float partf[DI_THREADS / 64];
-    __shared__ double partd[DI_THREADS / 64];
-    __shared__ int parti[DI_THREADS / 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float* __restrict__ base) {
+    constexpr int PIECES = F / 32;     // 8-byte pieces of a factor row per lane
+    constexpr int ROWS = NT / 16;      // factor rows that the workgroup reads side by side
+    constexpr int NWV = NT / 64;
+    extern __shared__ __attribute__((aligned(16))) char list_lds[];
+    const int kp = (k + 63) & ~63;
+    uint64_t* key = reinterpret_cast<uint64_t*>(list_lds);          // item and place; later p and log p of the merged entries
+    int32_t* sid = reinterpret_cast<int32_t*>(key + kp);            // by ascending item
+    float* sp = reinterpret_cast<float*>(sid + kp);                 // p
+    float* slogp = sp + kp;
+    int32_t* mid = reinterpret_cast<int32_t*>(slogp + kp);          // merged
+    float* mz = reinterpret_cast<float*>(mid + kp);                 // logits, then the coefficients of y in dX
+    float* mp = reinterpret_cast<float*>(key);
+    float* mlogp = mp + kp;
+    __shared__ float red[NWV][F];
+    __shared__ float range_w[64];
+    __shared__ float row_ref, row_mass;
+    __shared__ double partd[2][NWV];
+    __shared__ int parti[NWV];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = tid >> 4, sub = tid & 15;
     const double inv_t = 1.0 / (double)temperature;
-    const int64_t ytiles = (m + 31) / 32;
     const int sy = di_scale_exponent(parts + DI_PARTS);
+    auto block_sum = [&](double v, int which) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+        if (NWV == 1) return v;
+        if (lane == 0) partd[which][wave] = v;
+        __syncthreads();
+        v = partd[which][0];
+        for (int w = 1; w < NWV; ++w) v += partd[which][w];
+        __syncthreads();
+        return v;
+    };
 
     for (int64_t b = blockIdx.x; b < n; b += gridDim.x) {
-        float ref = -INFINITY, mass2 = 0.f, mean = 0.f;
-        for (int r = 0; r < ranges; ++r) ref = fmaxf(ref, pref[r * n + b]);
-        for (int r = 0; r < ranges; ++r) {
-            const float w = __builtin_amdgcn_exp2f(pref[r * n + b] - ref);
-            mass2 = __builtin_fmaf(pmass[r * n + b], w, mass2);
-            if (base && tid < f) mean = __builtin_fmaf(psum[(r * n + b) * f + tid], w, mean);
+        f32x2 x[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) x[i] = *reinterpret_cast<const f32x2*>(X + b * F + 2 * (sub + 16 * i));
+        __syncthreads();   // the row before is done with the shared arrays
+        if (wave == 0) {   // at most 64 ranges: one lane each
+            const float r = lane < ranges ? pref[lane * n + b] : -INFINITY;
+            const float pm = lane < ranges ? pmass[lane * n + b] : 0.f;
+            float top = r;
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            const float w = lane < ranges ? __builtin_amdgcn_exp2f(r - top) : 0.f;
+            const float sum = wave_sum(pm * w);
+            range_w[lane] = ldexpf(w / sum, -sy);
+            if (lane == 0) {
+                row_ref = top;
+                row_mass = ldexpf(sum, -(int)DI_HEADROOM);
+                ref_out[b] = row_ref;
+                mass_out[b] = row_mass;
+            }
         }
-        mean = ldexpf(mean / mass2, -sy);
-        mass2 = ldexpf(mass2, -(int)DI_HEADROOM);
-        const double log_mass = (double)ref * 0.69314718055994531 + log((double)mass2);   // log sum exp of the logits
-
-        const int32_t id = tid < k ? ids[b * k + tid] : -1;
-        const float s = tid < k ? scores[b * k + tid] : 0.f;
-        const bool valid = id >= 0 && id < m && s > -FLT_MAX;
-        const float top = di_block_max(valid ? s : -INFINITY, partf);
-        // log p of the entry (before merging)
-        const double d = s == top ? 0.0 : ((double)s - (double)top) * inv_t;
-        const double mass = di_block_sum(valid ? (double)expf((float)d) : 0.0, partd);
-        const int nvalid = __syncthreads_count(valid);
-        if (tid == 0) {
-            ref_out[b] = ref;
-            mass_out[b] = mass2;
+        // the entries that count, the best of them and their mass
+        float top = -INFINITY;
+        int valid = 0;
+        for (int e = tid; e < kp; e += NT) {
+            const int32_t id = e < k ? ids[b * k + e] : -1;
+            const float s = e < k ? scores[b * k + e] : 0.f;
+            const bool ok = id >= 0 && id < m && s > -FLT_MAX;
+            key[e] = ok ? ((uint64_t)id << 8) | (uint64_t)e : ~0ull;
+            slogp[e] = s;
+            if (ok) top = fmaxf(top, s);
+            valid += ok ? 1 : 0;
         }
-        if (nvalid == 0) {   // nothing to learn from this row
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            top = fmaxf(top, __shfl_xor(top, d, 64));
+            valid += __shfl_xor(valid, d, 64);
+        }
+        if (NWV > 1) {
+            if (lane == 0) {
+                sp[wave] = top;
+                parti[wave] = valid;
+            }
+            __syncthreads();
+            top = sp[0];
+            valid = parti[0];
+            for (int w = 1; w < NWV; ++w) {
+                top = fmaxf(top, sp[w]);
+                valid += parti[w];
+            }
+        }
+        __syncthreads();
+        if (valid == 0) {   // nothing to learn from this row
             if (tid == 0) {
                 loss[b] = 0.f;
                 a_out[b] = 0.f;
                 count_out[b] = 0;
             }
-            if (base) {
-                if (tid < f) base[b * f + tid] = 0.f;
-                for (int64_t t = tid; t <= ytiles; t += DI_LIST) start_out[b * (ytiles + 1) + t] = 0;
-            }
+            if (base)
+                for (int c = tid; c < F; c += NT) base[b * F + c] = 0.f;
             continue;
         }
-        const float logp = (float)(teacher_lse ? (double)s * inv_t - (double)teacher_lse[b] : d - log(mass));
-        key[tid] = valid ? ((uint64_t)id << 8) | (uint64_t)tid : ~0ull;
-        __syncthreads();
-        if (valid) {
+        // log sum exp of the student's logits and of the teacher's
+        const double log_mass = (double)row_ref * 0.69314718055994531 + log((double)row_mass);
+        double teacher = 0.0;
+        if (teacher_lse) {
+            teacher = (double)teacher_lse[b] - (double)top * inv_t;
+        } else {
+            double mass = 0.0;
+            for (int e = tid; e < kp; e += NT)
+                if (key[e] != ~0ull) mass += slogp[e] == top ? 1.0 : (double)expf((float)(((double)slogp[e] - (double)top) * inv_t));
+            teacher = log(block_sum(mass, 0));
+        }
+        for (int e = tid; e < kp; e += NT) {
+            const uint64_t mine = key[e];
+            if (mine == ~0ull) continue;
             int rank = 0;
-            const uint64_t mine = key[tid];
-            for (int j = 0; j < k; ++j) rank += key[j] < mine ? 1 : 0;
-            sid[rank] = id;
-            st[rank] = logp;
-            sp[rank] = expf(logp);
+            const ulonglong2* kv = reinterpret_cast<const ulonglong2*>(key);
+#pragma unroll 8
+            for (int j = 0; j < kp / 2; ++j) rank += (kv[j].x < mine ? 1 : 0) + (kv[j].y < mine ? 1 : 0);
+            const float s = slogp[e];
+            const float lp = (float)((s == top ? 0.0 : ((double)s - (double)top) * inv_t) - teacher);
+            sid[rank] = (int32_t)(mine >> 8);
+            mz[rank] = lp;
+            sp[rank] = expf(lp);
         }
         __syncthreads();
-        const bool head = tid < nvalid && (tid == 0 || sid[tid] != sid[tid - 1]);
-        const uint64_t votes = __ballot(head);
-        if (lane == 0) parti[wave] = __popcll(votes);
-        __syncthreads();
-        int at = __popcll(votes & ((1ull << lane) - 1)), merged = 0;
-        for (int w = 0; w < DI_THREADS / 64; ++w) {
-            at += w < wave ? parti[w] : 0;
-            merged += parti[w];
+        // entries of one item become one
+        int merged = 0;
+        for (int e0 = 0; e0 < valid; e0 += NT) {
+            const int e = e0 + tid;
+            const bool head = e < valid && (e == 0 || sid[e] != sid[e - 1]);
+            const uint64_t votes = __ballot(head);
+            int at = merged + __popcll(votes & ((1ull << lane) - 1));
+            if (NWV > 1) {
+                if (lane == 0) parti[wave] = __popcll(votes);
+                __syncthreads();
+                for (int w = 0; w < NWV; ++w) {
+                    at += w < wave ? parti[w] : 0;
+                    merged += parti[w];
+                }
+                __syncthreads();
+            } else {
+                merged += __popcll(votes);
+            }
+            if (head) {
+                float p = sp[e], lp = mz[e];
+                int j = e + 1;
+                for (; j < valid && sid[j] == sid[e]; ++j) p += sp[j];
+                if (j > e + 1) lp = logf(p);
+                mid[at] = sid[e];
+                mp[at] = p;
+                mlogp[at] = lp;
+            }
         }
-        if (head) {
-            float p = sp[tid], lp = st[tid];
-            int j = tid + 1;
-            for (; j < nvalid && sid[j] == sid[tid]; ++j) p += sp[j];
-            if (j > tid + 1) lp = logf(p);
-            mid[at] = sid[tid];
-            mp[at] = p;
-            mlogp[at] = lp;
-        }
         __syncthreads();
-        // the student's logits on the list: half a wavefront per entry
-        for (int e = tid >> 5; e < merged; e += DI_THREADS / 32) {
-            const float* y = Y + (int64_t)mid[e] * f;
-            float z = 0.f;
-            for (int c = tid & 31; c < f; c += 32) z = __builtin_fmaf(X[b * f + c], y[c], z);
+        // the student's logits on the list
+        for (int e0 = group; e0 - group < merged; e0 += 4 * ROWS) {
+            f32x2 y[4][PIECES];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
-            if ((tid & 31) == 0) mz[e] = z;
+            for (int u = 0; u < 4; ++u) {
+                const int e = e0 + u * ROWS;
+                const float* v = Y + (int64_t)mid[e < merged ? e : 0] * F + 2 * sub;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) y[u][i] = *reinterpret_cast<const f32x2*>(v + 32 * i);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int e = e0 + u * ROWS;
+                float z = 0.f;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    z = __builtin_fmaf(x[i][0], y[u][i][0], z);
+                    z = __builtin_fmaf(x[i][1], y[u][i][1], z);
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+                if (sub == 0 && e < merged) mz[e] = z;
+            }
         }
         __syncthreads();
-        const bool mine = tid < merged;
-        const double logq = mine ? (double)mz[tid] * inv_t - log_mass : 0.0;
-        const float q = mine ? expf((float)logq) : 0.f;
-        const float p = mine ? mp[tid] : 0.f;
-        // (a NaN probability stays in the sum)
-        double kl = di_block_sum(mine && !(p <= 0.f) ? (double)p * ((double)mlogp[tid] - logq) : 0.0, partd);
+        double kl = 0.0, sum_p = 0.0, sum_q = 0.0;
+        for (int e = tid; e < merged; e += NT) {
+            const double logq = (double)mz[e] * inv_t - log_mass;
+            const float p = mp[e], q = expf((float)logq);
+            if (!(p <= 0.f)) kl += (double)p * ((double)mlogp[e] - logq);   // (a NaN probability stays in the sum)
+            sum_p += (double)p;
+            sum_q += (double)q;
+            sp[e] = q;
+        }
+        kl = block_sum(kl, 0);
         float a = 1.f;
         if (teacher_lse) {
-            const double pr = fmax(1.0 - di_block_sum((double)p, partd), 0.0);
-            const double qr = fmax(1.0 - di_block_sum((double)q, partd), 0x1p-24);
+            const double pr = fmax(1.0 - block_sum(sum_p, 1), 0.0);
+            const double qr = fmax(1.0 - block_sum(sum_q, 0), 0x1p-24);
             if (pr > 0.0) {
                 kl += pr * log(pr / qr);
                 a = (float)(1.0 - pr / qr);
@@ -658,35 +787,122 @@ __global__ __launch_bounds__(DI_LIST) void distill_list_kernel(
             a_out[b] = a;
             count_out[b] = merged;
         }
-        if (mine) st[tid] = (1.f - a) * q - p;
-        if (base) {
-            if (mine) {
-                id_out[b * k + tid] = mid[tid];
-                val_out[b * k + tid] = q - p;
-            }
-            for (int64_t t = tid; t <= ytiles; t += DI_LIST) {
-                int lo = 0, hi = merged;
-                while (lo < hi) {
-                    const int c = (lo + hi) >> 1;
-                    if ((int64_t)mid[c] < t * 32) lo = c + 1;
-                    else hi = c;
-                }
-                start_out[b * (ytiles + 1) + t] = (uint16_t)lo;
-            }
-            __syncthreads();
-            if (tid < f) {
-                float acc = a * mean;
-                for (int e = 0; e < merged; ++e) acc = __builtin_fmaf(st[e], Y[(int64_t)mid[e] * f + tid], acc);
-                base[b * f + tid] = acc;
-            }
+        if (!base) continue;
+        for (int e = tid; e < merged; e += NT) {
+            id_out[b * k + e] = mid[e];
+            val_out[b * k + e] = sp[e] - mp[e];
+            mz[e] = (1.f - a) * sp[e] - mp[e];
         }
         __syncthreads();
+        // dX but for its weight: listed items and the ranges' sums under the softmax, by their coefficients
+        f32x2 sum[PIECES] = {};
+        for (int e0 = group; e0 - group < merged + ranges; e0 += 4 * ROWS) {
+            f32x2 y[4][PIECES];
+            float w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int e = e0 + u * ROWS, r = e - merged;
+                w[u] = e < merged ? mz[e] : r < ranges ? a * range_w[r] : 0.f;
+                const float* v = (e < merged ? Y + (int64_t)mid[e] * F : psum + ((r < ranges ? r : 0) * n + b) * F) + 2 * sub;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) y[u][i] = *reinterpret_cast<const f32x2*>(v + 32 * i);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool real = e0 + u * ROWS < merged + ranges;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    sum[i][0] = real ? __builtin_fmaf(w[u], y[u][i][0], sum[i][0]) : sum[i][0];
+                    sum[i][1] = real ? __builtin_fmaf(w[u], y[u][i][1], sum[i][1]) : sum[i][1];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float v = sum[i][j];
+                v += __shfl_xor(v, 16, 64);
+                v += __shfl_xor(v, 32, 64);
+                if (lane < 16) red[wave][2 * (sub + 16 * i) + j] = v;
+            }
+        __syncthreads();
+        for (int c = tid; c < F; c += NT) {
+            float v = red[0][c];
+            for (int w = 1; w < NWV; ++w) v += red[w][c];
+            base[b * F + c] = v;
+        }
     }
 }
 
-// dX, and the partial maxima of |grad| that scale the weights of the backward pass.
+// One workgroup per tile of 32 rows: their merged lists' entries grouped by item tile, (row in the tile, column in the
+// item tile, q - p) each, and where every item tile's group begins.  A group's order does not matter: its entries are
+// different places of one 32 x 32 block.  Item tiles are counted in LDS, DI_BINS at a time.
+__global__ __launch_bounds__(DI_GROUP_THREADS) void distill_group_kernel(const int32_t* __restrict__ count,
+                                                                   const int32_t* __restrict__ list_id,
+                                                                   const float* __restrict__ list_val, int64_t n, int k,
+                                                                   int64_t ytiles, uint16_t* __restrict__ start,
+                                                                   uint16_t* __restrict__ place, float* __restrict__ val) {
+    __shared__ int32_t bins[DI_BINS];
+    __shared__ int32_t part[DI_GROUP_THREADS / 64];
+    constexpr int PER = DI_BINS / DI_GROUP_THREADS;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t tile = blockIdx.x, row0 = tile * 32;
+    const int rows = (int)(n - row0 < 32 ? n - row0 : 32);
+    uint16_t* tile_start = start + tile * (ytiles + 1);
+    int base = 0;
+    for (int64_t t0 = 0; t0 < ytiles; t0 += DI_BINS) {
+        for (int i = tid; i < DI_BINS; i += DI_GROUP_THREADS) bins[i] = 0;
+        __syncthreads();
+        for (int e = tid; e < rows * k; e += DI_GROUP_THREADS)
+            if (e % k < count[row0 + e / k]) {
+                const int64_t t = list_id[row0 * k + e] / 32 - t0;
+                if (t >= 0 && t < DI_BINS) atomicAdd(&bins[t], 1);
+            }
+        __syncthreads();
+        int sum = 0;
+        for (int i = 0; i < PER; ++i) sum += bins[tid * PER + i];
+        int inc = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(inc, d, 64);
+            inc += lane >= d ? o : 0;
+        }
+        if (lane == 63) part[wave] = inc;
+        __syncthreads();
+        int at = base + inc - sum;
+        for (int w = 0; w < DI_GROUP_THREADS / 64; ++w) {
+            at += w < wave ? part[w] : 0;
+            base += part[w];
+        }
+        for (int i = 0; i < PER; ++i) {
+            const int c = bins[tid * PER + i];
+            bins[tid * PER + i] = at;
+            if (t0 + tid * PER + i < ytiles) tile_start[t0 + tid * PER + i] = (uint16_t)at;
+            at += c;
+        }
+        __syncthreads();
+        for (int e = tid; e < rows * k; e += DI_GROUP_THREADS)
+            if (e % k < count[row0 + e / k]) {
+                const int32_t id = list_id[row0 * k + e];
+                const int64_t t = id / 32 - t0;
+                if (t >= 0 && t < DI_BINS) {
+                    const int64_t to = row0 * k + atomicAdd(&bins[t], 1);
+                    place[to] = (uint16_t)(e / k * 32 + (id & 31));
+                    val[to] = list_val[row0 * k + e];
+                }
+            }
+        __syncthreads();
+    }
+    if (tid == 0) tile_start[ytiles] = (uint16_t)base;
+}
+
+// dX; what a row brings to the backward pass (the reference of its logits, the weight of a probability and that of a
+// list entry); the partial maxima of |grad| that scale those weights.
 __global__ __launch_bounds__(DI_THREADS) void distill_dx_kernel(const float* __restrict__ base, const float* __restrict__ grad,
                                                                 float temperature, int64_t n, int f, float* __restrict__ dX,
+                                                                const float* __restrict__ ref, const float* __restrict__ mass,
+                                                                const float* __restrict__ a, f32x4* __restrict__ rows,
                                                                 uint32_t* __restrict__ parts) {
     __shared__ uint32_t part[DI_THREADS / 64];
     uint32_t top = 0;
@@ -696,7 +912,9 @@ __global__ __launch_bounds__(DI_THREADS) void distill_dx_kernel(const float* __r
             *reinterpret_cast<f32x4*>(dX + e) = *reinterpret_cast<const f32x4*>(base + e) * g;
         }
     for (int64_t b = (int64_t)blockIdx.x * DI_THREADS + threadIdx.x; b < n; b += (int64_t)DI_PARTS * DI_THREADS) {
-        const uint32_t u = __float_as_uint(grad[b]) & 0x7fffffffu;
+        const float g = grad[b];
+        rows[b] = f32x4{-ref[b], g * (a[b] / mass[b]), g, 0.f};
+        const uint32_t u = __float_as_uint(g) & 0x7fffffffu;
         top = u > top ? u : top;
     }
 #pragma unroll
@@ -752,8 +970,10 @@ static int distill_lds(const void* kernel, int bytes, OncePerDevice& once, const
 }
 
 template <int F, bool GRAD>
-static int launch_forward(const DistillWorkspace& L, char* w, const float* X, int64_t n, const float* Y, int64_t m, float step,
-                          hipStream_t stream) {
+static int launch_forward(const DistillWorkspace& L, char* w, const float* X, int64_t n, const float* Y, int64_t m,
+                          const int32_t* ids, const float* scores, int k, float temperature, const float* teacher_lse,
+                          float* loss, hipStream_t stream) {
+    const float step = (float)(1.4426950408889634 / (double)temperature);
     static OncePerDevice once;
     constexpr int LDS = 2 * DistillTile<F>::BYTES;
     if (const int rc = distill_lds((const void*)distill_forward_kernel<F, GRAD>, LDS, once, "mirec_distill_loss")) return rc;
@@ -767,28 +987,39 @@ static int launch_forward(const DistillWorkspace& L, char* w, const float* X, in
                        w + L.ximg_off, n, blocks, w + L.yimg_off, m, L.ytiles, per, step, parts, (float*)(w + L.pref_off),
                        (float*)(w + L.pmass_off), (float*)(w + L.part_off));
     MIREC_LAUNCH_CHECK();
+    const int nt = n >= DI_MANY_ROWS ? 64 : 256;
+    hipLaunchKernelGGL(nt == 64 ? (distill_list_kernel<F, 64>) : (distill_list_kernel<F, 256>),
+                       dim3((unsigned)(n < 262144 ? n : 262144)), dim3(nt), (size_t)((k + 63) & ~63) * 28, stream, X, n, Y, m,
+                       ids, scores, k, temperature, teacher_lse, (int)ranges, (const float*)(w + L.pref_off),
+                       (const float*)(w + L.pmass_off), (const float*)(w + L.part_off), parts, loss, (float*)(w + L.ref_off),
+                       (float*)(w + L.mass_off), (float*)(w + L.a_off), (int32_t*)(w + L.count_off), (int32_t*)(w + L.id_off),
+                       (float*)(w + L.val_off), GRAD ? (float*)(w + L.base_off) : nullptr);
+    MIREC_LAUNCH_CHECK();
+    if (GRAD) {
+        hipLaunchKernelGGL(distill_group_kernel, dim3((unsigned)L.xtiles), dim3(DI_GROUP_THREADS), 0, stream,
+                           (const int32_t*)(w + L.count_off), (const int32_t*)(w + L.id_off), (const float*)(w + L.val_off), n, k,
+                           L.ytiles, (uint16_t*)(w + L.start_off), (uint16_t*)(w + L.place_off), (float*)(w + L.gval_off));
+        MIREC_LAUNCH_CHECK();
+    }
     return MIREC_OK;
 }
 
 template <int F>
 static int launch_backward(const DistillWorkspace& L, char* w, int64_t n, int64_t m, int k, float step, float temperature,
-                           const float* grad, float* dY, hipStream_t stream) {
+                           float* dY, hipStream_t stream) {
     static OncePerDevice once;
-    constexpr int LDS = 2 * DistillTile<F>::BYTES;
+    constexpr int LDS = 2 * DistillTile<F>::BYTES + DI_NW * (64 * 20 + 64) * 4;
     if (const int rc = distill_lds((const void*)distill_backward_kernel<F>, LDS, once, "mirec_distill_grad")) return rc;
-    const int64_t blocks = (m + DI_OWN - 1) / DI_OWN, per = (L.xtiles + L.splits_y - 1) / L.splits_y;
-    const int64_t ranges = (L.xtiles + per - 1) / per;
-    float* out = ranges > 1 ? (float*)(w + L.part_off) : dY;
-    hipLaunchKernelGGL((distill_backward_kernel<F>), dim3((unsigned)(blocks * ranges)), dim3(64 * DI_NW), LDS, stream,
-                       w + L.yimg_off, m, blocks, w + L.ximg_off, n, L.xtiles, per, step, temperature,
-                       (const uint32_t*)(w + L.max_off), (const float*)(w + L.ref_off), (const float*)(w + L.mass_off),
-                       (const float*)(w + L.a_off), grad, (const uint16_t*)(w + L.start_off), L.ytiles,
-                       (const int32_t*)(w + L.id_off), (const float*)(w + L.val_off), k, out);
+    const int64_t blocks = (m + DI_OWN - 1) / DI_OWN, steps = blocks * L.xtiles;
+    float* slots = (float*)(w + L.part_off);
+    hipLaunchKernelGGL((distill_backward_kernel<F>), dim3((unsigned)L.runs), dim3(64 * DI_NW), LDS, stream, w + L.yimg_off, m,
+                       steps, w + L.ximg_off, n, L.xtiles, step, temperature, (const uint32_t*)(w + L.max_off),
+                       (const f32x4*)(w + L.row_off), (const uint16_t*)(w + L.start_off), L.ytiles,
+                       (const uint16_t*)(w + L.place_off), (const float*)(w + L.gval_off), k, dY, slots);
     MIREC_LAUNCH_CHECK();
-    if (ranges > 1) {
-        const int64_t jb = (m * F / 4 + DI_THREADS - 1) / DI_THREADS;
-        hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)(jb < 4096 ? jb : 4096)), dim3(DI_THREADS), 0, stream, out,
-                           (int)ranges, m * F, dY);
+    if (L.runs > 1) {
+        hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)(L.runs - 1), (F / 32) * 4), dim3(DI_THREADS), 0, stream, slots, steps,
+                           L.runs, L.xtiles, m, F, dY);
         MIREC_LAUNCH_CHECK();
     }
     return MIREC_OK;
@@ -814,25 +1045,17 @@ extern "C" int mirec_distill_loss(const float* X, int64_t n, const float* Y, int
     const DistillWorkspace L = distill_layout(n, m, f, k);
     if (const int rc = distill_check_ws("mirec_distill_loss", ws, ws_bytes, L.bytes)) return rc;
     char* w = (char*)ws;
-    const float step = (float)(1.4426950408889634 / (double)temperature);
-    hipLaunchKernelGGL(distill_absmax_kernel, dim3(DI_PARTS, 2), dim3(DI_THREADS), 0, stream, X, n * f, Y, m * f,
+    hipLaunchKernelGGL(distill_absmax_kernel, dim3(DI_PARTS, 2), dim3(DI_MAX_THREADS), 0, stream, X, n * f, Y, m * f,
                        (uint32_t*)(w + L.max_off));
     MIREC_LAUNCH_CHECK();
-    int rc = MIREC_OK;
     switch (f) {
-#define MIREC_DISTILL_CASE(FW)                                                                                  case FW:                                                                                                        rc = with_grad ? launch_forward<FW, true>(L, w, X, n, Y, m, step, stream)                                                  : launch_forward<FW, false>(L, w, X, n, Y, m, step, stream);                                 break;
+#define MIREC_DISTILL_CASE(FW)                                                                                          \
+    case FW:                                                                                                            \
+        return with_grad ? launch_forward<FW, true>(L, w, X, n, Y, m, ids, scores, k, temperature, teacher_lse, loss, stream) \
+                         : launch_forward<FW, false>(L, w, X, n, Y, m, ids, scores, k, temperature, teacher_lse, loss, stream);
         MIREC_DISTILL_WIDTHS(MIREC_DISTILL_CASE)
 #undef MIREC_DISTILL_CASE
     }
-    if (rc) return rc;
-    const int64_t per = (L.ytiles + L.splits_x - 1) / L.splits_x;
-    hipLaunchKernelGGL(distill_list_kernel, dim3((unsigned)(n < 262144 ? n : 262144)), dim3(DI_LIST), 0, stream, X, n, Y, m, f,
-                       ids, scores, k, temperature, teacher_lse, (int)((L.ytiles + per - 1) / per),
-                       (const float*)(w + L.pref_off), (const float*)(w + L.pmass_off), (const float*)(w + L.part_off),
-                       (const uint32_t*)(w + L.max_off), loss, (float*)(w + L.ref_off), (float*)(w + L.mass_off),
-                       (float*)(w + L.a_off), (int32_t*)(w + L.count_off), (int32_t*)(w + L.id_off), (float*)(w + L.val_off),
-                       (uint16_t*)(w + L.start_off), with_grad ? (float*)(w + L.base_off) : nullptr);
-    MIREC_LAUNCH_CHECK();
     return MIREC_OK;
 }
 
@@ -856,14 +1079,15 @@ extern "C" int mirec_distill_grad(const float* X, int64_t n, const float* Y, int
     if (const int rc = distill_check_ws("mirec_distill_grad", ws, ws_bytes, L.bytes)) return rc;
     char* w = (char*)ws;
     hipLaunchKernelGGL(distill_dx_kernel, dim3(DI_PARTS), dim3(DI_THREADS), 0, stream, (const float*)(w + L.base_off), grad,
-                       temperature, n, f, dX, (uint32_t*)(w + L.max_off) + 2 * DI_PARTS);
+                       temperature, n, f, dX, (const float*)(w + L.ref_off), (const float*)(w + L.mass_off),
+                       (const float*)(w + L.a_off), (f32x4*)(w + L.row_off), (uint32_t*)(w + L.max_off) + 2 * DI_PARTS);
     MIREC_LAUNCH_CHECK();
     if (!dY) return MIREC_OK;
     const float step = (float)(1.4426950408889634 / (double)temperature);
     switch (f) {
 #define MIREC_DISTILL_CASE(FW) \
     case FW:                   \
-        return launch_backward<FW>(L, w, n, m, k, step, temperature, grad, dY, stream);
+        return launch_backward<FW>(L, w, n, m, k, step, temperature, dY, stream);
         MIREC_DISTILL_WIDTHS(MIREC_DISTILL_CASE)
 #undef MIREC_DISTILL_CASE
     }
