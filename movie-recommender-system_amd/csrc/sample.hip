@@ -9,20 +9,24 @@
 // are formed in, so a histogram by atomics, a split row and a scan give the same bits on every run, and a running sum
 // of 27 000 weights is exact where fp32 would move its borders by more than the width of an unlikely item.
 #include <float.h>
-#include <hip/hip_fp16.h>
+
+#include <type_traits>
 
 #include "common.h"
 
 namespace mirec {
 
-constexpr int SM_THREADS = 256;
 constexpr int SM_MAX_DRAWS = MIREC_SAMPLE_MAX_DRAWS;
 constexpr int64_t SM_MAX_MASKED_ITEMS = MIREC_SAMPLE_MAX_MASKED_ITEMS;   // the filter of a row is a bitmap in LDS
 constexpr double SM_MIN_TEMPERATURE = 1e-37;      // below: greedy
+constexpr int SM_SHORT = 256;                     // rows up to this length: one wavefront each
+constexpr int SM_BINS = 1024;                     // of a histogram over a row
+constexpr int SM_LIST = 512;                     // entries that are ranked against each other in LDS
 
 struct SampleParams {
-    double temperature, top_p, min_p;
+    double step, top_p, min_p;   // step: log2 e / temperature
     int32_t top_k;
+    bool greedy;
     const float* row_temperature;
     const int32_t* row_top_k;
     const float* row_top_p;
@@ -70,7 +74,7 @@ __device__ __forceinline__ uint64_t sm_weight(double t, int bits) {
     const double k = rint(t);
     const double f = t - k;
     double p = 7.054911620801121e-09;                 // ln2^10 / 10!
-    p = __builtin_fma(p, f, 1.0178086009239696e-07);   // ln2^9 / 9!
+    p = __builtin_fma(p, f, 1.0178086009239696e-07);  // ln2^9 / 9!
     p = __builtin_fma(p, f, 1.3215486790144305e-06);
     p = __builtin_fma(p, f, 1.5252733804059838e-05);
     p = __builtin_fma(p, f, 1.5403530393381606e-04);
@@ -84,276 +88,668 @@ __device__ __forceinline__ uint64_t sm_weight(double t, int bits) {
     return (uint64_t)__double_as_longlong(v) & 0xfffffffffffffull;
 }
 
-__device__ __forceinline__ uint64_t sm_shfl_xor(uint64_t v, int m) {
-    return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), m, 64) << 32) | (uint32_t)__shfl_xor((int)v, m, 64);
-}
+// ---- 64-bit sums over a wavefront, by data-parallel moves between lanes (no LDS)
 
-__device__ __forceinline__ uint64_t sm_shfl_up(uint64_t v, int d) {
-    return ((uint64_t)(uint32_t)__shfl_up((int)(v >> 32), d, 64) << 32) | (uint32_t)__shfl_up((int)v, d, 64);
-}
-
-__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += sm_shfl_xor(v, m);
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t sm_moved(uint64_t v) {   // 0 where no lane is moved from
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return ((uint64_t)hi << 32) | lo;
 }
 
 __device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {   // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = sm_shfl_up(v, d);
-        v += lane >= d ? o : 0ull;
-    }
+    v += sm_moved<0x111, 0xf>(v);   // shifted by 1, 2, 4, 8 within rows of 16 lanes
+    v += sm_moved<0x112, 0xf>(v);
+    v += sm_moved<0x114, 0xf>(v);
+    v += sm_moved<0x118, 0xf>(v);
+    v += sm_moved<0x142, 0xa>(v);   // lane 15 of a row to the next row: rows 1 and 3
+    v += sm_moved<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
     return v;
 }
 
-// One workgroup per row; the row is read again for every step (max, one histogram per byte of the key and per cut, the
-// kept mass, the draws).
-template <int DT>
-__global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(
-    const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,
-    const int32_t* __restrict__ ids, int64_t ids_stride, const int64_t* __restrict__ mask_indptr,
-    const int32_t* __restrict__ mask_indices, const float* __restrict__ uniforms, int draws, int replacement,
-    SampleParams par, int bits, int32_t* __restrict__ out_ids, float* __restrict__ out_logprob) {
-    extern __shared__ uint32_t liked[];   // one bit per item, when there is a filter
-    __shared__ uint64_t hist[256];
-    __shared__ uint64_t part[SM_THREADS / 64];
-    __shared__ uint32_t part32[SM_THREADS / 64];
-    __shared__ uint64_t bcast[2];
-    __shared__ int64_t drawn[SM_MAX_DRAWS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
 
-    for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_lane(sm_wave_scan(v), 63); }
+
+// Where a number of [0, 1) falls in a total: floor(u * total), u moved into [0, 1 - 2^-53].
+__device__ __forceinline__ uint64_t sm_target(float u, uint64_t total) {
+    const double uc = u > 0.f ? fmin((double)u, 1.0 - 0x1p-53) : 0.0;
+    return __umul64hi(total, (uint64_t)(uc * 0x1p53) << 11);
+}
+
+// What the cuts and the temperature of one row come to.
+struct RowCuts {
+    int64_t top_k;
+    double top_p, floor_w, step;   // step: log2 e / temperature
+};
+
+__device__ __forceinline__ RowCuts sm_cuts(const SampleParams& par, int64_t row, int64_t m, int bits) {
+    RowCuts c;
+    c.step = par.step;
+    bool greedy = par.greedy;
+    if (par.row_temperature) {
+        const double T = (double)par.row_temperature[row];
+        greedy = !(T >= SM_MIN_TEMPERATURE);
+        c.step = greedy ? 0.0 : 1.4426950408889634 / T;
+    }
+    c.top_p = par.row_top_p ? (double)par.row_top_p[row] : par.top_p;
+    const double min_p = par.row_min_p ? (double)par.row_min_p[row] : par.min_p;
+    c.top_k = par.row_top_k ? par.row_top_k[row] : par.top_k;
+    if (c.top_k <= 0 || c.top_k > m) c.top_k = m;
+    if (greedy) c.top_k = 1;
+    c.floor_w = min_p > 0.0 ? fmin(min_p, 1.0) * (double)(1ull << bits) : 0.0;
+    return c;
+}
+
+// log2 of a weight before rounding, from the key of its item and the row's best.
+__device__ __forceinline__ double sm_exponent(uint32_t key, uint32_t top, double best, double step) {
+    return key == top ? 0.0 : ((double)sm_unorder(key) - best) * step;
+}
+
+__device__ __forceinline__ float sm_logprob(double exponent, uint64_t total, int bits) {
+    return (float)(exponent * 0.69314718055994531 - log(ldexp((double)total, -bits)));
+}
+
+// ------------------------------------------------------------------------------------------------------ short rows
+
+// One wavefront per row of at most 64 E items, all of it in registers: item 64 j + l in lane l.  A ranked list is in
+// order already (one comparison of neighbours says so), and then the running sum in index order is the running sum in
+// rank order too: one scan serves the cuts and the draws.  Otherwise every item is compared with every other.
+template <int DT, int E>
+__global__ __launch_bounds__(256) void sample_short_kernel(
+    const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int m, int64_t stride, const int32_t* __restrict__ ids,
+    int64_t ids_stride, const int64_t* __restrict__ mask_indptr, const int32_t* __restrict__ mask_indices,
+    const float* __restrict__ uniforms, int draws, int replacement, SampleParams par, int bits,
+    int32_t* __restrict__ out_ids, float* __restrict__ out_logprob) {
+    const int lane = threadIdx.x & 63;
+    const int64_t waves = (int64_t)gridDim.x * 4;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < n; row += waves) {
         const typename ScoreType<DT>::raw* s = scores + row * stride;
-        const int32_t* id = ids ? ids + row * ids_stride : nullptr;
-        __syncthreads();
-        if (mask_indptr) {
-            for (int64_t w = tid; w < (m + 31) / 32; w += SM_THREADS) liked[w] = 0;
-            __syncthreads();
-            for (int64_t e = mask_indptr[row] + tid; e < mask_indptr[row + 1]; e += SM_THREADS) {
-                const int64_t it = mask_indices[e];
-                if (it >= 0 && it < m) atomicOr(&liked[it >> 5], 1u << (it & 31));
+        float value[E];
+        int32_t id[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int i = 64 * j + lane;
+            value[j] = i < m ? ScoreType<DT>::widen(s[i]) : -INFINITY;
+            id[j] = ids && i < m ? ids[row * ids_stride + i] : i;
+        }
+        uint32_t key[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) key[j] = value[j] > ScoreType<DT>::lowest && id[j] >= 0 ? sm_order(value[j]) : 0u;
+        if (mask_indptr) {   // each lane looks for its items in the row's filter
+            for (int64_t e = mask_indptr[row]; e < mask_indptr[row + 1]; ++e) {
+                const int32_t it = mask_indices[e];
+#pragma unroll
+                for (int j = 0; j < E; ++j) key[j] = it == 64 * j + lane ? 0u : key[j];
             }
-            __syncthreads();
         }
-        auto key_of = [&](int64_t i) -> uint32_t {
-            const float v = ScoreType<DT>::widen(s[i]);
-            bool ok = v > ScoreType<DT>::lowest;
-            if (mask_indptr) ok = ok && !((liked[i >> 5] >> (i & 31)) & 1u);
-            if (id) ok = ok && id[i] >= 0;
-            return ok ? sm_order(v) : 0u;
-        };
-        auto block_sum = [&](uint64_t v) -> uint64_t {
-            v = sm_wave_sum(v);
-            __syncthreads();
-            if (lane == 0) part[wave] = v;
-            __syncthreads();
-            uint64_t t = 0;
-            for (int w = 0; w < SM_THREADS / 64; ++w) t += part[w];
-            return t;
-        };
-
-        // the best score
-        uint32_t top = 0;
-        for (int64_t i = tid; i < m; i += SM_THREADS) {
-            const uint32_t k = key_of(i);
-            top = k > top ? k : top;
-        }
+        uint32_t top = key[0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) top = key[j] > top ? key[j] : top;
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) {
             const uint32_t o = (uint32_t)__shfl_xor((int)top, d, 64);
             top = o > top ? o : top;
         }
+        top = (uint32_t)__builtin_amdgcn_readfirstlane((int)top);
+        const RowCuts cut = sm_cuts(par, row, m, bits);
+        const double best = (double)sm_unorder(top);
+        uint64_t w[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) w[j] = key[j] ? sm_weight(sm_exponent(key[j], top, best, cut.step), bits) : 0ull;
+
+        bool ordered = true;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            uint32_t next = (uint32_t)__shfl_down((int)key[j], 1, 64);
+            if (lane == 63) next = 0;
+            ordered = ordered && key[j] >= next;
+            if (j + 1 < E) ordered = ordered && (lane < 63 || key[j] >= (uint32_t)__builtin_amdgcn_readlane((int)key[j + 1], 0));
+        }
+        uint64_t run[E];   // sum of the kept weights up to and with the item
+        uint64_t total = 0;
+        if (__all(ordered)) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                if (64 * j + lane >= cut.top_k) w[j] = 0;
+                run[j] = total + sm_wave_scan(w[j]);
+                total = sm_lane(run[j], 63);
+            }
+            if (cut.top_p < 1.0 || cut.floor_w > 0.0) {
+                const double bound = cut.top_p < 1.0 ? cut.top_p * (double)total : INFINITY;
+                uint64_t kept = 0;   // a prefix stays: the running sum at its end
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const bool stays = (64 * j + lane == 0 || (double)(run[j] - w[j]) < bound) && (double)w[j] >= cut.floor_w;
+                    if (!stays) w[j] = 0;
+                    const uint64_t votes = __ballot(stays && w[j] != 0);
+                    if (votes) kept = sm_lane(run[j], 63 - __builtin_clzll(votes));
+                }
+                total = kept;
+#pragma unroll
+                for (int j = 0; j < E; ++j) run[j] = run[j] < total ? run[j] : total;
+            }
+        } else {
+            uint32_t rank[E];
+            uint64_t before[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                rank[j] = 0;
+                before[j] = 0;
+            }
+            if (cut.top_k < m || cut.top_p < 1.0) {
+#pragma unroll
+                for (int q = 0; q < E; ++q)
+                    for (int l = 0; l < 64 && 64 * q + l < m; ++l) {
+                        const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key[q], l);
+                        const uint64_t kw = sm_lane(w[q], l);
+#pragma unroll
+                        for (int j = 0; j < E; ++j) {
+                            const bool ahead = k > key[j] || (k == key[j] && 64 * q + l < 64 * j + lane);
+                            rank[j] += ahead ? 1u : 0u;
+                            before[j] += ahead ? kw : 0ull;
+                        }
+                    }
+            }
+            uint64_t mass = 0;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                if (rank[j] >= cut.top_k) w[j] = 0;
+                mass += w[j];
+            }
+            const double bound = cut.top_p < 1.0 ? cut.top_p * (double)sm_wave_sum(mass) : INFINITY;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                if (!((rank[j] == 0 || (double)before[j] < bound) && (double)w[j] >= cut.floor_w)) w[j] = 0;
+                run[j] = total + sm_wave_scan(w[j]);
+                total = sm_lane(run[j], 63);
+            }
+        }
+
+        for (int d0 = 0; d0 < draws; d0 += 64) {
+            const int cnt = draws - d0 < 64 ? draws - d0 : 64;
+            const float u = lane < cnt ? uniforms[row * draws + d0 + lane] : 0.f;
+            int32_t got = -1;
+            uint32_t got_key = 0;
+            uint64_t got_total = 1;
+            for (int d = 0; d < cnt && total > 0; ++d) {
+                const uint64_t t = sm_target(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(u), d)), total);
+                bool found = false;
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const uint64_t votes = __ballot(run[j] > t);
+                    if (!found && votes) {
+                        found = true;
+                        const int l = __builtin_ctzll(votes);
+                        if (lane == d) {
+                            got_key = 0;   // below
+                            got_total = total;
+                        }
+                        const int32_t item = __builtin_amdgcn_readlane(id[j], l);
+                        const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key[j], l);
+                        if (lane == d) {
+                            got = item;
+                            got_key = k;
+                        }
+                        if (!replacement) {   // the item leaves: every running sum from it on is lower by its weight
+                            const uint64_t gone = sm_lane(w[j], l);
+                            if (lane == l) w[j] = 0;
+                            total -= gone;
+#pragma unroll
+                            for (int q = 0; q < E; ++q) run[q] -= 64 * q + lane >= 64 * j + l ? gone : 0ull;
+                        }
+                    }
+                }
+            }
+            if (lane < cnt) {
+                out_ids[row * draws + d0 + lane] = got;
+                out_logprob[row * draws + d0 + lane] =
+                    got >= 0 ? sm_logprob(sm_exponent(got_key, top, best, cut.step), got_total, bits) : -INFINITY;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- long rows
+
+// Scores of 16 bytes, from any address that is aligned to their type.
+typedef uint32_t sm_words __attribute__((ext_vector_type(4), aligned(2)));
+
+typedef uint32_t sm_held __attribute__((ext_vector_type(32)));   // eight chunks
+
+template <int DT>
+struct Chunk {
+    static constexpr int V = DT == MIREC_F32 ? 4 : 8;   // scores of a thread's 16 bytes
+    uint32_t word[4];
+    __device__ __forceinline__ float value(int v) const {
+        if constexpr (DT == MIREC_F32)
+            return __uint_as_float(word[v]);
+        else if constexpr (DT == MIREC_BF16)
+            return __uint_as_float(v & 1 ? word[v >> 1] & 0xffff0000u : word[v >> 1] << 16);
+        else
+            return (float)__builtin_bit_cast(_Float16, (uint16_t)(word[v >> 1] >> (16 * (v & 1))));
+    }
+    __device__ __forceinline__ uint32_t key(int v) const {
+        const float f = value(v);
+        return f > ScoreType<DT>::lowest ? sm_order(f) : 0u;
+    }
+    __device__ __forceinline__ void exclude(int v) {   // minus infinity
+        if constexpr (DT == MIREC_F32) word[v] = 0xff800000u;
+        else {
+            const uint32_t inf = DT == MIREC_BF16 ? 0xff80u : 0xfc00u;
+            word[v >> 1] = v & 1 ? (word[v >> 1] & 0xffffu) | (inf << 16) : (word[v >> 1] & 0xffff0000u) | inf;
+        }
+    }
+};
+
+// One workgroup of NT threads per row.  The row is cut into pieces of S chunks, a chunk is 16 bytes per lane; piece g NW + w
+// belongs to wavefront w, so pieces, chunks and lanes are in index order.  CH > 0: a wavefront's CH pieces (S = 1) stay in
+// its registers; CH = 0: each pass reads the row again, S makes at most SM_BINS pieces of it.
+//
+// A cut is a number: with K = (key, complemented index) larger for a better item, what is kept is K >= cut.  It is found
+// by a histogram whose bins are ordered like the items -- first by the score's distance from the best, in 1/32 octaves
+// of the weight, then, should a bin hold more than SM_LIST items, by equal ranges of K -- and by ranking the items of
+// the bin that the border falls into against each other.
+template <int DT, int NT, int CH>
+__global__ __launch_bounds__(NT, 4) void sample_long_kernel(
+    const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,
+    const int32_t* __restrict__ ids, int64_t ids_stride, const int64_t* __restrict__ mask_indptr,
+    const int32_t* __restrict__ mask_indices, const float* __restrict__ uniforms, int draws, int replacement,
+    SampleParams par, int bits, int32_t* __restrict__ out_ids, float* __restrict__ out_logprob) {
+    typedef Chunk<DT> C;
+    constexpr int V = C::V, NW = NT / 64, WAVE_CHUNK = 64 * V;
+    constexpr int BINS_PER = SM_BINS / NT;
+    constexpr int HELD = CH / 8;          // registers that hold the row, by 32
+    extern __shared__ uint32_t liked[];   // one bit per item, when there is a filter
+    __shared__ __attribute__((aligned(16))) ulonglong2 list[SM_LIST];   // K and weight
+    __shared__ uint64_t mass_bins[SM_BINS];
+    __shared__ uint32_t count_bins[SM_BINS];
+    __shared__ uint64_t part[2][NW];
+    __shared__ uint64_t shared_key[2];
+    __shared__ uint32_t shared_int[2];
+    __shared__ int32_t gone[SM_MAX_DRAWS];   // items drawn so far, when they do not come back
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t row_chunks = (m + WAVE_CHUNK - 1) / WAVE_CHUNK;
+    const int S = CH > 0 ? 1 : (int)((row_chunks + SM_BINS - 1) / SM_BINS);
+    const int pieces = (int)((row_chunks + S - 1) / S);   // at most SM_BINS
+
+    auto block_sum = [&](uint64_t v) -> uint64_t {
+        v = sm_wave_sum(v);
+        if (lane == 0) part[1][wave] = v;
         __syncthreads();
-        if (lane == 0) part32[wave] = top;
+        v = part[1][0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += part[1][w];
         __syncthreads();
-        for (int w = 0; w < SM_THREADS / 64; ++w) top = part32[w] > top ? part32[w] : top;
+        return v;
+    };
+
+    for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+        const typename ScoreType<DT>::raw* s = scores + row * stride;
+        const int32_t* id = ids ? ids + row * ids_stride : nullptr;
+        __syncthreads();   // the row before is done with the shared arrays
+        if (mask_indptr) {
+            for (int64_t w = tid; w < (m + 31) / 32; w += NT) liked[w] = 0;
+            __syncthreads();
+            for (int64_t e = mask_indptr[row] + tid; e < mask_indptr[row + 1]; e += NT) {
+                const int64_t it = mask_indices[e];
+                if (it >= 0 && it < m) atomicOr(&liked[it >> 5], 1u << (it & 31));
+            }
+            __syncthreads();
+        }
+        // a lane's first item of chunk `sub` of piece p
+        auto first_item = [&](int p, int sub) -> int64_t { return ((int64_t)p * S + sub) * WAVE_CHUNK + lane * V; };
+        // its 16 bytes; what is excluded or behind the row's end is minus infinity
+        auto load = [&](int p, int sub) -> C {
+            const int64_t i = first_item(p, sub);
+            C q;
+            if (i + V <= m) {
+                const sm_words x = *reinterpret_cast<const sm_words*>(s + i);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) q.word[v] = x[v];
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) q.word[v] = DT == MIREC_F32 ? 0xff800000u : DT == MIREC_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (i + v < m) {
+                        if constexpr (DT == MIREC_F32) q.word[v] = __float_as_uint(s[i + v]);
+                        else {
+                            const uint32_t raw = __builtin_bit_cast(uint16_t, s[i + v]);
+                            q.word[v >> 1] = v & 1 ? (q.word[v >> 1] & 0xffffu) | (raw << 16) : (q.word[v >> 1] & 0xffff0000u) | raw;
+                        }
+                    }
+            }
+            if (mask_indptr && i < m) {
+                const uint32_t out = liked[i >> 5] >> (i & 31);
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if ((out >> v) & 1u) q.exclude(v);
+            }
+            if (id) {
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (i + v < m && id[i + v] < 0) q.exclude(v);
+            }
+            return q;
+        };
+        // The row's chunks in registers, taken out one at a time by a number that is the same in all lanes: the passes are
+        // loops over the chunks, and not CH copies of their body (which neither fit the instruction cache nor, with what
+        // the compiler then carries from copy to copy, the registers).
+        sm_held held[HELD > 0 ? HELD : 1];
+        if constexpr (CH > 0) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const C q = load(c * NW + wave, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) held[c / 8][c % 8 * 4 + i] = q.word[i];
+            }
+        }
+        // f(chunk, the lane's first item, its piece, number within the piece) for every chunk of this wavefront, in order
+        auto each = [&](auto&& f) {
+            if constexpr (CH > 0) {
+#pragma unroll
+                for (int h = 0; h < HELD; ++h)
+#pragma nounroll
+                    for (int c = 0; c < 8 && (h * 8 + c) * NW + wave < pieces; ++c) {
+                        C q;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q.word[i] = held[h][c * 4 + i];
+                        f(q, first_item((h * 8 + c) * NW + wave, 0), (h * 8 + c) * NW + wave, 0);
+                    }
+            } else {
+#pragma nounroll
+                for (int p = wave; p < pieces; p += NW)
+                    for (int sub = 0; sub < S; ++sub) f(load(p, sub), first_item(p, sub), p, sub);
+            }
+        };
+        auto order_of = [&](uint32_t key, int64_t first, int v) -> uint64_t {
+            return ((uint64_t)key << 32) | (0xffffffffu - (uint32_t)(first + v));
+        };
+
+        // the best score
+        uint32_t top = 0;
+        each([&](const C& q, int64_t, int, int) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const uint32_t k = q.key(v);
+                top = k > top ? k : top;
+            }
+        });
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            const uint32_t o = (uint32_t)__shfl_xor((int)top, d, 64);
+            top = o > top ? o : top;
+        }
+        if (lane == 0) part[0][wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) top = (uint32_t)part[0][w] > top ? (uint32_t)part[0][w] : top;
+        __syncthreads();
         if (top == 0) {
-            for (int d = tid; d < draws; d += SM_THREADS) {
+            for (int d = tid; d < draws; d += NT) {
                 out_ids[row * draws + d] = -1;
                 out_logprob[row * draws + d] = -INFINITY;
             }
             continue;
         }
-
-        const double T = par.row_temperature ? (double)par.row_temperature[row] : par.temperature;
-        const double top_p = par.row_top_p ? (double)par.row_top_p[row] : par.top_p;
-        const double min_p = par.row_min_p ? (double)par.row_min_p[row] : par.min_p;
-        int64_t top_k = par.row_top_k ? par.row_top_k[row] : par.top_k;
-        const bool greedy = !(T >= SM_MIN_TEMPERATURE);
-        if (top_k <= 0 || top_k > m) top_k = m;
-        if (greedy) top_k = 1;
-        const double step = greedy ? 0.0 : 1.4426950408889634 / T;
-        const double best = (double)sm_unorder(top);
-        auto exponent = [&](uint32_t k) -> double { return k == top ? 0.0 : ((double)sm_unorder(k) - best) * step; };
-        auto weight = [&](uint32_t k) -> uint64_t { return sm_weight(exponent(k), bits); };
-
-        // `cut` is the last key kept, `ties` how many of the items that have it
-        uint32_t cut = 1;
-        int64_t ties = m;
-        if (top_k < m) {
-            uint32_t prefix = 0, known = 0;
-            uint64_t above = 0;   // items in buckets above the current one
-            bool all = false;
-            for (int shift = 24; shift >= 0 && !all; shift -= 8) {
-                hist[tid] = 0;
-                __syncthreads();
-                for (int64_t i = tid; i < m; i += SM_THREADS) {
-                    const uint32_t k = key_of(i);
-                    if (k && (k & known) == prefix) atomicAdd((unsigned long long*)&hist[(k >> shift) & 255], 1ull);
-                }
-                __syncthreads();
-                if (tid == 0) {
-                    uint64_t a = above;
-                    int b = 255;
-                    while (b >= 0 && a + hist[b] < (uint64_t)top_k) a += hist[b--];
-                    bcast[0] = a;
-                    bcast[1] = (uint64_t)(int64_t)b;
-                }
-                __syncthreads();
-                const int b = (int)(int64_t)bcast[1];
-                above = bcast[0];
-                all = b < 0;   // fewer than top_k items in the row
-                if (!all) {
-                    prefix |= (uint32_t)b << shift;
-                    known |= 255u << shift;
-                }
-                __syncthreads();
-            }
-            if (!all) {
-                cut = prefix;
-                ties = top_k - (int64_t)above;
-            }
-        }
-        if (top_p < 1.0) {
-            // the mass of what top_k left
-            uint64_t v = 0;
-            for (int64_t i = tid; i < m; i += SM_THREADS) {
-                const uint32_t k = key_of(i);
-                if (k > cut) v += weight(k);
-            }
-            const uint64_t total = block_sum(v) + (cut > 1 ? (uint64_t)ties * weight(cut) : 0ull);
-            const double bound = top_p * (double)total;
-            uint32_t prefix = 0, known = 0;
-            uint64_t above = 0;
-            bool all = false;
-            for (int shift = 24; shift >= 0 && !all; shift -= 8) {
-                hist[tid] = 0;
-                __syncthreads();
-                for (int64_t i = tid; i < m; i += SM_THREADS) {
-                    const uint32_t k = key_of(i);
-                    if (k > cut && (k & known) == prefix)
-                        atomicAdd((unsigned long long*)&hist[(k >> shift) & 255], (unsigned long long)weight(k));
-                }
-                __syncthreads();
-                if (tid == 0) {
-                    uint64_t* hc = hist;
-                    if (cut > 1 && (cut & known) == prefix) hc[(cut >> shift) & 255] += (uint64_t)ties * weight(cut);
-                    // the last bucket with mass that starts before the bound
-                    uint64_t a = above;
-                    int b = 255, last = -1;
-                    uint64_t at = above;
-                    for (; b >= 0; --b) {
-                        if (hc[b] == 0) continue;
-                        if (last >= 0 && !((double)a < bound)) break;
-                        last = b;
-                        at = a;
-                        a += hc[b];
-                    }
-                    bcast[0] = at;
-                    bcast[1] = (uint64_t)(int64_t)last;
-                }
-                __syncthreads();
-                const int b = (int)(int64_t)bcast[1];
-                above = bcast[0];
-                all = b < 0;
-                if (!all) {
-                    prefix |= (uint32_t)b << shift;
-                    known |= 255u << shift;
-                }
-                __syncthreads();
-            }
-            if (!all) {
-                // of the items with this key the first r with above + (r - 1) w < bound
-                const double w = (double)weight(prefix);
-                double r = ceil((bound - (double)above) / w);
-                r = r < 1.0 ? 1.0 : r;
-                int64_t have = prefix == cut ? ties : m;
-                ties = r < (double)have ? (int64_t)r : have;
-                cut = prefix;
-            }
-        }
-        const double floor_w = min_p > 0.0 ? fmin(min_p, 1.0) * (double)(1ull << bits) : 0.0;
-
-        // kept weights in index order; `drawn_count` positions have been taken out
-        int drawn_count = 0;
-        auto kept = [&](int64_t i, int64_t& seen) -> uint64_t {   // called by the whole workgroup, i ascending over it
-            const uint32_t k = i < m ? key_of(i) : 0u;
-            const bool tie = k == cut && k != 0;
-            const uint64_t votes = __ballot(tie);
-            __syncthreads();
-            if (lane == 0) part32[wave] = (uint32_t)__popcll(votes);
-            __syncthreads();
-            int64_t before = seen + __popcll(votes & ((1ull << lane) - 1));
-            for (int w = 0; w < SM_THREADS / 64; ++w) {
-                before += w < wave ? part32[w] : 0;
-                seen += part32[w];
-            }
-            uint64_t wgt = 0;
-            if (k > cut || (tie && before < ties)) {
-                wgt = weight(k);
-                if ((double)wgt < floor_w) wgt = 0;
-            }
-            for (int j = 0; j < drawn_count; ++j) wgt = drawn[j] == i ? 0ull : wgt;
-            return wgt;
+        const RowCuts cuts = sm_cuts(par, row, m, bits);
+        const float best32 = sm_unorder(top), step32 = (float)(cuts.step * 32.0);
+        const double best = (double)best32;
+        auto weight = [&](uint32_t key) -> uint64_t { return sm_weight(sm_exponent(key, top, best, cuts.step), bits); };
+        // a bin of the first histogram: in 1/32 octaves below the best, everything from 32 octaves on in the last
+        auto first_bin = [&](uint32_t key) -> int {
+            const float d = key == top ? 0.f : (best32 - sm_unorder(key)) * step32;
+            return d < (float)(SM_BINS - 1) ? (int)d : d != d ? 0 : SM_BINS - 1;
         };
-        uint64_t total = 0;
-        for (int d = 0; d < draws; ++d) {
-            if (d == 0 || !replacement) {
-                uint64_t v = 0;
-                int64_t seen = 0;
-                for (int64_t i0 = 0; i0 < m; i0 += SM_THREADS) v += kept(i0 + tid, seen);
-                total = block_sum(v);
-            }
-            int32_t got = -1;
-            if (total > 0) {
-                const float u = uniforms[row * draws + d];
-                const double uc = u > 0.f ? fmin((double)u, 1.0 - 0x1p-53) : 0.0;
-                const uint64_t t = __umul64hi(total, (uint64_t)(uc * 0x1p53) << 11);
-                uint64_t run = 0;
-                int64_t seen = 0;
-                if (tid == 0) bcast[0] = ~0ull;
-                for (int64_t i0 = 0; i0 < m && run <= t; i0 += SM_THREADS) {
-                    const int64_t i = i0 + tid;
-                    const uint64_t w = kept(i, seen);
-                    const uint64_t inc = sm_wave_scan(w);
-                    __syncthreads();
-                    if (lane == 63) part[wave] = inc;
-                    __syncthreads();
-                    uint64_t base = run;
-                    for (int v = 0; v < SM_THREADS / 64; ++v) {
-                        base += v < wave ? part[v] : 0ull;
-                        run += part[v];
-                    }
-                    if (w && base + inc > t && base + inc - w <= t) bcast[0] = (uint64_t)i;
-                    __syncthreads();
+
+        uint64_t cut = 1ull << 32;   // every item with a key
+        // Moves `cut` to the item at the border: the target-th in order (by count), or the last item whose
+        // predecessors hold less than the share top_p of the mass at or above `cut`.  Where the row has no border it stays.
+        auto find_cut = [&](auto by_mass, uint64_t target, double top_p) {
+            constexpr bool BY_MASS = decltype(by_mass)::value;
+            uint64_t base = 0;      // count or mass of the items above the current range
+            uint64_t lo = cut, hi = ~0ull;
+            double bound = 0.0;
+            int shift = -1;         // -1: the first histogram
+            for (;;) {
+                for (int b = tid; b < SM_BINS; b += NT) {
+                    count_bins[b] = 0;
+                    if (BY_MASS) mass_bins[b] = 0;
                 }
-                __syncthreads();
-                const int64_t i = (int64_t)bcast[0];
-                got = 0;
                 if (tid == 0) {
-                    out_ids[row * draws + d] = id ? id[i] : (int32_t)i;
-                    out_logprob[row * draws + d] =
-                        (float)(exponent(key_of(i)) * 0.69314718055994531 - log(ldexp((double)total, -bits)));
-                    drawn[drawn_count] = i;
+                    shared_int[0] = 0;   // the bin, plus one
+                    shared_int[1] = 0;   // entries in the list
+                    shared_key[0] = ~0ull;
+                    shared_key[1] = 0;
                 }
-                if (!replacement) ++drawn_count;
+                __syncthreads();
+                auto bin_of = [&](uint64_t K) -> int { return shift < 0 ? first_bin((uint32_t)(K >> 32)) : (int)((hi - K) >> shift); };
+                each([&](const C& q, int64_t first, int p, int sub) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const uint32_t key = q.key(v);
+                        const uint64_t K = order_of(key, first, v);
+                        if (K >= lo && K <= hi) {
+                            const int b = bin_of(K);
+                            atomicAdd(&count_bins[b], 1u);
+                            if (BY_MASS) atomicAdd((unsigned long long*)&mass_bins[b], (unsigned long long)weight(key));
+                        }
+                    }
+                });
+                __syncthreads();
+                // running sums over the bins, BINS_PER neighbouring ones per thread
+                uint64_t sum = 0;
+                uint64_t mine[BINS_PER];
+#pragma unroll
+                for (int i = 0; i < BINS_PER; ++i) {
+                    mine[i] = BY_MASS ? mass_bins[tid * BINS_PER + i] : (uint64_t)count_bins[tid * BINS_PER + i];
+                    sum += mine[i];
+                }
+                const uint64_t inc = sm_wave_scan(sum);
+                if (lane == 63) part[0][wave] = inc;
+                __syncthreads();
+                uint64_t start = base + inc - sum, all = 0;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    start += w < wave ? part[0][w] : 0ull;
+                    all += part[0][w];
+                }
+                if (BY_MASS && shift < 0) bound = top_p * (double)all;
+                // The border's bin.  By count: the one that takes the running count to the target.  By mass: the last
+                // with mass that starts below the bound, or the first with mass.
+                uint64_t at = start;
+                int here = -1;
+                uint64_t here_start = 0;
+#pragma unroll
+                for (int i = 0; i < BINS_PER; ++i) {
+                    if (BY_MASS ? mine[i] > 0 && ((double)at < bound || at == base) : at < target && at + mine[i] >= target) {
+                        here = tid * BINS_PER + i;
+                        here_start = at;
+                    }
+                    at += mine[i];
+                }
+                if (here >= 0) atomicMax(&shared_int[0], (uint32_t)here + 1);
+                __syncthreads();
+                const int b = (int)shared_int[0] - 1;
+                if (b < 0) return;   // by count: fewer items than the target
+                if (here == b) shared_key[1] = here_start;
+                __syncthreads();
+                base = shared_key[1];
+                const uint32_t members = count_bins[b];
+                if (members <= SM_LIST) {
+                    each([&](const C& q, int64_t first, int p, int sub) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            const uint32_t key = q.key(v);
+                            const uint64_t K = order_of(key, first, v);
+                            if (K >= lo && K <= hi && bin_of(K) == b) {
+                                ulonglong2 e;
+                                e.x = K;
+                                e.y = BY_MASS ? weight(key) : 1ull;
+                                list[atomicAdd(&shared_int[1], 1u)] = e;
+                            }
+                        }
+                    });
+                    __syncthreads();
+                    for (uint32_t e = tid; e < members; e += NT) {
+                        const ulonglong2 x = list[e];
+                        uint64_t before = base;
+#pragma unroll 8
+                        for (uint32_t j = 0; j < members; ++j) before += list[j].x > x.x ? list[j].y : 0ull;
+                        const bool kept = BY_MASS ? x.y > 0 && ((double)before < bound || before == base) : before < target;
+                        if (kept) atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)x.x);
+                    }
+                    __syncthreads();
+                    cut = shared_key[0];
+                    __syncthreads();
+                    return;
+                }
+                // too many for the list: the bin's range of K, in equal parts
+                if (shift < 0) {
+                    uint64_t first = 0, last = ~0ull;
+                    each([&](const C& q, int64_t i0, int, int) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            const uint64_t K = order_of(q.key(v), i0, v);
+                            if (K >= lo && K <= hi && bin_of(K) == b) {
+                                first = K > first ? K : first;
+                                last = K < last ? K : last;
+                            }
+                        }
+                    });
+                    __syncthreads();
+                    if (tid == 0) shared_key[1] = 0;
+                    __syncthreads();
+                    atomicMax((unsigned long long*)&shared_key[1], (unsigned long long)first);
+                    atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)last);
+                    __syncthreads();
+                    hi = shared_key[1];
+                    lo = shared_key[0];
+                } else {
+                    hi -= (uint64_t)b << shift;
+                    const uint64_t down = hi - ((1ull << shift) - 1);
+                    lo = down > lo ? down : lo;
+                }
+                shift = 64 - __builtin_clzll((hi - lo) | 1ull) - 10;
+                shift = shift > 0 ? shift : 0;
                 __syncthreads();
             }
-            if (got < 0 && tid == 0) {
-                out_ids[row * draws + d] = -1;
-                out_logprob[row * draws + d] = -INFINITY;
+        };
+
+        if (cuts.top_k < m) find_cut(std::false_type{}, (uint64_t)cuts.top_k, 0.0);
+        if (cuts.top_p < 1.0) find_cut(std::true_type{}, 0ull, cuts.top_p);
+
+        // The kept mass of every piece, then its running sum in index order.
+        auto kept_weight = [&](const C& q, int64_t first, int v) -> uint64_t {
+            const uint32_t key = q.key(v);
+            if (order_of(key, first, v) < cut) return 0ull;
+            const uint64_t w = weight(key);
+            return (double)w >= cuts.floor_w ? w : 0ull;
+        };
+        for (int p = tid; p < SM_BINS; p += NT) mass_bins[p] = 0;
+        __syncthreads();
+        {
+            uint64_t w = 0;
+            each([&](const C& q, int64_t first, int p, int sub) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) w += kept_weight(q, first, v);
+                if (sub == S - 1) {
+                    w = sm_wave_sum(w);
+                    if (lane == 0) mass_bins[p] = w;
+                    w = 0;
+                }
+            });
+        }
+        __syncthreads();
+        uint64_t sum = 0, mine[BINS_PER];
+#pragma unroll
+        for (int i = 0; i < BINS_PER; ++i) {
+            mine[i] = mass_bins[tid * BINS_PER + i];
+            sum += mine[i];
+        }
+        const uint64_t inc = sm_wave_scan(sum);
+        if (lane == 63) part[0][wave] = inc;
+        __syncthreads();
+        uint64_t at = inc - sum, total = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            at += w < wave ? part[0][w] : 0ull;
+            total += part[0][w];
+        }
+#pragma unroll
+        for (int i = 0; i < BINS_PER; ++i) {
+            at += mine[i];
+            mass_bins[tid * BINS_PER + i] = at;
+        }
+        __syncthreads();
+
+        // A draw: the piece its number falls into, by two looks at the running sums, then the item, from the piece's
+        // scores once more.  Draws that come back are shared out over the wavefronts; those that do not are one
+        // wavefront's, which takes a drawn item's weight out of every running sum behind it.
+        if (!replacement && wave != 0) continue;
+        int taken = 0;
+        for (int d = replacement ? wave : 0; d < draws; d += replacement ? NW : 1) {
+            if (total == 0) {
+                if (lane == 0) {
+                    out_ids[row * draws + d] = -1;
+                    out_logprob[row * draws + d] = -INFINITY;
+                }
+                continue;
+            }
+            const uint64_t t = sm_target(uniforms[row * draws + d], total);
+            const int p16 = __builtin_ctzll(__ballot(mass_bins[lane * (SM_BINS / 64) + SM_BINS / 64 - 1] > t));
+            const int p = p16 * (SM_BINS / 64) + __builtin_ctzll(__ballot(lane >= SM_BINS / 64 || mass_bins[p16 * (SM_BINS / 64) + (lane & (SM_BINS / 64 - 1))] > t));
+            uint64_t run = p > 0 ? mass_bins[p - 1] : 0ull;
+            for (int sub = 0; sub < S; ++sub) {
+                const C q = load(p, sub);
+                const int64_t first = first_item(p, sub);
+                uint64_t w[V], mine_w = 0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    w[v] = kept_weight(q, first, v);
+                    for (int j = 0; j < taken; ++j) w[v] = gone[j] == (int32_t)(first + v) ? 0ull : w[v];
+                    mine_w += w[v];
+                }
+                const uint64_t upto = run + sm_wave_scan(mine_w);
+                const uint64_t votes = __ballot(upto > t);
+                if (votes == 0) {
+                    run = sm_lane(upto, 63);
+                    continue;
+                }
+                const int l = __builtin_ctzll(votes);
+                uint64_t before = upto - mine_w, drawn = 0;
+                int at_v = 0;
+                bool found = false;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (!found && w[v] && before + w[v] > t) {
+                        found = true;
+                        at_v = v;
+                        drawn = w[v];
+                    }
+                    before += w[v];
+                }
+                if (lane == l) {
+                    const int64_t item = first + at_v;
+                    uint32_t key = 0;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) key = at_v == v ? q.key(v) : key;
+                    out_ids[row * draws + d] = id ? id[item] : (int32_t)item;
+                    out_logprob[row * draws + d] = sm_logprob(sm_exponent(key, top, best, cuts.step), total, bits);
+                    if (!replacement) gone[taken] = (int32_t)item;
+                }
+                if (!replacement) {
+                    ++taken;
+                    const uint64_t less = sm_lane(drawn, l);
+                    total -= less;
+                    for (int j = p + lane; j < SM_BINS; j += 64) mass_bins[j] -= less;
+                    asm volatile("" ::: "memory");
+                }
+                break;
             }
         }
     }
@@ -364,6 +760,58 @@ static int sample_bits(int64_t m) {
     int b = 0;
     while (((int64_t)1 << b) < m) ++b;
     return 62 - b < 51 ? 62 - b : 51;
+}
+
+template <int DT, int E>
+static int launch_short(const typename ScoreType<DT>::raw* scores, int64_t n, int m, int64_t stride, const int32_t* ids,
+                        int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
+                        int draws, int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
+                        hipStream_t stream) {
+    const int64_t blocks = (n + 3) / 4;
+    hipLaunchKernelGGL((sample_short_kernel<DT, E>), dim3((unsigned)(blocks < 262144 ? blocks : 262144)), dim3(256), 0, stream,
+                       scores, n, m, stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits,
+                       out_ids, out_logprob);
+    MIREC_LAUNCH_CHECK();
+    return MIREC_OK;
+}
+
+template <int DT, int NT, int CH>
+static int launch_long(const typename ScoreType<DT>::raw* scores, int64_t n, int64_t m, int64_t stride, const int32_t* ids,
+                       int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
+                       int draws, int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
+                       hipStream_t stream) {
+    // the filter's bitmap of a long row (up to 64 KiB) takes more dynamic LDS than a kernel gets unasked
+    static OncePerDevice once;   // idempotent; a race only repeats the call
+    bool* done = once.slot();
+    MIREC_REQUIRE(done, MIREC_E_HIP, "mirec_sample: cannot read the current device");
+    if (!*done) {
+        MIREC_HIP(hipFuncSetAttribute((const void*)sample_long_kernel<DT, NT, CH>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)(SM_MAX_MASKED_ITEMS / 8)));
+        *done = true;
+    }
+    const size_t lds = mask_indptr ? (size_t)((m + 31) / 32) * 4 : 0;
+    hipLaunchKernelGGL((sample_long_kernel<DT, NT, CH>), dim3((unsigned)(n < 262144 ? n : 262144)), dim3(NT), lds, stream, scores,
+                       n, m, stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids,
+                       out_logprob);
+    MIREC_LAUNCH_CHECK();
+    return MIREC_OK;
+}
+
+template <int DT>
+static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stride, const int32_t* ids, int64_t ids_stride,
+                         const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms, int draws,
+                         int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
+                         hipStream_t stream) {
+    const typename ScoreType<DT>::raw* scores = (const typename ScoreType<DT>::raw*)scores_;
+#define MIREC_SAMPLE_ARGS stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids, out_logprob, stream
+    if (m <= 64) return launch_short<DT, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    if (m <= 128) return launch_short<DT, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    if (m <= SM_SHORT) return launch_short<DT, 4>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    constexpr int V = Chunk<DT>::V;
+    if (m <= 256 * V * 8) return launch_long<DT, 256, 8>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (m <= 512 * V * 16) return launch_long<DT, 512, 16>(scores, n, m, MIREC_SAMPLE_ARGS);
+    return launch_long<DT, 1024, 0>(scores, n, m, MIREC_SAMPLE_ARGS);
+#undef MIREC_SAMPLE_ARGS
 }
 
 }  // namespace mirec
@@ -404,30 +852,26 @@ extern "C" int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m,
     MIREC_REQUIRE(!mask_indptr || m <= SM_MAX_MASKED_ITEMS, MIREC_E_UNSUPPORTED,
                   "mirec_sample: a filter over %lld items; at most %lld are supported", (long long)m,
                   (long long)SM_MAX_MASKED_ITEMS);
-    const SampleParams par = {temperature, top_p, min_p, top_k, row_temperature, row_top_k, row_top_p, row_min_p};
+    SampleParams par = {};
+    par.greedy = !(temperature >= SM_MIN_TEMPERATURE);
+    par.step = par.greedy ? 0.0 : 1.4426950408889634 / temperature;
+    par.top_p = top_p;
+    par.min_p = min_p;
+    par.top_k = top_k;
+    par.row_temperature = row_temperature;
+    par.row_top_k = row_top_k;
+    par.row_top_p = row_top_p;
+    par.row_min_p = row_min_p;
     const int bits = sample_bits(m);
-    const unsigned blocks = (unsigned)(n < 262144 ? n : 262144);
-    const size_t lds = mask_indptr ? (size_t)((m + 31) / 32) * 4 : 0;
-    // the filter's bitmap of a long row (up to 64 KiB) takes more dynamic LDS than a kernel gets unasked
-#define MIREC_SAMPLE(DT)                                                                                             \
-    do {                                                                                                             \
-        static OncePerDevice once;                                                                                   \
-        bool* done = once.slot();                                                                                    \
-        MIREC_REQUIRE(done, MIREC_E_HIP, "mirec_sample: cannot read the current device");                            \
-        if (!*done) {                                                                                                \
-            MIREC_HIP(hipFuncSetAttribute((const void*)sample_rows_kernel<DT>,                                       \
-                                          hipFuncAttributeMaxDynamicSharedMemorySize,                                \
-                                          (int)(SM_MAX_MASKED_ITEMS / 8)));                                          \
-            *done = true;                                                                                            \
-        }                                                                                                            \
-        hipLaunchKernelGGL((sample_rows_kernel<DT>), dim3(blocks), dim3(SM_THREADS), lds, stream,                    \
-                           (const ScoreType<DT>::raw*)scores, n, m, row_stride, ids, ids_stride, mask_indptr,        \
-                           mask_indices, uniforms, draws, replacement, par, bits, out_ids, out_logprob);             \
-    } while (0)
-    if (dtype == MIREC_F32) MIREC_SAMPLE(MIREC_F32);
-    else if (dtype == MIREC_F16) MIREC_SAMPLE(MIREC_F16);
-    else MIREC_SAMPLE(MIREC_BF16);
-#undef MIREC_SAMPLE
-    MIREC_LAUNCH_CHECK();
-    return MIREC_OK;
+    switch (dtype) {
+        case MIREC_F32:
+            return launch_sample<MIREC_F32>(scores, n, m, row_stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws,
+                                            replacement, par, bits, out_ids, out_logprob, stream);
+        case MIREC_F16:
+            return launch_sample<MIREC_F16>(scores, n, m, row_stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws,
+                                            replacement, par, bits, out_ids, out_logprob, stream);
+        default:
+            return launch_sample<MIREC_BF16>(scores, n, m, row_stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws,
+                                             replacement, par, bits, out_ids, out_logprob, stream);
+    }
 }
