@@ -10,6 +10,7 @@
 // of 27 000 weights is exact where fp32 would move its borders by more than the width of an unlikely item.
 #include <float.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -20,11 +21,13 @@ constexpr int SM_MAX_DRAWS = MIREC_SAMPLE_MAX_DRAWS;
 constexpr int64_t SM_MAX_MASKED_ITEMS = MIREC_SAMPLE_MAX_MASKED_ITEMS;   // the filter of a row is a bitmap in LDS
 constexpr double SM_MIN_TEMPERATURE = 1e-37;      // below: greedy
 constexpr int SM_SHORT = 256;                     // rows up to this length: one wavefront each
+constexpr int64_t SM_FEW_ROWS = 256;              // no more rows than compute units: larger workgroups
 constexpr int SM_BINS = 1024;                     // of a histogram over a row
 constexpr int SM_LIST = 512;                     // entries that are ranked against each other in LDS
 
 struct SampleParams {
-    double step, top_p, min_p;   // step: log2 e / temperature
+    double step, top_p;   // step: log2 e / temperature
+    uint64_t floor_w;     // least weight that min_p keeps
     int32_t top_k;
     bool greedy;
     const float* row_temperature;
@@ -66,26 +69,50 @@ struct ScoreType<MIREC_BF16> {
     __device__ static __forceinline__ float widen(raw v) { return __uint_as_float((uint32_t)v << 16); }
 };
 
-// 2^t for t <= 0 as a fixed-point number with `bits` fraction bits (bits <= 51): t = k + f with |f| <= 1/2, 2^f by its
-// power series to the tenth term (the eleventh is below 2.2e-13 of the value), scaled and rounded to an integer by
-// adding 2^52.
-__device__ __forceinline__ uint64_t sm_weight(double t, int bits) {
-    t = fmax(t, -2000.0);   // also what an infinite difference times a zero step gives
-    const double k = rint(t);
-    const double f = t - k;
-    double p = 7.054911620801121e-09;                 // ln2^10 / 10!
-    p = __builtin_fma(p, f, 1.0178086009239696e-07);  // ln2^9 / 9!
-    p = __builtin_fma(p, f, 1.3215486790144305e-06);
-    p = __builtin_fma(p, f, 1.5252733804059838e-05);
-    p = __builtin_fma(p, f, 1.5403530393381606e-04);
-    p = __builtin_fma(p, f, 1.3333558146428441e-03);
-    p = __builtin_fma(p, f, 9.618129107628477e-03);
-    p = __builtin_fma(p, f, 5.5504108664821576e-02);
-    p = __builtin_fma(p, f, 2.402265069591007e-01);
-    p = __builtin_fma(p, f, 6.931471805599453e-01);
-    p = __builtin_fma(p, f, 1.0);
-    const double v = ldexp(p, (int)k + bits) + 4503599627370496.0;
+// a b + c with c in scalar registers.  (Left alone, the compiler copies each constant into the accumulator of a
+// two-address multiply-add first: nine copies for nine steps below.)
+__device__ __forceinline__ double sm_fma(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+
+// 2^f for |f| <= 1/2 to 1.6e-14 of it: 1 + f q(f), q of degree 8 fitted to the least largest relative error (a Lawson
+// iteration on (2^f - 1) / f); exact at f = 0.
+__device__ __forceinline__ double sm_exp2_fraction(double f) {
+    double p = 1.0148328577088516e-07;
+    p = sm_fma(p, f, 1.3258336037497191e-06);
+    p = sm_fma(p, f, 1.5252989797007882e-05);
+    p = sm_fma(p, f, 1.5403440872165233e-04);
+    p = sm_fma(p, f, 1.3333557626651542e-03);
+    p = sm_fma(p, f, 9.618129181194148e-03);
+    p = sm_fma(p, f, 5.550410866839772e-02);
+    p = sm_fma(p, f, 2.4022650695722697e-01);
+    p = sm_fma(p, f, 6.931471805598861e-01);
+    return __builtin_fma(p, f, 1.0);
+}
+
+constexpr double SM_ROUND = 6755399441055744.0;   // 1.5 2^52: the sum's low bits are the nearest integer
+
+// The weight of a score: 2^((s - best) step) with `bits` (at most 51) fraction bits, the nearest such number; 0 for minus
+// infinity.  Vector float64 instructions run at the rate of float32 ones here, and about twenty of them are all there is.
+__device__ __forceinline__ uint64_t sm_weight(float score, double best, double step, int bits) {
+    const double t = fmax(((double)score - best) * step, -80.0);   // (a NaN, infinity times zero, becomes -80 too)
+    const double k = t + SM_ROUND;
+    const double p = sm_exp2_fraction(t - (k - SM_ROUND));
+    // 2^(k + bits) into the exponent, 2^52 to round, the integer out of the mantissa
+    const double v = __longlong_as_double(__double_as_longlong(p) + ((int64_t)((int)(uint32_t)__double_as_longlong(k) + bits) << 52)) +
+                     4503599627370496.0;
     return (uint64_t)__double_as_longlong(v) & 0xfffffffffffffull;
+}
+
+// log2 x of a positive normal number to 1e-13 or so: the fp32 logarithm, then one Newton step with the power above.
+__device__ __forceinline__ double sm_log2(double x) {
+    const double l = (double)__builtin_amdgcn_logf((float)x);
+    const double k = l + SM_ROUND;
+    const double back = sm_exp2_fraction((k - SM_ROUND) - l);   // 2^(k - l)
+    const double r = ldexp(x, -(int)(uint32_t)__double_as_longlong(k)) * back - 1.0;   // x / 2^l - 1
+    return __builtin_fma(r * (1.0 - 0.5 * r), 1.4426950408889634, l);
 }
 
 // ---- 64-bit sums over a wavefront, by data-parallel moves between lanes (no LDS)
@@ -114,16 +141,33 @@ __device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {
 
 __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_lane(sm_wave_scan(v), 63); }
 
+__device__ __forceinline__ float sm_wave_max(float v) {
+#define SM_MAX_STEP(CTRL, ROWS)                                                                                        \
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(v), CTRL, ROWS, 0xf, false)))
+    SM_MAX_STEP(0x111, 0xf);
+    SM_MAX_STEP(0x112, 0xf);
+    SM_MAX_STEP(0x114, 0xf);
+    SM_MAX_STEP(0x118, 0xf);
+    SM_MAX_STEP(0x142, 0xa);
+    SM_MAX_STEP(0x143, 0xc);
+#undef SM_MAX_STEP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
 // Where a number of [0, 1) falls in a total: floor(u * total), u moved into [0, 1 - 2^-53].
 __device__ __forceinline__ uint64_t sm_target(float u, uint64_t total) {
     const double uc = u > 0.f ? fmin((double)u, 1.0 - 0x1p-53) : 0.0;
     return __umul64hi(total, (uint64_t)(uc * 0x1p53) << 11);
 }
 
+// The least integer mass that is not below a share of a total.
+__device__ __forceinline__ uint64_t sm_bound(double share, uint64_t total) { return (uint64_t)ceil(fmax(share, 0.0) * (double)total); }
+
 // What the cuts and the temperature of one row come to.
 struct RowCuts {
     int64_t top_k;
-    double top_p, floor_w, step;   // step: log2 e / temperature
+    double top_p, step;   // step: log2 e / temperature
+    uint64_t floor_w;     // least weight that min_p keeps
 };
 
 __device__ __forceinline__ RowCuts sm_cuts(const SampleParams& par, int64_t row, int64_t m, int bits) {
@@ -136,101 +180,123 @@ __device__ __forceinline__ RowCuts sm_cuts(const SampleParams& par, int64_t row,
         c.step = greedy ? 0.0 : 1.4426950408889634 / T;
     }
     c.top_p = par.row_top_p ? (double)par.row_top_p[row] : par.top_p;
-    const double min_p = par.row_min_p ? (double)par.row_min_p[row] : par.min_p;
+    c.floor_w = par.floor_w;
+    if (par.row_min_p) {
+        const double min_p = (double)par.row_min_p[row];
+        c.floor_w = min_p > 0.0 ? sm_bound(fmin(min_p, 1.0), 1ull << bits) : 0ull;
+    }
     c.top_k = par.row_top_k ? par.row_top_k[row] : par.top_k;
     if (c.top_k <= 0 || c.top_k > m) c.top_k = m;
     if (greedy) c.top_k = 1;
-    c.floor_w = min_p > 0.0 ? fmin(min_p, 1.0) * (double)(1ull << bits) : 0.0;
     return c;
 }
 
-// log2 of a weight before rounding, from the key of its item and the row's best.
-__device__ __forceinline__ double sm_exponent(uint32_t key, uint32_t top, double best, double step) {
-    return key == top ? 0.0 : ((double)sm_unorder(key) - best) * step;
-}
-
-__device__ __forceinline__ float sm_logprob(double exponent, uint64_t total, int bits) {
-    return (float)(exponent * 0.69314718055994531 - log(ldexp((double)total, -bits)));
+__device__ __forceinline__ float sm_logprob(float score, double best, double step, uint64_t total, int bits) {
+    const double t = fmax(((double)score - best) * step, -80.0);
+    return (float)((t - sm_log2(ldexp((double)total, -bits))) * 0.69314718055994531);
 }
 
 // ------------------------------------------------------------------------------------------------------ short rows
 
-// One wavefront per row of at most 64 E items, all of it in registers: item 64 j + l in lane l.  A ranked list is in
-// order already (one comparison of neighbours says so), and then the running sum in index order is the running sum in
-// rank order too: one scan serves the cuts and the draws.  Otherwise every item is compared with every other.
+// One wavefront per row of at most 64 E items, all of it in registers: items E l .. E l + E - 1 in lane l, so that one scan
+// over the lanes gives every running sum.  A ranked list is in order already (one comparison of neighbours says so), and
+// then the running sum in index order is the running sum in rank order too: the scan serves the cuts and the draws.
+// Otherwise every item is compared with every other.  A wavefront takes `rows_each` rows, one after the other, and leaves
+// their draws in its lanes, one each, until there are 64 of them: logarithms and stores are then one for all.
+// What bounds it is the number of vector instructions per row.
 template <int DT, int E>
 __global__ __launch_bounds__(256) void sample_short_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int m, int64_t stride, const int32_t* __restrict__ ids,
     int64_t ids_stride, const int64_t* __restrict__ mask_indptr, const int32_t* __restrict__ mask_indices,
-    const float* __restrict__ uniforms, int draws, int replacement, SampleParams par, int bits,
+    const float* __restrict__ uniforms, int draws, int replacement, int rows_each, SampleParams par, int bits,
     int32_t* __restrict__ out_ids, float* __restrict__ out_logprob) {
     const int lane = threadIdx.x & 63;
-    const int64_t waves = (int64_t)gridDim.x * 4;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < n; row += waves) {
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * rows_each;
+    const int64_t row1 = row0 + rows_each < n ? row0 + rows_each : n;
+    // draws that are not written yet, in lanes 0 .. waiting - 1: number out0 + lane
+    int waiting = 0;
+    int64_t out0 = row0 * draws;
+    int32_t got = -1;
+    float got_f = 0.f, got_best = 0.f;
+    double got_step = 0.0;
+    uint64_t got_total = 1;
+    auto flush = [&]() {
+        if (lane < waiting) {
+            out_ids[out0 + lane] = got;
+            out_logprob[out0 + lane] = got >= 0 ? sm_logprob(got_f, (double)got_best, got_step, got_total, bits) : -INFINITY;
+        }
+        out0 += waiting;
+        waiting = 0;
+    };
+
+    for (int64_t row = row0; row < row1; ++row) {
         const typename ScoreType<DT>::raw* s = scores + row * stride;
-        float value[E];
+        const int first = E * lane;
+        float f[E];   // minus infinity where excluded; infinity counts as the largest finite score
         int32_t id[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            const int i = 64 * j + lane;
-            value[j] = i < m ? ScoreType<DT>::widen(s[i]) : -INFINITY;
-            id[j] = ids && i < m ? ids[row * ids_stride + i] : i;
+            f[j] = first + j < m ? ScoreType<DT>::widen(s[first + j]) : -INFINITY;
+            id[j] = ids && first + j < m ? ids[row * ids_stride + first + j] : first + j;
         }
-        uint32_t key[E];
+        const float u0 = lane < draws ? uniforms[row * draws + lane] : 0.f;
 #pragma unroll
-        for (int j = 0; j < E; ++j) key[j] = value[j] > ScoreType<DT>::lowest && id[j] >= 0 ? sm_order(value[j]) : 0u;
+        for (int j = 0; j < E; ++j) f[j] = f[j] > ScoreType<DT>::lowest && id[j] >= 0 ? fminf(f[j], FLT_MAX) : -INFINITY;
         if (mask_indptr) {   // each lane looks for its items in the row's filter
             for (int64_t e = mask_indptr[row]; e < mask_indptr[row + 1]; ++e) {
                 const int32_t it = mask_indices[e];
 #pragma unroll
-                for (int j = 0; j < E; ++j) key[j] = it == 64 * j + lane ? 0u : key[j];
+                for (int j = 0; j < E; ++j) f[j] = it == first + j ? -INFINITY : f[j];
             }
         }
-        uint32_t top = key[0];
+        float top = f[0];
 #pragma unroll
-        for (int j = 1; j < E; ++j) top = key[j] > top ? key[j] : top;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            const uint32_t o = (uint32_t)__shfl_xor((int)top, d, 64);
-            top = o > top ? o : top;
-        }
-        top = (uint32_t)__builtin_amdgcn_readfirstlane((int)top);
+        for (int j = 1; j < E; ++j) top = fmaxf(top, f[j]);
+        top = sm_wave_max(top);
         const RowCuts cut = sm_cuts(par, row, m, bits);
-        const double best = (double)sm_unorder(top);
+        const float best32 = top > -INFINITY ? top : 0.f;
+        const double best = (double)best32;
         uint64_t w[E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) w[j] = key[j] ? sm_weight(sm_exponent(key[j], top, best, cut.step), bits) : 0ull;
+        for (int j = 0; j < E; ++j) w[j] = sm_weight(f[j], best, cut.step, bits);
 
+        // in order if no item is better than the one before it (the next lane's first: minus infinity after lane 63)
+        float before_f = __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(f[0]), 0x130, 0xf, 0xf, false));
         bool ordered = true;
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            uint32_t next = (uint32_t)__shfl_down((int)key[j], 1, 64);
-            if (lane == 63) next = 0;
-            ordered = ordered && key[j] >= next;
-            if (j + 1 < E) ordered = ordered && (lane < 63 || key[j] >= (uint32_t)__builtin_amdgcn_readlane((int)key[j + 1], 0));
+        for (int j = E - 1; j >= 0; --j) {
+            ordered = ordered && f[j] >= before_f;
+            before_f = f[j];
         }
         uint64_t run[E];   // sum of the kept weights up to and with the item
-        uint64_t total = 0;
-        if (__all(ordered)) {
+        auto scan = [&]() -> uint64_t {
+            uint64_t sum = w[0];
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                if (64 * j + lane >= cut.top_k) w[j] = 0;
-                run[j] = total + sm_wave_scan(w[j]);
-                total = sm_lane(run[j], 63);
+            for (int j = 1; j < E; ++j) sum += w[j];
+            const uint64_t inc = sm_wave_scan(sum);
+            run[E - 1] = inc;
+#pragma unroll
+            for (int j = E - 1; j > 0; --j) run[j - 1] = run[j] - w[j];
+            return sm_lane(inc, 63);
+        };
+        uint64_t total;
+        if (__all(ordered)) {
+            if (cut.top_k < m) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) w[j] = first + j < cut.top_k ? w[j] : 0ull;
             }
-            if (cut.top_p < 1.0 || cut.floor_w > 0.0) {
-                const double bound = cut.top_p < 1.0 ? cut.top_p * (double)total : INFINITY;
-                uint64_t kept = 0;   // a prefix stays: the running sum at its end
+            total = scan();
+            if (cut.top_p < 1.0 || cut.floor_w > 0) {
+                const uint64_t bound = cut.top_p < 1.0 ? sm_bound(cut.top_p, total) : ~0ull;
+                uint64_t last = 0;   // a prefix stays: the running sum at its end
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
-                    const bool stays = (64 * j + lane == 0 || (double)(run[j] - w[j]) < bound) && (double)w[j] >= cut.floor_w;
-                    if (!stays) w[j] = 0;
-                    const uint64_t votes = __ballot(stays && w[j] != 0);
-                    if (votes) kept = sm_lane(run[j], 63 - __builtin_clzll(votes));
+                    const bool stays = (first + j == 0 || run[j] - w[j] < bound) && w[j] >= cut.floor_w && w[j] != 0;
+                    w[j] = stays ? w[j] : 0ull;
+                    last = stays ? run[j] : last;
                 }
-                total = kept;
-#pragma unroll
-                for (int j = 0; j < E; ++j) run[j] = run[j] < total ? run[j] : total;
+                const uint64_t votes = __ballot(last != 0);
+                total = votes ? sm_lane(last, 63 - __builtin_clzll(votes)) : 0ull;
             }
         } else {
             uint32_t rank[E];
@@ -241,16 +307,16 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
                 before[j] = 0;
             }
             if (cut.top_k < m || cut.top_p < 1.0) {
+                for (int l = 0; E * l < m; ++l)
 #pragma unroll
-                for (int q = 0; q < E; ++q)
-                    for (int l = 0; l < 64 && 64 * q + l < m; ++l) {
-                        const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key[q], l);
-                        const uint64_t kw = sm_lane(w[q], l);
+                    for (int q = 0; q < E; ++q) {
+                        const float g = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[q]), l));
+                        const uint64_t gw = sm_lane(w[q], l);
 #pragma unroll
                         for (int j = 0; j < E; ++j) {
-                            const bool ahead = k > key[j] || (k == key[j] && 64 * q + l < 64 * j + lane);
+                            const bool ahead = g > f[j] || (g == f[j] && E * l + q < first + j);
                             rank[j] += ahead ? 1u : 0u;
-                            before[j] += ahead ? kw : 0ull;
+                            before[j] += ahead ? gw : 0ull;
                         }
                     }
             }
@@ -260,57 +326,63 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
                 if (rank[j] >= cut.top_k) w[j] = 0;
                 mass += w[j];
             }
-            const double bound = cut.top_p < 1.0 ? cut.top_p * (double)sm_wave_sum(mass) : INFINITY;
+            const uint64_t bound = cut.top_p < 1.0 ? sm_bound(cut.top_p, sm_wave_sum(mass)) : ~0ull;
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                if (!((rank[j] == 0 || (double)before[j] < bound) && (double)w[j] >= cut.floor_w)) w[j] = 0;
-                run[j] = total + sm_wave_scan(w[j]);
-                total = sm_lane(run[j], 63);
-            }
+            for (int j = 0; j < E; ++j)
+                if (!((rank[j] == 0 || before[j] < bound) && w[j] >= cut.floor_w)) w[j] = 0;
+            total = scan();
         }
 
         for (int d0 = 0; d0 < draws; d0 += 64) {
             const int cnt = draws - d0 < 64 ? draws - d0 : 64;
-            const float u = lane < cnt ? uniforms[row * draws + d0 + lane] : 0.f;
-            int32_t got = -1;
-            uint32_t got_key = 0;
-            uint64_t got_total = 1;
-            for (int d = 0; d < cnt && total > 0; ++d) {
-                const uint64_t t = sm_target(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(u), d)), total);
-                bool found = false;
+            const float u = d0 == 0 ? u0 : lane < cnt ? uniforms[row * draws + d0 + lane] : 0.f;
+            if (waiting + cnt > 64) flush();
+            const uint64_t targets = sm_target(u, total);
+            for (int d = 0; d < cnt; ++d, ++waiting) {
+                if (total == 0) {
+                    if (lane == waiting) got = -1;
+                    continue;
+                }
+                const uint64_t t = replacement ? sm_lane(targets, d)
+                                               : sm_target(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(u), d)), total);
+                // the first lane whose last running sum is above the number, and its first item for which that holds
+                const int l = __builtin_ctzll(__ballot(run[E - 1] > t));
+                int j_of = E - 1;
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const uint64_t votes = __ballot(run[j] > t);
-                    if (!found && votes) {
-                        found = true;
-                        const int l = __builtin_ctzll(votes);
-                        if (lane == d) {
-                            got_key = 0;   // below
-                            got_total = total;
-                        }
-                        const int32_t item = __builtin_amdgcn_readlane(id[j], l);
-                        const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key[j], l);
-                        if (lane == d) {
-                            got = item;
-                            got_key = k;
-                        }
-                        if (!replacement) {   // the item leaves: every running sum from it on is lower by its weight
-                            const uint64_t gone = sm_lane(w[j], l);
-                            if (lane == l) w[j] = 0;
-                            total -= gone;
+                for (int j = E - 2; j >= 0; --j) j_of = run[j] > t ? j : j_of;
+                int32_t my_id = id[E - 1];
+                float my_f = f[E - 1];
 #pragma unroll
-                            for (int q = 0; q < E; ++q) run[q] -= 64 * q + lane >= 64 * j + l ? gone : 0ull;
-                        }
+                for (int j = E - 2; j >= 0; --j) {
+                    my_id = j_of == j ? id[j] : my_id;
+                    my_f = j_of == j ? f[j] : my_f;
+                }
+                const int32_t item = __builtin_amdgcn_readlane(my_id, l);
+                const float score = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_f), l));
+                if (lane == waiting) {
+                    got = item;
+                    got_f = score;
+                    got_best = best32;
+                    got_step = cut.step;
+                    got_total = total;
+                }
+                if (!replacement) {   // the item leaves: every running sum from it on is lower by its weight
+                    const int at = E * l + __builtin_amdgcn_readlane(j_of, l);
+                    uint64_t mine = 0;
+#pragma unroll
+                    for (int j = 0; j < E; ++j) mine = first + j == at ? w[j] : mine;
+                    const uint64_t gone = sm_lane(mine, l);
+                    total -= gone;
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        w[j] = first + j == at ? 0ull : w[j];
+                        run[j] -= first + j >= at ? gone : 0ull;
                     }
                 }
             }
-            if (lane < cnt) {
-                out_ids[row * draws + d0 + lane] = got;
-                out_logprob[row * draws + d0 + lane] =
-                    got >= 0 ? sm_logprob(sm_exponent(got_key, top, best, cut.step), got_total, bits) : -INFINITY;
-            }
         }
     }
+    flush();
 }
 
 // ------------------------------------------------------------------------------------------------------- long rows
@@ -324,7 +396,7 @@ template <int DT>
 struct Chunk {
     static constexpr int V = DT == MIREC_F32 ? 4 : 8;   // scores of a thread's 16 bytes
     uint32_t word[4];
-    __device__ __forceinline__ float value(int v) const {
+    __device__ __forceinline__ float raw(int v) const {
         if constexpr (DT == MIREC_F32)
             return __uint_as_float(word[v]);
         else if constexpr (DT == MIREC_BF16)
@@ -332,15 +404,23 @@ struct Chunk {
         else
             return (float)__builtin_bit_cast(_Float16, (uint16_t)(word[v >> 1] >> (16 * (v & 1))));
     }
-    __device__ __forceinline__ uint32_t key(int v) const {
-        const float f = value(v);
-        return f > ScoreType<DT>::lowest ? sm_order(f) : 0u;
-    }
-    __device__ __forceinline__ void exclude(int v) {   // minus infinity
+    // minus infinity where excluded (once settle() has run); infinity counts as the largest finite score
+    __device__ __forceinline__ float score(int v) const { return DT == MIREC_F32 ? raw(v) : fminf(raw(v), FLT_MAX); }
+    __device__ __forceinline__ void exclude(int v) {
         if constexpr (DT == MIREC_F32) word[v] = 0xff800000u;
         else {
             const uint32_t inf = DT == MIREC_BF16 ? 0xff80u : 0xfc00u;
             word[v >> 1] = v & 1 ? (word[v >> 1] & 0xffffu) | (inf << 16) : (word[v >> 1] & 0xffff0000u) | inf;
+        }
+    }
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float f = raw(v);
+            if constexpr (DT == MIREC_F32)
+                word[v] = __float_as_uint(f > ScoreType<DT>::lowest ? fminf(f, FLT_MAX) : -INFINITY);
+            else if (!(f > ScoreType<DT>::lowest))
+                exclude(v);
         }
     }
 };
@@ -349,10 +429,14 @@ struct Chunk {
 // belongs to wavefront w, so pieces, chunks and lanes are in index order.  CH > 0: a wavefront's CH pieces (S = 1) stay in
 // its registers; CH = 0: each pass reads the row again, S makes at most SM_BINS pieces of it.
 //
-// A cut is a number: with K = (key, complemented index) larger for a better item, what is kept is K >= cut.  It is found
-// by a histogram whose bins are ordered like the items -- first by the score's distance from the best, in 1/32 octaves
-// of the weight, then, should a bin hold more than SM_LIST items, by equal ranges of K -- and by ranking the items of
-// the bin that the border falls into against each other.
+// A cut is the last item that stays (score and index).  It is found by a histogram whose bins are ordered like the items
+// -- first by the score's distance from the best, in 1/32 octaves of the weight, then, should a bin hold more than
+// SM_LIST items, by equal ranges of K = (monotone image of the score, complemented index), which is larger for a better
+// item -- and by ranking the items of the bin that the border falls into against each other.
+//
+// What bounds it: the instructions per score (about 25 for a weight, 10 for a place in a histogram), then the chain of
+// barriers of a row, not the bytes: hence two rows of 512 threads side by side on a compute unit, or one of 1024 where
+// there are fewer rows than compute units.
 template <int DT, int NT, int CH>
 __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,
@@ -401,10 +485,10 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
             __syncthreads();
         }
         // a lane's first item of chunk `sub` of piece p
-        auto first_item = [&](int p, int sub) -> int64_t { return ((int64_t)p * S + sub) * WAVE_CHUNK + lane * V; };
+        auto first_item = [&](int p, int sub) -> int32_t { return (p * S + sub) * WAVE_CHUNK + lane * V; };
         // its 16 bytes; what is excluded or behind the row's end is minus infinity
         auto load = [&](int p, int sub) -> C {
-            const int64_t i = first_item(p, sub);
+            const int32_t i = first_item(p, sub);
             C q;
             if (i + V <= m) {
                 const sm_words x = *reinterpret_cast<const sm_words*>(s + i);
@@ -423,6 +507,7 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                         }
                     }
             }
+            q.settle();
             if (mask_indptr && i < m) {
                 const uint32_t out = liked[i >> 5] >> (i & 31);
 #pragma unroll
@@ -466,30 +551,23 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                     for (int sub = 0; sub < S; ++sub) f(load(p, sub), first_item(p, sub), p, sub);
             }
         };
-        auto order_of = [&](uint32_t key, int64_t first, int v) -> uint64_t {
-            return ((uint64_t)key << 32) | (0xffffffffu - (uint32_t)(first + v));
+        auto order_of = [&](float f, int32_t item) -> uint64_t {
+            return ((uint64_t)sm_order(f) << 32) | (0xffffffffu - (uint32_t)item);
         };
 
         // the best score
-        uint32_t top = 0;
-        each([&](const C& q, int64_t, int, int) {
+        float top = -INFINITY;
+        each([&](const C& q, int32_t, int, int) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const uint32_t k = q.key(v);
-                top = k > top ? k : top;
-            }
+            for (int v = 0; v < V; ++v) top = fmaxf(top, q.score(v));
         });
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            const uint32_t o = (uint32_t)__shfl_xor((int)top, d, 64);
-            top = o > top ? o : top;
-        }
-        if (lane == 0) part[0][wave] = top;
+        top = sm_wave_max(top);
+        if (lane == 0) part[0][wave] = __float_as_uint(top);
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < NW; ++w) top = (uint32_t)part[0][w] > top ? (uint32_t)part[0][w] : top;
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, __uint_as_float((uint32_t)part[0][w]));
         __syncthreads();
-        if (top == 0) {
+        if (!(top > -INFINITY)) {
             for (int d = tid; d < draws; d += NT) {
                 out_ids[row * draws + d] = -1;
                 out_logprob[row * draws + d] = -INFINITY;
@@ -497,23 +575,32 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
             continue;
         }
         const RowCuts cuts = sm_cuts(par, row, m, bits);
-        const float best32 = sm_unorder(top), step32 = (float)(cuts.step * 32.0);
-        const double best = (double)best32;
-        auto weight = [&](uint32_t key) -> uint64_t { return sm_weight(sm_exponent(key, top, best, cuts.step), bits); };
+        const float step32 = cuts.step > 0.0 ? (float)(cuts.step * 32.0) : 32.f;   // (any scale finds the best item)
+        const double best = (double)top;
+        auto weight = [&](float f) -> uint64_t { return sm_weight(f, best, cuts.step, bits); };
         // a bin of the first histogram: in 1/32 octaves below the best, everything from 32 octaves on in the last
-        auto first_bin = [&](uint32_t key) -> int {
-            const float d = key == top ? 0.f : (best32 - sm_unorder(key)) * step32;
-            return d < (float)(SM_BINS - 1) ? (int)d : d != d ? 0 : SM_BINS - 1;
+        auto first_bin = [&](float f) -> uint32_t {
+            const uint32_t b = (uint32_t)((top - f) * step32);
+            return b < SM_BINS - 1 ? b : SM_BINS - 1;
         };
 
-        uint64_t cut = 1ull << 32;   // every item with a key
+        // the last item that stays; at first every item that is not excluded does
+        float cut_f = -INFINITY;
+        int32_t cut_i = -1;
+        auto kept = [&](float f, int32_t item) -> bool { return (f > cut_f) | ((f == cut_f) & (item <= cut_i)); };
+        // whether a wavefront's chunk holds an item that may stay
+        auto any_kept = [&](const C& q) -> bool {
+            float most = q.score(0);
+#pragma unroll
+            for (int v = 1; v < V; ++v) most = fmaxf(most, q.score(v));
+            return __any(most >= cut_f && most > -INFINITY);
+        };
         // Moves `cut` to the item at the border: the target-th in order (by count), or the last item whose
-        // predecessors hold less than the share top_p of the mass at or above `cut`.  Where the row has no border it stays.
+        // predecessors hold less than the share top_p of what stayed so far.  Where the row has no border it stays.
         auto find_cut = [&](auto by_mass, uint64_t target, double top_p) {
             constexpr bool BY_MASS = decltype(by_mass)::value;
             uint64_t base = 0;      // count or mass of the items above the current range
-            uint64_t lo = cut, hi = ~0ull;
-            double bound = 0.0;
+            uint64_t lo = 0, hi = 0, bound = 0;
             int shift = -1;         // -1: the first histogram
             for (;;) {
                 for (int b = tid; b < SM_BINS; b += NT) {
@@ -527,19 +614,33 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                     shared_key[1] = 0;
                 }
                 __syncthreads();
-                auto bin_of = [&](uint64_t K) -> int { return shift < 0 ? first_bin((uint32_t)(K >> 32)) : (int)((hi - K) >> shift); };
-                each([&](const C& q, int64_t first, int p, int sub) {
+                if (shift < 0) {
+                    each([&](const C& q, int32_t first, int, int) {
+                        if (!any_kept(q)) return;
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const uint32_t key = q.key(v);
-                        const uint64_t K = order_of(key, first, v);
-                        if (K >= lo && K <= hi) {
-                            const int b = bin_of(K);
-                            atomicAdd(&count_bins[b], 1u);
-                            if (BY_MASS) atomicAdd((unsigned long long*)&mass_bins[b], (unsigned long long)weight(key));
+                        for (int v = 0; v < V; ++v) {
+                            const float f = q.score(v);
+                            if (kept(f, first + v)) {
+                                const uint32_t b = first_bin(f);
+                                atomicAdd(&count_bins[b], 1u);
+                                if (BY_MASS) atomicAdd((unsigned long long*)&mass_bins[b], (unsigned long long)weight(f));
+                            }
                         }
-                    }
-                });
+                    });
+                } else {
+                    each([&](const C& q, int32_t first, int, int) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            const float f = q.score(v);
+                            const uint64_t K = order_of(f, first + v);
+                            if (K >= lo && K <= hi) {
+                                const int b = (int)((hi - K) >> shift);
+                                atomicAdd(&count_bins[b], 1u);
+                                if (BY_MASS) atomicAdd((unsigned long long*)&mass_bins[b], (unsigned long long)weight(f));
+                            }
+                        }
+                    });
+                }
                 __syncthreads();
                 // running sums over the bins, BINS_PER neighbouring ones per thread
                 uint64_t sum = 0;
@@ -558,7 +659,7 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                     start += w < wave ? part[0][w] : 0ull;
                     all += part[0][w];
                 }
-                if (BY_MASS && shift < 0) bound = top_p * (double)all;
+                if (BY_MASS && shift < 0) bound = sm_bound(top_p, all);
                 // The border's bin.  By count: the one that takes the running count to the target.  By mass: the last
                 // with mass that starts below the bound, or the first with mass.
                 uint64_t at = start;
@@ -566,7 +667,7 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                 uint64_t here_start = 0;
 #pragma unroll
                 for (int i = 0; i < BINS_PER; ++i) {
-                    if (BY_MASS ? mine[i] > 0 && ((double)at < bound || at == base) : at < target && at + mine[i] >= target) {
+                    if (BY_MASS ? mine[i] > 0 && (at < bound || at == base) : at < target && at + mine[i] >= target) {
                         here = tid * BINS_PER + i;
                         here_start = at;
                     }
@@ -580,17 +681,21 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                 __syncthreads();
                 base = shared_key[1];
                 const uint32_t members = count_bins[b];
+                auto member = [&](float f, int32_t item) -> bool {
+                    if (shift < 0) return kept(f, item) & (first_bin(f) == (uint32_t)b);
+                    const uint64_t K = order_of(f, item);
+                    return K >= lo && K <= hi && (int)((hi - K) >> shift) == b;
+                };
                 if (members <= SM_LIST) {
-                    each([&](const C& q, int64_t first, int p, int sub) {
+                    each([&](const C& q, int32_t first, int, int) {
 #pragma unroll
                         for (int v = 0; v < V; ++v) {
-                            const uint32_t key = q.key(v);
-                            const uint64_t K = order_of(key, first, v);
-                            if (K >= lo && K <= hi && bin_of(K) == b) {
+                            const float f = q.score(v);
+                            if (member(f, first + v)) {
                                 ulonglong2 e;
-                                e.x = K;
-                                e.y = BY_MASS ? weight(key) : 1ull;
-                                list[atomicAdd(&shared_int[1], 1u)] = e;
+                                e.x = order_of(f, first + v);
+                                e.y = BY_MASS ? weight(f) : 1ull;
+                                list[atomicAdd(&shared_int[1], 1u) & (SM_LIST - 1)] = e;   // (never more than `members`)
                             }
                         }
                     });
@@ -600,32 +705,34 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                         uint64_t before = base;
 #pragma unroll 8
                         for (uint32_t j = 0; j < members; ++j) before += list[j].x > x.x ? list[j].y : 0ull;
-                        const bool kept = BY_MASS ? x.y > 0 && ((double)before < bound || before == base) : before < target;
-                        if (kept) atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)x.x);
+                        const bool stays = BY_MASS ? x.y > 0 && (before < bound || before == base) : before < target;
+                        if (stays) atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)x.x);
                     }
                     __syncthreads();
-                    cut = shared_key[0];
+                    cut_f = sm_unorder((uint32_t)(shared_key[0] >> 32));
+                    cut_i = (int32_t)(0xffffffffu - (uint32_t)shared_key[0]);
                     __syncthreads();
                     return;
                 }
                 // too many for the list: the bin's range of K, in equal parts
                 if (shift < 0) {
-                    uint64_t first = 0, last = ~0ull;
-                    each([&](const C& q, int64_t i0, int, int) {
+                    uint64_t most = 0, least = ~0ull;
+                    each([&](const C& q, int32_t first, int, int) {
 #pragma unroll
                         for (int v = 0; v < V; ++v) {
-                            const uint64_t K = order_of(q.key(v), i0, v);
-                            if (K >= lo && K <= hi && bin_of(K) == b) {
-                                first = K > first ? K : first;
-                                last = K < last ? K : last;
+                            const float f = q.score(v);
+                            if (member(f, first + v)) {
+                                const uint64_t K = order_of(f, first + v);
+                                most = K > most ? K : most;
+                                least = K < least ? K : least;
                             }
                         }
                     });
                     __syncthreads();
                     if (tid == 0) shared_key[1] = 0;
                     __syncthreads();
-                    atomicMax((unsigned long long*)&shared_key[1], (unsigned long long)first);
-                    atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)last);
+                    atomicMax((unsigned long long*)&shared_key[1], (unsigned long long)most);
+                    atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)least);
                     __syncthreads();
                     hi = shared_key[1];
                     lo = shared_key[0];
@@ -644,19 +751,19 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
         if (cuts.top_p < 1.0) find_cut(std::true_type{}, 0ull, cuts.top_p);
 
         // The kept mass of every piece, then its running sum in index order.
-        auto kept_weight = [&](const C& q, int64_t first, int v) -> uint64_t {
-            const uint32_t key = q.key(v);
-            if (order_of(key, first, v) < cut) return 0ull;
-            const uint64_t w = weight(key);
-            return (double)w >= cuts.floor_w ? w : 0ull;
+        auto kept_weight = [&](float f, int32_t item) -> uint64_t {
+            const uint64_t w = weight(f);
+            return kept(f, item) & (w >= cuts.floor_w) ? w : 0ull;
         };
         for (int p = tid; p < SM_BINS; p += NT) mass_bins[p] = 0;
         __syncthreads();
         {
             uint64_t w = 0;
-            each([&](const C& q, int64_t first, int p, int sub) {
+            each([&](const C& q, int32_t first, int p, int sub) {
+                if (any_kept(q)) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) w += kept_weight(q, first, v);
+                    for (int v = 0; v < V; ++v) w += kept_weight(q.score(v), first + v);
+                }
                 if (sub == S - 1) {
                     w = sm_wave_sum(w);
                     if (lane == 0) mass_bins[p] = w;
@@ -706,12 +813,12 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
             uint64_t run = p > 0 ? mass_bins[p - 1] : 0ull;
             for (int sub = 0; sub < S; ++sub) {
                 const C q = load(p, sub);
-                const int64_t first = first_item(p, sub);
+                const int32_t first = first_item(p, sub);
                 uint64_t w[V], mine_w = 0;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    w[v] = kept_weight(q, first, v);
-                    for (int j = 0; j < taken; ++j) w[v] = gone[j] == (int32_t)(first + v) ? 0ull : w[v];
+                    w[v] = kept_weight(q.score(v), first + v);
+                    for (int j = 0; j < taken; ++j) w[v] = gone[j] == first + v ? 0ull : w[v];
                     mine_w += w[v];
                 }
                 const uint64_t upto = run + sm_wave_scan(mine_w);
@@ -734,13 +841,13 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                     before += w[v];
                 }
                 if (lane == l) {
-                    const int64_t item = first + at_v;
-                    uint32_t key = 0;
+                    const int32_t item = first + at_v;
+                    float f = 0.f;
 #pragma unroll
-                    for (int v = 0; v < V; ++v) key = at_v == v ? q.key(v) : key;
-                    out_ids[row * draws + d] = id ? id[item] : (int32_t)item;
-                    out_logprob[row * draws + d] = sm_logprob(sm_exponent(key, top, best, cuts.step), total, bits);
-                    if (!replacement) gone[taken] = (int32_t)item;
+                    for (int v = 0; v < V; ++v) f = at_v == v ? q.score(v) : f;
+                    out_ids[row * draws + d] = id ? id[item] : item;
+                    out_logprob[row * draws + d] = sm_logprob(f, best, cuts.step, total, bits);
+                    if (!replacement) gone[taken] = item;
                 }
                 if (!replacement) {
                     ++taken;
@@ -767,10 +874,14 @@ static int launch_short(const typename ScoreType<DT>::raw* scores, int64_t n, in
                         int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
                         int draws, int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
                         hipStream_t stream) {
-    const int64_t blocks = (n + 3) / 4;
-    hipLaunchKernelGGL((sample_short_kernel<DT, E>), dim3((unsigned)(blocks < 262144 ? blocks : 262144)), dim3(256), 0, stream,
-                       scores, n, m, stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits,
-                       out_ids, out_logprob);
+    // a row per wavefront until the chip is full (256 compute units of 28 wavefronts), then runs of up to 64
+    int64_t rows_each = n / (256 * 28);
+    rows_each = rows_each < 1 ? 1 : rows_each > 64 ? 64 : rows_each;
+    const int64_t blocks = (n + 4 * rows_each - 1) / (4 * rows_each);
+    MIREC_REQUIRE(blocks < ((int64_t)1 << 24), MIREC_E_UNSUPPORTED, "mirec_sample: more than 2^32 rows");
+    hipLaunchKernelGGL((sample_short_kernel<DT, E>), dim3((unsigned)blocks), dim3(256), 0, stream, scores, n, m, stride, ids,
+                       ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, (int)rows_each, par, bits, out_ids,
+                       out_logprob);
     MIREC_LAUNCH_CHECK();
     return MIREC_OK;
 }
@@ -809,7 +920,10 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
     if (m <= SM_SHORT) return launch_short<DT, 4>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     constexpr int V = Chunk<DT>::V;
     if (m <= 256 * V * 8) return launch_long<DT, 256, 8>(scores, n, m, MIREC_SAMPLE_ARGS);
-    if (m <= 512 * V * 16) return launch_long<DT, 512, 16>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (m <= 1024 * V * 8) {
+        if (n <= SM_FEW_ROWS) return launch_long<DT, 1024, 8>(scores, n, m, MIREC_SAMPLE_ARGS);
+        return launch_long<DT, 512, 16>(scores, n, m, MIREC_SAMPLE_ARGS);
+    }
     return launch_long<DT, 1024, 0>(scores, n, m, MIREC_SAMPLE_ARGS);
 #undef MIREC_SAMPLE_ARGS
 }
@@ -835,7 +949,7 @@ extern "C" int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m,
                   "mirec_sample: unknown score type %d", dtype);
     MIREC_REQUIRE(draws <= SM_MAX_DRAWS, MIREC_E_UNSUPPORTED, "mirec_sample: %d draws a row; at most %d are supported",
                   draws, SM_MAX_DRAWS);
-    MIREC_REQUIRE(m < ((int64_t)1 << 31), MIREC_E_UNSUPPORTED, "mirec_sample: more than 2^31 items");
+    MIREC_REQUIRE(m <= ((int64_t)1 << 30), MIREC_E_UNSUPPORTED, "mirec_sample: more than 2^30 items");
     MIREC_REQUIRE(row_temperature || (temperature >= 0.0 && temperature < INFINITY), MIREC_E_INVALID,
                   "mirec_sample: temperature must be finite and not negative (got %g)", temperature);
     MIREC_REQUIRE(row_top_p || (top_p >= 0.0 && top_p <= 1.0), MIREC_E_INVALID,
@@ -856,13 +970,13 @@ extern "C" int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m,
     par.greedy = !(temperature >= SM_MIN_TEMPERATURE);
     par.step = par.greedy ? 0.0 : 1.4426950408889634 / temperature;
     par.top_p = top_p;
-    par.min_p = min_p;
     par.top_k = top_k;
     par.row_temperature = row_temperature;
     par.row_top_k = row_top_k;
     par.row_top_p = row_top_p;
     par.row_min_p = row_min_p;
     const int bits = sample_bits(m);
+    par.floor_w = (uint64_t)std::ceil(min_p * (double)(1ull << bits));
     switch (dtype) {
         case MIREC_F32:
             return launch_sample<MIREC_F32>(scores, n, m, row_stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws,

@@ -1,8 +1,8 @@
 """Drawing items from scores: engine.sample_scores / mirec_sample against a float64 statement of its definition.
 
 A draw is checked by the interval of (0, 1) that belongs to the item: the device's running sum may sit off the float64 one
-by the weights' own error.  A weight is 2^f by a power series whose first dropped term is below 2.2e-13 of it, in
-float64 arithmetic (a dozen roundings, each 2^-53), rounded to S = min(51, 62 - ceil(log2 m)) fraction bits; with the
+by the weights' own error.  A weight is 2^f by a polynomial within 1.6e-14 of it, its exponent a product of float64 numbers below 2^7
+(2^-46 ln 2 of it at most) in float64 arithmetic (a dozen roundings, each 2^-53), rounded to S = min(51, 62 - ceil(log2 m)) fraction bits; with the
 largest weight 1 the borders of the normalised running sum are off by at most 2 (3e-13 + m 2^-(S+1)).  The logarithm of
 the probability carries the same and one rounding to fp32 (half a step: 2^-24 of it)."""
 
@@ -104,7 +104,7 @@ def call(scores=16, dtype=0, n=2, m=4, stride=4, ids=None, ids_stride=0, indptr=
 
 @pytest.mark.parametrize("change,code,text", [
     ({"n": -1}, -1, "negative"), ({"m": -1}, -1, "negative"), ({"draws": -1}, -1, "negative"),
-    ({"dtype": 3}, -1, "type"), ({"draws": 1025}, -4, "1024"), ({"m": 1 << 31}, -4, "2^31"),
+    ({"dtype": 3}, -1, "type"), ({"draws": 1025}, -4, "1024"), ({"m": (1 << 30) + 1}, -4, "2^30"),
     ({"T": -0.5}, -1, "temperature"), ({"T": float("nan")}, -1, "temperature"), ({"T": float("inf")}, -1, "temperature"),
     ({"p": -0.1}, -1, "top_p"), ({"p": 1.1}, -1, "top_p"), ({"p": float("nan")}, -1, "top_p"),
     ({"q": -0.1}, -1, "min_p"), ({"q": 1.1}, -1, "min_p"), ({"k": -1}, -1, "top_k"),
