@@ -22,7 +22,9 @@ constexpr int64_t SM_MAX_MASKED_ITEMS = MIREC_SAMPLE_MAX_MASKED_ITEMS;   // the 
 constexpr double SM_MIN_TEMPERATURE = 1e-37;      // below: greedy
 constexpr int SM_SHORT = 256;                     // rows up to this length: one wavefront each
 constexpr int64_t SM_FEW_ROWS = 256;              // no more rows than compute units: larger workgroups
+constexpr int SM_AHEAD = 2;                       // loads in flight ahead of the work
 constexpr int SM_BINS = 1024;                     // of a histogram over a row
+constexpr int SM_FEW = 256;                        // entries that one wavefront finishes
 constexpr int SM_LIST = 512;                     // entries that are ranked against each other in LDS
 
 struct SampleParams {
@@ -95,16 +97,17 @@ __device__ __forceinline__ double sm_exp2_fraction(double f) {
 constexpr double SM_ROUND = 6755399441055744.0;   // 1.5 2^52: the sum's low bits are the nearest integer
 
 // The weight of a score: 2^((s - best) step) with `bits` (at most 51) fraction bits, the nearest such number; 0 for minus
-// infinity.  Vector float64 instructions run at the rate of float32 ones here, and about twenty of them are all there is.
-__device__ __forceinline__ uint64_t sm_weight(float score, double best, double step, int bits) {
+// infinity.  Vector float64 instructions run at the rate of float32 ones here, and about twenty of them are all there is:
+// adding 2^(52 - bits) rounds and leaves the integer in the mantissa.
+__device__ __forceinline__ uint64_t sm_weight(float score, double best, double step, double rounder) {
     const double t = fmax(((double)score - best) * step, -80.0);   // (a NaN, infinity times zero, becomes -80 too)
     const double k = t + SM_ROUND;
     const double p = sm_exp2_fraction(t - (k - SM_ROUND));
-    // 2^(k + bits) into the exponent, 2^52 to round, the integer out of the mantissa
-    const double v = __longlong_as_double(__double_as_longlong(p) + ((int64_t)((int)(uint32_t)__double_as_longlong(k) + bits) << 52)) +
-                     4503599627370496.0;
+    const double v = __hiloint2double(__double2hiint(p) + (__double2loint(k) << 20), __double2loint(p)) + rounder;   // p 2^k
     return (uint64_t)__double_as_longlong(v) & 0xfffffffffffffull;
 }
+
+__device__ __forceinline__ double sm_rounder(int bits) { return __hiloint2double((1023 + 52 - bits) << 20, 0); }   // 2^(52 - bits)
 
 // log2 x of a positive normal number to 1e-13 or so: the fp32 logarithm, then one Newton step with the power above.
 __device__ __forceinline__ double sm_log2(double x) {
@@ -211,6 +214,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
     const float* __restrict__ uniforms, int draws, int replacement, int rows_each, SampleParams par, int bits,
     int32_t* __restrict__ out_ids, float* __restrict__ out_logprob) {
     const int lane = threadIdx.x & 63;
+    const double rounder = sm_rounder(bits);
     const int64_t row0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * rows_each;
     const int64_t row1 = row0 + rows_each < n ? row0 + rows_each : n;
     // draws that are not written yet, in lanes 0 .. waiting - 1: number out0 + lane
@@ -258,7 +262,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
         const double best = (double)best32;
         uint64_t w[E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) w[j] = sm_weight(f[j], best, cut.step, bits);
+        for (int j = 0; j < E; ++j) w[j] = sm_weight(f[j], best, cut.step, rounder);
 
         // in order if no item is better than the one before it (the next lane's first: minus infinity after lane 63)
         float before_f = __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(f[0]), 0x130, 0xf, 0xf, false));
@@ -390,8 +394,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
 // Scores of 16 bytes, from any address that is aligned to their type.
 typedef uint32_t sm_words __attribute__((ext_vector_type(4), aligned(2)));
 
-typedef uint32_t sm_held __attribute__((ext_vector_type(32)));   // eight chunks
-
+typedef uint16_t sm_u16x2 __attribute__((ext_vector_type(2)));
 template <int DT>
 struct Chunk {
     static constexpr int V = DT == MIREC_F32 ? 4 : 8;   // scores of a thread's 16 bytes
@@ -411,6 +414,24 @@ struct Chunk {
         else {
             const uint32_t inf = DT == MIREC_BF16 ? 0xff80u : 0xfc00u;
             word[v >> 1] = v & 1 ? (word[v >> 1] & 0xffffu) | (inf << 16) : (word[v >> 1] & 0xffff0000u) | inf;
+        }
+    }
+    // Whether a score is not below the largest finite magnitude: it may be one that is excluded, or infinite.
+    __device__ __forceinline__ bool unsettled() const {
+        if constexpr (DT == MIREC_F32) {
+            uint32_t most = word[0] & 0x7fffffffu;
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                const uint32_t a = word[i] & 0x7fffffffu;
+                most = a > most ? a : most;
+            }
+            return most >= 0x7f7fffffu;
+        } else {
+            sm_u16x2 most = __builtin_bit_cast(sm_u16x2, word[0] & 0x7fff7fffu);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(sm_u16x2, word[i] & 0x7fff7fffu));
+            const uint16_t limit = DT == MIREC_BF16 ? 0x7f7f : 0x7bff;
+            return most[0] >= limit || most[1] >= limit;
         }
     }
     __device__ __forceinline__ void settle() {
@@ -437,8 +458,8 @@ struct Chunk {
 // What bounds it: the instructions per score (about 25 for a weight, 10 for a place in a histogram), then the chain of
 // barriers of a row, not the bytes: hence two rows of 512 threads side by side on a compute unit, or one of 1024 where
 // there are fewer rows than compute units.
-template <int DT, int NT, int CH>
-__global__ __launch_bounds__(NT, 4) void sample_long_kernel(
+template <int DT, int NT>
+__global__ __launch_bounds__(NT, 6) void sample_long_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,
     const int32_t* __restrict__ ids, int64_t ids_stride, const int64_t* __restrict__ mask_indptr,
     const int32_t* __restrict__ mask_indices, const float* __restrict__ uniforms, int draws, int replacement,
@@ -446,7 +467,6 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
     typedef Chunk<DT> C;
     constexpr int V = C::V, NW = NT / 64, WAVE_CHUNK = 64 * V;
     constexpr int BINS_PER = SM_BINS / NT;
-    constexpr int HELD = CH / 8;          // registers that hold the row, by 32
     extern __shared__ uint32_t liked[];   // one bit per item, when there is a filter
     __shared__ __attribute__((aligned(16))) ulonglong2 list[SM_LIST];   // K and weight
     __shared__ uint64_t mass_bins[SM_BINS];
@@ -456,8 +476,9 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
     __shared__ uint32_t shared_int[2];
     __shared__ int32_t gone[SM_MAX_DRAWS];   // items drawn so far, when they do not come back
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const double rounder = sm_rounder(bits);
     const int64_t row_chunks = (m + WAVE_CHUNK - 1) / WAVE_CHUNK;
-    const int S = CH > 0 ? 1 : (int)((row_chunks + SM_BINS - 1) / SM_BINS);
+    const int S = (int)((row_chunks + SM_BINS - 1) / SM_BINS);
     const int pieces = (int)((row_chunks + S - 1) / S);   // at most SM_BINS
 
     auto block_sum = [&](uint64_t v) -> uint64_t {
@@ -486,17 +507,17 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
         }
         // a lane's first item of chunk `sub` of piece p
         auto first_item = [&](int p, int sub) -> int32_t { return (p * S + sub) * WAVE_CHUNK + lane * V; };
-        // its 16 bytes; what is excluded or behind the row's end is minus infinity
+        // its 16 bytes (minus infinity behind the row's end), and what is excluded set to minus infinity
         auto load = [&](int p, int sub) -> C {
             const int32_t i = first_item(p, sub);
             C q;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) q.word[v] = DT == MIREC_F32 ? 0xff800000u : DT == MIREC_BF16 ? 0xff80ff80u : 0xfc00fc00u;
             if (i + V <= m) {
                 const sm_words x = *reinterpret_cast<const sm_words*>(s + i);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) q.word[v] = x[v];
-            } else {
-#pragma unroll
-                for (int v = 0; v < 4; ++v) q.word[v] = DT == MIREC_F32 ? 0xff800000u : DT == MIREC_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+            } else if (i < m) {
 #pragma unroll
                 for (int v = 0; v < V; ++v)
                     if (i + v < m) {
@@ -507,61 +528,66 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                         }
                     }
             }
-            q.settle();
-            if (mask_indptr && i < m) {
-                const uint32_t out = liked[i >> 5] >> (i & 31);
+            return q;
+        };
+        auto filter = [&](C& q, int32_t i) {
+            if (__any(q.unsettled())) q.settle();
+            if (mask_indptr) {
+                const uint32_t out = i < m ? (liked[i >> 5] >> (i & 31)) & ((1u << V) - 1) : 0u;
+                if (__any(out != 0)) {
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if ((out >> v) & 1u) q.exclude(v);
+                    for (int v = 0; v < V; ++v)
+                        if ((out >> v) & 1u) q.exclude(v);
+                }
             }
             if (id) {
 #pragma unroll
                 for (int v = 0; v < V; ++v)
                     if (i + v < m && id[i + v] < 0) q.exclude(v);
             }
-            return q;
         };
-        // The row's chunks in registers, taken out one at a time by a number that is the same in all lanes: the passes are
-        // loops over the chunks, and not CH copies of their body (which neither fit the instruction cache nor, with what
-        // the compiler then carries from copy to copy, the registers).
-        sm_held held[HELD > 0 ? HELD : 1];
-        if constexpr (CH > 0) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const C q = load(c * NW + wave, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) held[c / 8][c % 8 * 4 + i] = q.word[i];
-            }
-        }
-        // f(chunk, the lane's first item, its piece, number within the piece) for every chunk of this wavefront, in order
+        // f(chunk, the lane's first item, its piece, number within the piece) for every chunk of this wavefront, in order,
+        // SM_AHEAD loads ahead of the work
         auto each = [&](auto&& f) {
-            if constexpr (CH > 0) {
+            const int mine = wave < pieces ? ((pieces - wave - 1) / NW + 1) * S : 0;
+            C ahead[SM_AHEAD];
+            int lp = wave, lsub = 0;   // the chunk to load next
+            auto fetch = [&](C& q) {
+                if (lp < pieces) q = load(lp, lsub);
+                if (++lsub == S) {
+                    lsub = 0;
+                    lp += NW;
+                }
+            };
 #pragma unroll
-                for (int h = 0; h < HELD; ++h)
-#pragma nounroll
-                    for (int c = 0; c < 8 && (h * 8 + c) * NW + wave < pieces; ++c) {
-                        C q;
+            for (int u = 0; u < SM_AHEAD; ++u) fetch(ahead[u]);
+            int p = wave, sub = 0;
+            for (int c = 0; c < mine; c += SM_AHEAD)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) q.word[i] = held[h][c * 4 + i];
-                        f(q, first_item((h * 8 + c) * NW + wave, 0), (h * 8 + c) * NW + wave, 0);
+                for (int u = 0; u < SM_AHEAD; ++u)
+                    if (c + u < mine) {
+                        C q = ahead[u];
+                        fetch(ahead[u]);
+                        const int32_t first = first_item(p, sub);
+                        filter(q, first);
+                        f(q, first, p, sub);
+                        if (++sub == S) {
+                            sub = 0;
+                            p += NW;
+                        }
                     }
-            } else {
-#pragma nounroll
-                for (int p = wave; p < pieces; p += NW)
-                    for (int sub = 0; sub < S; ++sub) f(load(p, sub), first_item(p, sub), p, sub);
-            }
         };
         auto order_of = [&](float f, int32_t item) -> uint64_t {
             return ((uint64_t)sm_order(f) << 32) | (0xffffffffu - (uint32_t)item);
         };
 
         // the best score
-        float top = -INFINITY;
+        float own_top = -INFINITY;
         each([&](const C& q, int32_t, int, int) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) top = fmaxf(top, q.score(v));
+            for (int v = 0; v < V; ++v) own_top = fmaxf(own_top, q.score(v));
         });
-        top = sm_wave_max(top);
+        float top = sm_wave_max(own_top);
         if (lane == 0) part[0][wave] = __float_as_uint(top);
         __syncthreads();
 #pragma unroll
@@ -577,12 +603,179 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
         const RowCuts cuts = sm_cuts(par, row, m, bits);
         const float step32 = cuts.step > 0.0 ? (float)(cuts.step * 32.0) : 32.f;   // (any scale finds the best item)
         const double best = (double)top;
-        auto weight = [&](float f) -> uint64_t { return sm_weight(f, best, cuts.step, bits); };
+        auto weight = [&](float f) -> uint64_t { return sm_weight(f, best, cuts.step, rounder); };
         // a bin of the first histogram: in 1/32 octaves below the best, everything from 32 octaves on in the last
         auto first_bin = [&](float f) -> uint32_t {
             const uint32_t b = (uint32_t)((top - f) * step32);
             return b < SM_BINS - 1 ? b : SM_BINS - 1;
         };
+
+        // The bin in which a running sum over the bins, from `base` on, satisfies here(sum before it, its own); -1 if none
+        // does.  Leaves the sum before the bin in shared_key[1]; `all`: the sum over all bins.
+        auto find_bin = [&](auto bins, uint64_t base, auto&& here, uint64_t& all) -> int {
+            uint64_t sum = 0, mine[BINS_PER];
+#pragma unroll
+            for (int i = 0; i < BINS_PER; ++i) {
+                mine[i] = (uint64_t)bins[tid * BINS_PER + i];
+                sum += mine[i];
+            }
+            const uint64_t inc = sm_wave_scan(sum);
+            if (lane == 63) part[0][wave] = inc;
+            if (tid == 0) {
+                shared_int[0] = 0;
+                shared_key[1] = 0;
+            }
+            __syncthreads();
+            uint64_t at = base + inc - sum;
+            all = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                at += w < wave ? part[0][w] : 0ull;
+                all += part[0][w];
+            }
+            int found = -1;
+            uint64_t found_at = 0;
+#pragma unroll
+            for (int i = 0; i < BINS_PER; ++i) {
+                if (here(at, mine[i], all)) {
+                    found = tid * BINS_PER + i;
+                    found_at = at;
+                }
+                at += mine[i];
+            }
+            if (found >= 0) atomicMax(&shared_int[0], (uint32_t)found + 1);
+            __syncthreads();
+            const int b = (int)shared_int[0] - 1;
+            if (found == b && b >= 0) shared_key[1] = found_at;
+            __syncthreads();
+            return b;
+        };
+
+        // A handful of items are to stay.  The top_k-th best of the threads' own best scores is not above the row's
+        // top_k-th best score, and few scores are above it: those go to a list, and one wavefront does the rest there.
+        if (cuts.top_k <= SM_FEW / 2) {
+            for (int b = tid; b < SM_BINS; b += NT) count_bins[b] = 0;
+            if (tid == 0) shared_int[1] = 0;
+            __syncthreads();
+            if (own_top > -INFINITY) atomicAdd(&count_bins[first_bin(own_top)], 1u);
+            __syncthreads();
+            uint64_t all;
+            const int found = find_bin(count_bins, 0, [&](uint64_t at, uint64_t mine, uint64_t) { return at < (uint64_t)cuts.top_k && at + mine >= (uint64_t)cuts.top_k; }, all);
+            const uint32_t last_bin = found >= 0 ? (uint32_t)found : SM_BINS - 1;   // (fewer threads with scores: all of them)
+            each([&](const C& q, int32_t first, int, int) {
+                float most = q.score(0);
+#pragma unroll
+                for (int v = 1; v < V; ++v) most = fmaxf(most, q.score(v));
+                if (!__any(most > -INFINITY && first_bin(most) <= last_bin)) return;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float f = q.score(v);
+                    if (f > -INFINITY && first_bin(f) <= last_bin) {
+                        const uint32_t e = atomicAdd(&shared_int[1], 1u);
+                        if (e < SM_FEW) list[e].x = order_of(f, first + v);
+                    }
+                }
+            });
+            __syncthreads();
+            const uint32_t have = shared_int[1];
+            if (have <= SM_FEW) {
+                if (wave != 0) continue;
+                constexpr int SLOTS = SM_FEW / 64;
+                uint64_t K[SLOTS], w[SLOTS], run[SLOTS];
+                float f[SLOTS];
+#pragma unroll
+                for (int i = 0; i < SLOTS; ++i) {
+                    const uint32_t e = lane + 64 * i;
+                    K[i] = e < have ? list[e].x : 0ull;
+                    f[i] = sm_unorder((uint32_t)(K[i] >> 32));
+                    w[i] = 0;
+                    if (64 * i < (int)have && e < have) {
+                        w[i] = weight(f[i]);
+                        list[e].y = w[i];
+                    }
+                }
+                asm volatile("" ::: "memory");
+                // place and mass before it, in rank order
+                uint32_t rank[SLOTS];
+                uint64_t before[SLOTS], mass = 0;
+#pragma unroll
+                for (int i = 0; i < SLOTS; ++i) {
+                    rank[i] = 0;
+                    before[i] = 0;
+                }
+#pragma unroll 4
+                for (uint32_t j = 0; j < have; ++j) {
+                    const ulonglong2 x = list[j];
+#pragma unroll
+                    for (int i = 0; i < SLOTS; ++i)
+                        if (64 * i < (int)have) {
+                            rank[i] += x.x > K[i] ? 1u : 0u;
+                            before[i] += x.x > K[i] ? x.y : 0ull;
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < SLOTS; ++i) {
+                    w[i] = rank[i] < cuts.top_k ? w[i] : 0ull;
+                    mass += w[i];
+                }
+                const uint64_t bound = cuts.top_p < 1.0 ? sm_bound(cuts.top_p, sm_wave_sum(mass)) : ~0ull;
+                mass = 0;
+#pragma unroll
+                for (int i = 0; i < SLOTS; ++i) {
+                    w[i] = (rank[i] == 0 || before[i] < bound) && w[i] >= cuts.floor_w ? w[i] : 0ull;
+                    mass += w[i];
+                    const uint32_t e = lane + 64 * i;
+                    if (64 * i < (int)have && e < have) list[e].y = w[i];
+                    run[i] = 0;
+                }
+                uint64_t total = sm_wave_sum(mass);
+                asm volatile("" ::: "memory");
+                // running sums in index order: a larger complement is a smaller index
+#pragma unroll 4
+                for (uint32_t j = 0; j < have; ++j) {
+                    const ulonglong2 x = list[j];
+#pragma unroll
+                    for (int i = 0; i < SLOTS; ++i)
+                        if (64 * i < (int)have) run[i] += (uint32_t)x.x >= (uint32_t)K[i] ? x.y : 0ull;
+                }
+                for (int d = 0; d < draws; ++d) {
+                    if (total == 0) {
+                        if (lane == 0) {
+                            out_ids[row * draws + d] = -1;
+                            out_logprob[row * draws + d] = -INFINITY;
+                        }
+                        continue;
+                    }
+                    const uint64_t t = sm_target(uniforms[row * draws + d], total);
+                    uint64_t out_K = 0, out_w = 0;
+                    float out_f = 0.f;
+#pragma unroll
+                    for (int i = 0; i < SLOTS; ++i) {
+                        const bool here = w[i] != 0 && run[i] > t && run[i] - w[i] <= t;
+                        out_K = here ? K[i] : out_K;
+                        out_w = here ? w[i] : out_w;
+                        out_f = here ? f[i] : out_f;
+                    }
+                    if (out_w != 0) {
+                        const int32_t item = (int32_t)(0xffffffffu - (uint32_t)out_K);
+                        out_ids[row * draws + d] = id ? id[item] : item;
+                        out_logprob[row * draws + d] = sm_logprob(out_f, best, cuts.step, total, bits);
+                    }
+                    if (!replacement) {
+                        const int l = __builtin_ctzll(__ballot(out_w != 0));
+                        const uint64_t gone = sm_lane(out_K, l), less = sm_lane(out_w, l);
+                        total -= less;
+#pragma unroll
+                        for (int i = 0; i < SLOTS; ++i) {
+                            run[i] -= (uint32_t)gone >= (uint32_t)K[i] ? less : 0ull;
+                            w[i] = K[i] == gone ? 0ull : w[i];
+                        }
+                    }
+                }
+                continue;
+            }
+            __syncthreads();   // the list overflowed: the cuts below
+        }
 
         // the last item that stays; at first every item that is not excluded does
         float cut_f = -INFINITY;
@@ -604,27 +797,25 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
             int shift = -1;         // -1: the first histogram
             for (;;) {
                 for (int b = tid; b < SM_BINS; b += NT) {
-                    count_bins[b] = 0;
                     if (BY_MASS) mass_bins[b] = 0;
+                    else count_bins[b] = 0;
                 }
                 if (tid == 0) {
-                    shared_int[0] = 0;   // the bin, plus one
                     shared_int[1] = 0;   // entries in the list
                     shared_key[0] = ~0ull;
-                    shared_key[1] = 0;
                 }
                 __syncthreads();
+                auto count = [&](uint32_t b, float f) {
+                    if (BY_MASS) atomicAdd((unsigned long long*)&mass_bins[b], (unsigned long long)weight(f));
+                    else atomicAdd(&count_bins[b], 1u);
+                };
                 if (shift < 0) {
                     each([&](const C& q, int32_t first, int, int) {
                         if (!any_kept(q)) return;
 #pragma unroll
                         for (int v = 0; v < V; ++v) {
                             const float f = q.score(v);
-                            if (kept(f, first + v)) {
-                                const uint32_t b = first_bin(f);
-                                atomicAdd(&count_bins[b], 1u);
-                                if (BY_MASS) atomicAdd((unsigned long long*)&mass_bins[b], (unsigned long long)weight(f));
-                            }
+                            if (kept(f, first + v)) count(first_bin(f), f);
                         }
                     });
                 } else {
@@ -633,72 +824,43 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
                         for (int v = 0; v < V; ++v) {
                             const float f = q.score(v);
                             const uint64_t K = order_of(f, first + v);
-                            if (K >= lo && K <= hi) {
-                                const int b = (int)((hi - K) >> shift);
-                                atomicAdd(&count_bins[b], 1u);
-                                if (BY_MASS) atomicAdd((unsigned long long*)&mass_bins[b], (unsigned long long)weight(f));
-                            }
+                            if (K >= lo && K <= hi) count((uint32_t)((hi - K) >> shift), f);
                         }
                     });
                 }
                 __syncthreads();
-                // running sums over the bins, BINS_PER neighbouring ones per thread
-                uint64_t sum = 0;
-                uint64_t mine[BINS_PER];
-#pragma unroll
-                for (int i = 0; i < BINS_PER; ++i) {
-                    mine[i] = BY_MASS ? mass_bins[tid * BINS_PER + i] : (uint64_t)count_bins[tid * BINS_PER + i];
-                    sum += mine[i];
-                }
-                const uint64_t inc = sm_wave_scan(sum);
-                if (lane == 63) part[0][wave] = inc;
-                __syncthreads();
-                uint64_t start = base + inc - sum, all = 0;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    start += w < wave ? part[0][w] : 0ull;
-                    all += part[0][w];
-                }
-                if (BY_MASS && shift < 0) bound = sm_bound(top_p, all);
                 // The border's bin.  By count: the one that takes the running count to the target.  By mass: the last
                 // with mass that starts below the bound, or the first with mass.
-                uint64_t at = start;
-                int here = -1;
-                uint64_t here_start = 0;
-#pragma unroll
-                for (int i = 0; i < BINS_PER; ++i) {
-                    if (BY_MASS ? mine[i] > 0 && (at < bound || at == base) : at < target && at + mine[i] >= target) {
-                        here = tid * BINS_PER + i;
-                        here_start = at;
-                    }
-                    at += mine[i];
-                }
-                if (here >= 0) atomicMax(&shared_int[0], (uint32_t)here + 1);
-                __syncthreads();
-                const int b = (int)shared_int[0] - 1;
+                uint64_t all;
+                int b;
+                if constexpr (BY_MASS)
+                    b = find_bin(mass_bins, base, [&](uint64_t at, uint64_t mine, uint64_t sum) {
+                        if (shift < 0) bound = sm_bound(top_p, sum);
+                        return mine > 0 && (at < bound || at == base);
+                    }, all);
+                else
+                    b = find_bin(count_bins, base, [&](uint64_t at, uint64_t mine, uint64_t) { return at < target && at + mine >= target; }, all);
                 if (b < 0) return;   // by count: fewer items than the target
-                if (here == b) shared_key[1] = here_start;
-                __syncthreads();
                 base = shared_key[1];
-                const uint32_t members = count_bins[b];
                 auto member = [&](float f, int32_t item) -> bool {
-                    if (shift < 0) return kept(f, item) & (first_bin(f) == (uint32_t)b);
+                    if (shift < 0) return first_bin(f) == (uint32_t)b && kept(f, item);
                     const uint64_t K = order_of(f, item);
                     return K >= lo && K <= hi && (int)((hi - K) >> shift) == b;
                 };
-                if (members <= SM_LIST) {
-                    each([&](const C& q, int32_t first, int, int) {
+                each([&](const C& q, int32_t first, int, int) {
 #pragma unroll
-                        for (int v = 0; v < V; ++v) {
-                            const float f = q.score(v);
-                            if (member(f, first + v)) {
-                                ulonglong2 e;
-                                e.x = order_of(f, first + v);
-                                e.y = BY_MASS ? weight(f) : 1ull;
-                                list[atomicAdd(&shared_int[1], 1u) & (SM_LIST - 1)] = e;   // (never more than `members`)
-                            }
+                    for (int v = 0; v < V; ++v) {
+                        const float f = q.score(v);
+                        if (member(f, first + v)) {
+                            const uint32_t e = atomicAdd(&shared_int[1], 1u);
+                            if (e < SM_LIST) list[e].x = order_of(f, first + v);
                         }
-                    });
+                    }
+                });
+                __syncthreads();
+                const uint32_t members = shared_int[1];
+                if (members <= SM_LIST) {
+                    for (uint32_t e = tid; e < members; e += NT) list[e].y = BY_MASS ? weight(sm_unorder((uint32_t)(list[e].x >> 32))) : 1ull;
                     __syncthreads();
                     for (uint32_t e = tid; e < members; e += NT) {
                         const ulonglong2 x = list[e];
@@ -755,12 +917,16 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
             const uint64_t w = weight(f);
             return kept(f, item) & (w >= cuts.floor_w) ? w : 0ull;
         };
+        const bool uncut = cut_f == -INFINITY && cuts.floor_w == 0;   // an excluded item has no weight
         for (int p = tid; p < SM_BINS; p += NT) mass_bins[p] = 0;
         __syncthreads();
         {
             uint64_t w = 0;
             each([&](const C& q, int32_t first, int p, int sub) {
-                if (any_kept(q)) {
+                if (uncut) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) w += weight(q.score(v));
+                } else if (any_kept(q)) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) w += kept_weight(q.score(v), first + v);
                 }
@@ -812,8 +978,9 @@ __global__ __launch_bounds__(NT, 4) void sample_long_kernel(
             const int p = p16 * (SM_BINS / 64) + __builtin_ctzll(__ballot(lane >= SM_BINS / 64 || mass_bins[p16 * (SM_BINS / 64) + (lane & (SM_BINS / 64 - 1))] > t));
             uint64_t run = p > 0 ? mass_bins[p - 1] : 0ull;
             for (int sub = 0; sub < S; ++sub) {
-                const C q = load(p, sub);
+                C q = load(p, sub);
                 const int32_t first = first_item(p, sub);
+                filter(q, first);
                 uint64_t w[V], mine_w = 0;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
@@ -886,7 +1053,7 @@ static int launch_short(const typename ScoreType<DT>::raw* scores, int64_t n, in
     return MIREC_OK;
 }
 
-template <int DT, int NT, int CH>
+template <int DT, int NT>
 static int launch_long(const typename ScoreType<DT>::raw* scores, int64_t n, int64_t m, int64_t stride, const int32_t* ids,
                        int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
                        int draws, int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
@@ -896,12 +1063,12 @@ static int launch_long(const typename ScoreType<DT>::raw* scores, int64_t n, int
     bool* done = once.slot();
     MIREC_REQUIRE(done, MIREC_E_HIP, "mirec_sample: cannot read the current device");
     if (!*done) {
-        MIREC_HIP(hipFuncSetAttribute((const void*)sample_long_kernel<DT, NT, CH>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        MIREC_HIP(hipFuncSetAttribute((const void*)sample_long_kernel<DT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)(SM_MAX_MASKED_ITEMS / 8)));
         *done = true;
     }
     const size_t lds = mask_indptr ? (size_t)((m + 31) / 32) * 4 : 0;
-    hipLaunchKernelGGL((sample_long_kernel<DT, NT, CH>), dim3((unsigned)(n < 262144 ? n : 262144)), dim3(NT), lds, stream, scores,
+    hipLaunchKernelGGL((sample_long_kernel<DT, NT>), dim3((unsigned)(n < 262144 ? n : 262144)), dim3(NT), lds, stream, scores,
                        n, m, stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids,
                        out_logprob);
     MIREC_LAUNCH_CHECK();
@@ -918,13 +1085,9 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
     if (m <= 64) return launch_short<DT, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= 128) return launch_short<DT, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= SM_SHORT) return launch_short<DT, 4>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
-    constexpr int V = Chunk<DT>::V;
-    if (m <= 256 * V * 8) return launch_long<DT, 256, 8>(scores, n, m, MIREC_SAMPLE_ARGS);
-    if (m <= 1024 * V * 8) {
-        if (n <= SM_FEW_ROWS) return launch_long<DT, 1024, 8>(scores, n, m, MIREC_SAMPLE_ARGS);
-        return launch_long<DT, 512, 16>(scores, n, m, MIREC_SAMPLE_ARGS);
-    }
-    return launch_long<DT, 1024, 0>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (n <= SM_FEW_ROWS && m > 8192) return launch_long<DT, 1024>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (m > 8192) return launch_long<DT, 512>(scores, n, m, MIREC_SAMPLE_ARGS);
+    return launch_long<DT, 256>(scores, n, m, MIREC_SAMPLE_ARGS);
 #undef MIREC_SAMPLE_ARGS
 }
 
