@@ -60,6 +60,8 @@ struct DistillTile {
     static constexpr int NT = F / 32;          // tiles of columns
     static constexpr int PLANE = 64 * F;       // bytes of one plane, either kind
     static constexpr int BYTES = 256 * F;
+    // tiles in LDS at once: a narrow tile's work (0.6 us at F = 64) is shorter than the way of the next one from L2
+    static constexpr int STAGES_FORWARD = F <= 96 ? 4 : 3, STAGES_BACKWARD = F <= 96 ? 4 : F <= 128 ? 3 : 2;
 };
 
 // Workspace of a call pair (host side): what mirec_distill_loss leaves for mirec_distill_grad, and scratch.
@@ -111,7 +113,7 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.start_off = take((size_t)w.xtiles * (w.ytiles + 1) * 2);
     w.place_off = take((size_t)n * k * 2);
     w.gval_off = take((size_t)n * k * 4);
-    w.row_off = take((size_t)n * 16);         // what a row brings to the backward pass
+    w.row_off = take((size_t)w.xtiles * 32 * 16);   // what a row brings to the backward pass
     w.base_off = take((size_t)n * f * 4);     // dX_b / (grad_b T)
     w.ximg_off = take((size_t)w.xtiles * 256 * f);
     w.yimg_off = take((size_t)w.ytiles * 256 * f);
@@ -161,8 +163,16 @@ __global__ __launch_bounds__(DI_MAX_THREADS) void distill_absmax_kernel(const fl
     }
 }
 
-// Power of two that puts the largest magnitude into [2^14, 2^15), within 2^+-100 (1 where there is none, or it is not
-// finite).  Called by a whole wavefront.
+// Exponent of the power of two that puts the largest magnitude (a bit pattern) into [2^14, 2^15), within 2^+-100 (2^0
+// where there is none, or it is not finite).
+__device__ __forceinline__ int di_exponent_of(uint32_t top) {
+    const int e = (int)(top >> 23);   // |v| in [2^(e - 127), 2^(e - 126))
+    if (top == 0 || e == 255) return 0;
+    const int s = 14 + 127 - e;
+    return s > 100 ? 100 : (s < -100 ? -100 : s);
+}
+
+// The same from partial maxima, by a whole wavefront.
 __device__ __forceinline__ int di_scale_exponent(const uint32_t* __restrict__ parts) {
     uint32_t top = 0;
 #pragma unroll
@@ -175,10 +185,7 @@ __device__ __forceinline__ int di_scale_exponent(const uint32_t* __restrict__ pa
         const uint32_t o = (uint32_t)__shfl_xor((int)top, d, 64);
         top = o > top ? o : top;
     }
-    const int e = (int)(top >> 23);   // |v| in [2^(e - 127), 2^(e - 126))
-    if (top == 0 || e == 255) return 0;
-    const int s = 14 + 127 - e;
-    return s > 100 ? 100 : (s < -100 ? -100 : s);
+    return di_exponent_of(top);
 }
 
 __device__ __forceinline__ uint32_t di_pack(float a, float b) {
@@ -248,12 +255,25 @@ __global__ __launch_bounds__(DI_THREADS) void distill_image_kernel(const float* 
 
 // ------------------------------------------------------------------------------------------------------ the passes
 
-// Queue the copy of `bytes` (a multiple of 8 KiB) of a tile's image into LDS: 1 KiB per wavefront and instruction.
-__device__ __forceinline__ void di_fetch(const char* __restrict__ src, char* lds, int bytes) {
+// Queue the copy of BYTES (a multiple of 4 KiB) of a tile's image into LDS: 1 KiB per wavefront and instruction.
+template <int BYTES>
+__device__ __forceinline__ void di_fetch(const char* __restrict__ src, char* lds) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int o = wave * 1024; o < bytes; o += DI_NW * 1024)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + lane * 16),
-                                         (__attribute__((address_space(3))) void*)(lds + o), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < (BYTES / 1024 + DI_NW - 1) / DI_NW; ++i) {
+        const int o = (i * DI_NW + wave) * 1024;
+        if ((i + 1) * DI_NW * 1024 <= BYTES || o < BYTES)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + lane * 16),
+                                             (__attribute__((address_space(3))) void*)(lds + o), 16, 0, 0);
+    }
+}
+
+// Wait for a tile whose copy was queued TILES copies (of at least PER instructions a wavefront) before the newest; copies
+// return in order, and whatever else was asked for in between only makes the wait stricter.
+template <int TILES, int PER>
+__device__ __forceinline__ void di_wait(bool more) {
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TILES * PER) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 __device__ __forceinline__ f32x16 di_mma(u32x4 a, u32x4 b, f32x16 c) {
@@ -328,7 +348,7 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
     int64_t tiles_per_range, float step, const uint32_t* __restrict__ parts, float* __restrict__ pref,
     float* __restrict__ pmass, float* __restrict__ psum) {
     typedef DistillTile<F> D;
-    constexpr int FETCH = GRAD ? D::BYTES : 2 * D::PLANE;
+    constexpr int FETCH = GRAD ? D::BYTES : 2 * D::PLANE, STAGES = D::STAGES_FORWARD;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int64_t work = di_work_index();
@@ -339,16 +359,19 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
     const bool active = own0 < n;
     const float c = ldexpf(step, -di_scale_exponent(parts) - di_scale_exponent(parts + DI_PARTS));
 
-    di_fetch(yimg + t0 * D::BYTES, lds, FETCH);
     u32x4 own[2][F / 16];
     if (active) di_load_own<F>(ximg + (own0 / 32) * D::BYTES, own);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+        if (t0 + i < t1) di_fetch<FETCH>(yimg + (t0 + i) * D::BYTES, lds + i * FETCH);
     f32x16 acc[F / 32] = {};
     float ref = -INFINITY, mass = 0.f;
-    for (int64_t t = t0; t < t1; ++t) {
-        const char* tile = lds + ((t - t0) & 1) * D::BYTES;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    int cur = 0;   // the buffer of the current tile
+    for (int64_t t = t0; t < t1; ++t, cur = cur + 1 < STAGES ? cur + 1 : 0) {
+        const char* tile = lds + cur * FETCH;
+        di_wait<STAGES - 2, FETCH / (DI_NW * 1024)>(t + STAGES - 2 < t1);
         __syncthreads();   // this tile has arrived, and every wavefront is done with the one before it
-        if (t + 1 < t1) di_fetch(yimg + (t + 1) * D::BYTES, lds + ((t + 1 - t0) & 1) * D::BYTES, FETCH);
+        if (t + STAGES - 1 < t1) di_fetch<FETCH>(yimg + (t + STAGES - 1) * D::BYTES, lds + (cur > 0 ? cur - 1 : STAGES - 1) * FETCH);
         if (!active) continue;
         f32x16 z = di_logits<F>(tile, own);
         if (t == ytiles - 1 && (m & 31)) {   // rows behind the last item
@@ -409,12 +432,12 @@ __host__ __device__ __forceinline__ int64_t di_run_begin(int64_t w, int64_t step
 template <int F>
 __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
     const char* __restrict__ yimg, int64_t m, int64_t steps, const char* __restrict__ ximg, int64_t n, int64_t xtiles,
-    float step, float temperature, const uint32_t* __restrict__ parts, const f32x4* __restrict__ row_const,
+    float step, float temperature, const uint32_t* __restrict__ parts, const float* __restrict__ row_const,
     const uint16_t* __restrict__ start, int64_t ytiles, const uint16_t* __restrict__ place, const float* __restrict__ gval,
     int k, float* __restrict__ dY, float* __restrict__ slots) {
     typedef DistillTile<F> D;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
-    __shared__ __attribute__((aligned(16))) float row_off[2][32], row_w[2][32], row_v[2][32];
+    constexpr int STAGES = D::STAGES_BACKWARD;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];   // tiles, what their rows bring, list entries on their way
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int64_t run0 = di_run_begin(blockIdx.x, steps, gridDim.x), run1 = di_run_begin(blockIdx.x + 1, steps, gridDim.x);
     const int sx = di_scale_exponent(parts), sy = di_scale_exponent(parts + DI_PARTS);
@@ -423,21 +446,15 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
 
     const float back = ldexpf(temperature, -sx - sg);
 
-    f32x4 p_row = {0.f, 0.f, 0.f, 0.f};
-    auto fetch_rows = [&](int64_t t) {
-        if (tid < 32) {
-            const int64_t b = t * 32 + tid;
-            p_row = b < n ? row_const[b] : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+    // a tile of rows and what its rows bring (zero behind the last row), into a buffer
+    char* row_lds = lds + STAGES * D::BYTES;
+    auto fetch_tile = [&](int64_t t, int buffer) {
+        di_fetch<D::BYTES>(ximg + t * D::BYTES, lds + buffer * D::BYTES);
+        if (wave == 0 && half == 0)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(row_const + t * 128 + lane * 4),
+                                             (__attribute__((address_space(3))) void*)(row_lds + buffer * 512), 16, 0, 0);
     };
     int cur = 0;   // the buffer of the current step
-    auto store_rows = [&]() {
-        if (tid < 32) {
-            row_off[cur][tid] = p_row[0];
-            row_w[cur][tid] = ldexpf(p_row[1], sg);
-            row_v[cur][tid] = ldexpf(p_row[2], sg);
-        }
-    };
     // The list entries that fall on this wavefront's items and a tile's rows.  Where they begin and end is asked for
     // two steps ahead, the first 64 of them (one per lane) one step ahead.
     struct Step {
@@ -471,13 +488,17 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
     };
     // Their values on the way to the lanes and registers that hold their places: 16 values per lane (rows of 20: 16-byte
     // reads of neighbouring lanes fall into distinct banks) and a bit for each that is there.
-    float* fix = reinterpret_cast<float*>(lds + 2 * D::BYTES) + wave * (64 * 20 + 64);
+    float* fix = reinterpret_cast<float*>(lds + STAGES * (D::BYTES + 512)) + wave * (64 * 20 + 64);
     uint32_t* fix_bits = reinterpret_cast<uint32_t*>(fix + 64 * 20);
     fix_bits[lane] = 0;
     Step now = {(int)(run0 / xtiles), (int)(run0 % xtiles)};
-    di_fetch(ximg + (int64_t)now.t * D::BYTES, lds, D::BYTES);
-    fetch_rows(now.t);
     fetch_extent(now);
+    Step ahead = now;   // the next tile to copy
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+        if (run0 + i < run1) fetch_tile(ahead.t, i);
+        ahead = after(ahead);
+    }
     fetch_entries(now);
     Step next = after(now);
     fetch_extent(next);
@@ -490,10 +511,10 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
         u32x4 own[2][F / 16];
         if (active) di_load_own<F>(yimg + own0 / 32 * D::BYTES, own);
         f32x16 acc[F / 32] = {};
-        for (int t = t0; t < t1; ++t, cur ^= 1) {
+        for (int t = t0; t < t1; ++t, cur = cur + 1 < STAGES ? cur + 1 : 0) {
             const char* tile = lds + cur * D::BYTES;
-            store_rows();
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const float* rows = reinterpret_cast<const float*>(row_lds + cur * 512);
+            di_wait<STAGES - 2, D::BYTES / (DI_NW * 1024)>(left > STAGES - 2);
             __syncthreads();
             const int have = entries;
             for (int done = 0; done < have; done += 64) {
@@ -503,27 +524,27 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
                 }
                 if (lane < have - done) {
                     const int r = spot >> 5, to = (spot & 31) + 32 * ((r >> 2) & 1), reg = 4 * (r >> 3) + (r & 3);
-                    fix[to * 20 + reg] = val * row_v[cur][r];
+                    fix[to * 20 + reg] = val * rows[64 + r];
                     atomicOr(&fix_bits[to], 1u << reg);
                 }
             }
             now = next;
             next = after(next);
             if (--left > 0) {
-                di_fetch(ximg + (int64_t)now.t * D::BYTES, lds + (cur ^ 1) * D::BYTES, D::BYTES);
-                fetch_rows(now.t);
                 fetch_entries(now);
                 fetch_extent(next);   // (behind the run's last step: read, not used)
             }
+            if (left > STAGES - 2) fetch_tile(ahead.t, cur > 0 ? cur - 1 : STAGES - 1);
+            ahead = after(ahead);
             if (!active) continue;
             f32x16 z = di_logits<F>(tile, own);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 o = *reinterpret_cast<const f32x4*>(&row_off[cur][8 * g + 4 * half]);
-                const f32x4 w = *reinterpret_cast<const f32x4*>(&row_w[cur][8 * g + 4 * half]);
+                const f32x4 off = *reinterpret_cast<const f32x4*>(rows + 8 * g + 4 * half);
+                const f32x4 w = *reinterpret_cast<const f32x4*>(rows + 32 + 8 * g + 4 * half);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    z[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + i], c, o[i])) * w[i];
+                    z[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + i], c, off[i])) * w[i];
             }
             // where an item is on a row's list, its gradient is not A q but q - p
             if (have > 0) {
@@ -897,25 +918,22 @@ __global__ __launch_bounds__(DI_GROUP_THREADS) void distill_group_kernel(const i
     if (tid == 0) tile_start[ytiles] = (uint16_t)base;
 }
 
-// dX; what a row brings to the backward pass (the reference of its logits, the weight of a probability and that of a
-// list entry); the partial maxima of |grad| that scale those weights.
+// dX; and per tile of rows what they bring to the backward pass, 32 numbers each: minus the reference of a row's logits,
+// the weight of its probabilities, the weight of its list entries, the two scaled by the power of two that the largest
+// |grad| asks for (every workgroup finds that for itself; `parts` gets it for the backward pass).
 __global__ __launch_bounds__(DI_THREADS) void distill_dx_kernel(const float* __restrict__ base, const float* __restrict__ grad,
                                                                 float temperature, int64_t n, int f, float* __restrict__ dX,
                                                                 const float* __restrict__ ref, const float* __restrict__ mass,
-                                                                const float* __restrict__ a, f32x4* __restrict__ rows,
+                                                                const float* __restrict__ a, float* __restrict__ rows,
                                                                 uint32_t* __restrict__ parts) {
     __shared__ uint32_t part[DI_THREADS / 64];
     uint32_t top = 0;
-    if (dX)
-        for (int64_t e = ((int64_t)blockIdx.x * DI_THREADS + threadIdx.x) * 4; e < n * f; e += (int64_t)DI_PARTS * DI_THREADS * 4) {
-            const float g = grad[e / f] * temperature;
-            *reinterpret_cast<f32x4*>(dX + e) = *reinterpret_cast<const f32x4*>(base + e) * g;
-        }
-    for (int64_t b = (int64_t)blockIdx.x * DI_THREADS + threadIdx.x; b < n; b += (int64_t)DI_PARTS * DI_THREADS) {
-        const float g = grad[b];
-        rows[b] = f32x4{-ref[b], g * (a[b] / mass[b]), g, 0.f};
-        const uint32_t u = __float_as_uint(g) & 0x7fffffffu;
-        top = u > top ? u : top;
+    for (int64_t b0 = threadIdx.x; b0 < n; b0 += 8 * DI_THREADS) {
+        uint32_t u[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = b0 + i * DI_THREADS < n ? __float_as_uint(grad[b0 + i * DI_THREADS]) & 0x7fffffffu : 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = u[i] > top ? u[i] : top;
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -924,9 +942,21 @@ __global__ __launch_bounds__(DI_THREADS) void distill_dx_kernel(const float* __r
     }
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < DI_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
-        parts[blockIdx.x] = top;
+    for (int w = 0; w < DI_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
+    if (threadIdx.x == 0) parts[blockIdx.x] = top;
+    const int sg = di_exponent_of(top);
+    if (dX)
+        for (int64_t e = ((int64_t)blockIdx.x * DI_THREADS + threadIdx.x) * 4; e < n * f; e += (int64_t)DI_PARTS * DI_THREADS * 4) {
+            const float g = grad[e / f] * temperature;
+            *reinterpret_cast<f32x4*>(dX + e) = *reinterpret_cast<const f32x4*>(base + e) * g;
+        }
+    for (int64_t b = (int64_t)blockIdx.x * DI_THREADS + threadIdx.x; b < ((n + 31) & ~(int64_t)31); b += (int64_t)DI_PARTS * DI_THREADS) {
+        float* to = rows + b / 32 * 128 + b % 32;
+        const float g = b < n ? ldexpf(grad[b], sg) : 0.f;
+        to[0] = b < n ? -ref[b] : 0.f;
+        to[32] = b < n ? g * (a[b] / mass[b]) : 0.f;
+        to[64] = g;
+        to[96] = 0.f;
     }
 }
 
@@ -975,7 +1005,7 @@ static int launch_forward(const DistillWorkspace& L, char* w, const float* X, in
                           float* loss, hipStream_t stream) {
     const float step = (float)(1.4426950408889634 / (double)temperature);
     static OncePerDevice once;
-    constexpr int LDS = 2 * DistillTile<F>::BYTES;
+    constexpr int LDS = DistillTile<F>::STAGES_FORWARD * (GRAD ? DistillTile<F>::BYTES : 2 * DistillTile<F>::PLANE);
     if (const int rc = distill_lds((const void*)distill_forward_kernel<F, GRAD>, LDS, once, "mirec_distill_loss")) return rc;
     uint32_t* parts = (uint32_t*)(w + L.max_off);
     hipLaunchKernelGGL((distill_image_kernel<F>), dim3((unsigned)(L.xtiles + L.ytiles)), dim3(DI_THREADS), 0, stream, X, n,
@@ -1008,13 +1038,13 @@ template <int F>
 static int launch_backward(const DistillWorkspace& L, char* w, int64_t n, int64_t m, int k, float step, float temperature,
                            float* dY, hipStream_t stream) {
     static OncePerDevice once;
-    constexpr int LDS = 2 * DistillTile<F>::BYTES + DI_NW * (64 * 20 + 64) * 4;
+    constexpr int LDS = DistillTile<F>::STAGES_BACKWARD * (DistillTile<F>::BYTES + 512) + DI_NW * (64 * 20 + 64) * 4;
     if (const int rc = distill_lds((const void*)distill_backward_kernel<F>, LDS, once, "mirec_distill_grad")) return rc;
     const int64_t blocks = (m + DI_OWN - 1) / DI_OWN, steps = blocks * L.xtiles;
     float* slots = (float*)(w + L.part_off);
     hipLaunchKernelGGL((distill_backward_kernel<F>), dim3((unsigned)L.runs), dim3(64 * DI_NW), LDS, stream, w + L.yimg_off, m,
                        steps, w + L.ximg_off, n, L.xtiles, step, temperature, (const uint32_t*)(w + L.max_off),
-                       (const f32x4*)(w + L.row_off), (const uint16_t*)(w + L.start_off), L.ytiles,
+                       (const float*)(w + L.row_off), (const uint16_t*)(w + L.start_off), L.ytiles,
                        (const uint16_t*)(w + L.place_off), (const float*)(w + L.gval_off), k, dY, slots);
     MIREC_LAUNCH_CHECK();
     if (L.runs > 1) {
@@ -1080,7 +1110,7 @@ extern "C" int mirec_distill_grad(const float* X, int64_t n, const float* Y, int
     char* w = (char*)ws;
     hipLaunchKernelGGL(distill_dx_kernel, dim3(DI_PARTS), dim3(DI_THREADS), 0, stream, (const float*)(w + L.base_off), grad,
                        temperature, n, f, dX, (const float*)(w + L.ref_off), (const float*)(w + L.mass_off),
-                       (const float*)(w + L.a_off), (f32x4*)(w + L.row_off), (uint32_t*)(w + L.max_off) + 2 * DI_PARTS);
+                       (const float*)(w + L.a_off), (float*)(w + L.row_off), (uint32_t*)(w + L.max_off) + 2 * DI_PARTS);
     MIREC_LAUNCH_CHECK();
     if (!dY) return MIREC_OK;
     const float step = (float)(1.4426950408889634 / (double)temperature);
