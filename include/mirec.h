@@ -282,19 +282,17 @@ int mirec_topk_ordered(const float* Q, int64_t nq, const float* Y, int64_t ni, i
  *   row_*        per-row parameters (null: the one value for all rows).  In rows: a
  *                temperature that is not >= 1e-37 is greedy, top_k <= 0, top_p not
  *                below 1 and min_p not above 0 do not cut, min_p above 1 counts as 1.
- * ws: mirec_sample_workspace_bytes(...) bytes of device scratch, 256-byte aligned (null if
- * 0); two calls that overlap in time need one each. */
+ * No workspace; m <= 2^30, draws <= MIREC_SAMPLE_MAX_DRAWS. */
 #define MIREC_F32 0
 #define MIREC_F16 1
 #define MIREC_BF16 2
 #define MIREC_SAMPLE_MAX_DRAWS 1024
 #define MIREC_SAMPLE_MAX_MASKED_ITEMS 524288
-size_t mirec_sample_workspace_bytes(int64_t n, int64_t m, int dtype, int draws);
 int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m, int64_t row_stride, const int32_t* ids,
                  int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
                  int draws, int replacement, double temperature, const float* row_temperature, int32_t top_k,
                  const int32_t* row_top_k, double top_p, const float* row_top_p, double min_p, const float* row_min_p,
-                 int32_t* out_ids, float* out_logprob, void* ws, size_t ws_bytes, mirec_stream_t stream);
+                 int32_t* out_ids, float* out_logprob, mirec_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Distillation of a factor model from a teacher's ranked lists (a larger ALS model's

@@ -53,9 +53,8 @@ SIGNATURES = {
     "mirec_topk_ordered": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _sz, _vp]),
     "mirec_topk_small_workspace_bytes": (_sz, [_i64, _i64, _int]),
     "mirec_topk_small": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _sz, _vp]),
-    "mirec_sample_workspace_bytes": (_sz, [_i64, _i64, _int, _int]),
     "mirec_sample": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _int, _int, _c.c_double, _vp, _i32, _vp,
-                            _c.c_double, _vp, _c.c_double, _vp, _vp, _vp, _vp, _sz, _vp]),
+                            _c.c_double, _vp, _c.c_double, _vp, _vp, _vp, _vp]),
     "mirec_distill_workspace_bytes": (_sz, [_i64, _i64, _int, _int]),
     "mirec_distill_loss": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _vp, _int, _f32, _vp, _int, _vp, _vp, _sz, _vp]),
     "mirec_distill_grad": (_int, [_vp, _i64, _vp, _i64, _int, _int, _f32, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -39,8 +39,9 @@ constexpr int DI_NW = 8;                          // wavefronts of a workgroup o
 constexpr int DI_OWN = 32 * DI_NW;                // rows it owns
 constexpr int DI_PARTS = 256;                     // partial maxima of a matrix
 constexpr int DI_MAX_THREADS = 1024;              // of the workgroups that find them
-constexpr int DI_GROUP_THREADS = 1024;
-constexpr int DI_BINS = 4096;                     // item tiles that distill_group_kernel counts at a time
+constexpr int DI_PREPARE_THREADS = 1024;
+constexpr int DI_WEIGH_BLOCKS = 64;
+constexpr int DI_BINS = 4096;                     // item tiles that di_group counts at a time
 constexpr int DI_CUS = 256;                       // workgroups that run at once
 constexpr float DI_HEADROOM = 7.f;                // log2 of a probability's scale when its row's reference is current
 
@@ -859,23 +860,21 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
 // One workgroup per tile of 32 rows: their merged lists' entries grouped by item tile, (row in the tile, column in the
 // item tile, q - p) each, and where every item tile's group begins.  A group's order does not matter: its entries are
 // different places of one 32 x 32 block.  Item tiles are counted in LDS, DI_BINS at a time.
-__global__ __launch_bounds__(DI_GROUP_THREADS) void distill_group_kernel(const int32_t* __restrict__ count,
-                                                                   const int32_t* __restrict__ list_id,
-                                                                   const float* __restrict__ list_val, int64_t n, int k,
-                                                                   int64_t ytiles, uint16_t* __restrict__ start,
-                                                                   uint16_t* __restrict__ place, float* __restrict__ val) {
+__device__ __forceinline__ void di_group(int64_t tile, const int32_t* __restrict__ count, const int32_t* __restrict__ list_id,
+                                         const float* __restrict__ list_val, int64_t n, int k, int64_t ytiles,
+                                         uint16_t* __restrict__ start, uint16_t* __restrict__ place, float* __restrict__ val) {
     __shared__ int32_t bins[DI_BINS];
-    __shared__ int32_t part[DI_GROUP_THREADS / 64];
-    constexpr int PER = DI_BINS / DI_GROUP_THREADS;
+    __shared__ int32_t part[DI_PREPARE_THREADS / 64];
+    constexpr int PER = DI_BINS / DI_PREPARE_THREADS;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t tile = blockIdx.x, row0 = tile * 32;
+    const int64_t row0 = tile * 32;
     const int rows = (int)(n - row0 < 32 ? n - row0 : 32);
     uint16_t* tile_start = start + tile * (ytiles + 1);
     int base = 0;
     for (int64_t t0 = 0; t0 < ytiles; t0 += DI_BINS) {
-        for (int i = tid; i < DI_BINS; i += DI_GROUP_THREADS) bins[i] = 0;
+        for (int i = tid; i < DI_BINS; i += DI_PREPARE_THREADS) bins[i] = 0;
         __syncthreads();
-        for (int e = tid; e < rows * k; e += DI_GROUP_THREADS)
+        for (int e = tid; e < rows * k; e += DI_PREPARE_THREADS)
             if (e % k < count[row0 + e / k]) {
                 const int64_t t = list_id[row0 * k + e] / 32 - t0;
                 if (t >= 0 && t < DI_BINS) atomicAdd(&bins[t], 1);
@@ -892,7 +891,7 @@ __global__ __launch_bounds__(DI_GROUP_THREADS) void distill_group_kernel(const i
         if (lane == 63) part[wave] = inc;
         __syncthreads();
         int at = base + inc - sum;
-        for (int w = 0; w < DI_GROUP_THREADS / 64; ++w) {
+        for (int w = 0; w < DI_PREPARE_THREADS / 64; ++w) {
             at += w < wave ? part[w] : 0;
             base += part[w];
         }
@@ -903,7 +902,7 @@ __global__ __launch_bounds__(DI_GROUP_THREADS) void distill_group_kernel(const i
             at += c;
         }
         __syncthreads();
-        for (int e = tid; e < rows * k; e += DI_GROUP_THREADS)
+        for (int e = tid; e < rows * k; e += DI_PREPARE_THREADS)
             if (e % k < count[row0 + e / k]) {
                 const int32_t id = list_id[row0 * k + e];
                 const int64_t t = id / 32 - t0;
@@ -921,17 +920,16 @@ __global__ __launch_bounds__(DI_GROUP_THREADS) void distill_group_kernel(const i
 // dX; and per tile of rows what they bring to the backward pass, 32 numbers each: minus the reference of a row's logits,
 // the weight of its probabilities, the weight of its list entries, the two scaled by the power of two that the largest
 // |grad| asks for (every workgroup finds that for itself; `parts` gets it for the backward pass).
-__global__ __launch_bounds__(DI_THREADS) void distill_dx_kernel(const float* __restrict__ base, const float* __restrict__ grad,
-                                                                float temperature, int64_t n, int f, float* __restrict__ dX,
-                                                                const float* __restrict__ ref, const float* __restrict__ mass,
-                                                                const float* __restrict__ a, float* __restrict__ rows,
-                                                                uint32_t* __restrict__ parts) {
-    __shared__ uint32_t part[DI_THREADS / 64];
+__device__ __forceinline__ void di_weigh(int block, const float* __restrict__ base, const float* __restrict__ grad,
+                                         float temperature, int64_t n, int f, float* __restrict__ dX,
+                                         const float* __restrict__ ref, const float* __restrict__ mass, const float* __restrict__ a,
+                                         float* __restrict__ rows, uint32_t* __restrict__ parts) {
+    __shared__ uint32_t part[DI_PREPARE_THREADS / 64];
     uint32_t top = 0;
-    for (int64_t b0 = threadIdx.x; b0 < n; b0 += 8 * DI_THREADS) {
+    for (int64_t b0 = threadIdx.x; b0 < n; b0 += 8 * DI_PREPARE_THREADS) {
         uint32_t u[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = b0 + i * DI_THREADS < n ? __float_as_uint(grad[b0 + i * DI_THREADS]) & 0x7fffffffu : 0u;
+        for (int i = 0; i < 8; ++i) u[i] = b0 + i * DI_PREPARE_THREADS < n ? __float_as_uint(grad[b0 + i * DI_PREPARE_THREADS]) & 0x7fffffffu : 0u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = u[i] > top ? u[i] : top;
     }
@@ -942,15 +940,15 @@ __global__ __launch_bounds__(DI_THREADS) void distill_dx_kernel(const float* __r
     }
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
-    for (int w = 0; w < DI_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
-    if (threadIdx.x == 0) parts[blockIdx.x] = top;
+    for (int w = 0; w < DI_PREPARE_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
+    if (block == 0 && threadIdx.x < DI_PARTS) parts[threadIdx.x] = top;
     const int sg = di_exponent_of(top);
     if (dX)
-        for (int64_t e = ((int64_t)blockIdx.x * DI_THREADS + threadIdx.x) * 4; e < n * f; e += (int64_t)DI_PARTS * DI_THREADS * 4) {
+        for (int64_t e = ((int64_t)block * DI_PREPARE_THREADS + threadIdx.x) * 4; e < n * f; e += (int64_t)DI_WEIGH_BLOCKS * DI_PREPARE_THREADS * 4) {
             const float g = grad[e / f] * temperature;
             *reinterpret_cast<f32x4*>(dX + e) = *reinterpret_cast<const f32x4*>(base + e) * g;
         }
-    for (int64_t b = (int64_t)blockIdx.x * DI_THREADS + threadIdx.x; b < ((n + 31) & ~(int64_t)31); b += (int64_t)DI_PARTS * DI_THREADS) {
+    for (int64_t b = (int64_t)block * DI_PREPARE_THREADS + threadIdx.x; b < ((n + 31) & ~(int64_t)31); b += (int64_t)DI_WEIGH_BLOCKS * DI_PREPARE_THREADS) {
         float* to = rows + b / 32 * 128 + b % 32;
         const float g = b < n ? ldexpf(grad[b], sg) : 0.f;
         to[0] = b < n ? -ref[b] : 0.f;
@@ -958,6 +956,20 @@ __global__ __launch_bounds__(DI_THREADS) void distill_dx_kernel(const float* __r
         to[64] = g;
         to[96] = 0.f;
     }
+}
+
+// What the gradients need beside the two passes: workgroups 0 .. DI_WEIGH_BLOCKS - 1 weigh the rows, the others group the
+// lists (one launch: each alone leaves most of the chip idle).
+__global__ __launch_bounds__(DI_PREPARE_THREADS) void distill_prepare_kernel(
+    const float* __restrict__ base, const float* __restrict__ grad, float temperature, int64_t n, int f, float* __restrict__ dX,
+    const float* __restrict__ ref, const float* __restrict__ mass, const float* __restrict__ a, float* __restrict__ rows,
+    uint32_t* __restrict__ parts, const int32_t* __restrict__ count, const int32_t* __restrict__ list_id,
+    const float* __restrict__ list_val, int k, int64_t ytiles, uint16_t* __restrict__ start, uint16_t* __restrict__ place,
+    float* __restrict__ val) {
+    if (blockIdx.x < DI_WEIGH_BLOCKS)
+        di_weigh((int)blockIdx.x, base, grad, temperature, n, f, dX, ref, mass, a, rows, parts);
+    else
+        di_group((int64_t)blockIdx.x - DI_WEIGH_BLOCKS, count, list_id, list_val, n, k, ytiles, start, place, val);
 }
 
 __global__ __launch_bounds__(DI_THREADS) void distill_zero_kernel(float* __restrict__ out, int64_t cnt) {
@@ -1025,12 +1037,6 @@ static int launch_forward(const DistillWorkspace& L, char* w, const float* X, in
                        (float*)(w + L.mass_off), (float*)(w + L.a_off), (int32_t*)(w + L.count_off), (int32_t*)(w + L.id_off),
                        (float*)(w + L.val_off), GRAD ? (float*)(w + L.base_off) : nullptr);
     MIREC_LAUNCH_CHECK();
-    if (GRAD) {
-        hipLaunchKernelGGL(distill_group_kernel, dim3((unsigned)L.xtiles), dim3(DI_GROUP_THREADS), 0, stream,
-                           (const int32_t*)(w + L.count_off), (const int32_t*)(w + L.id_off), (const float*)(w + L.val_off), n, k,
-                           L.ytiles, (uint16_t*)(w + L.start_off), (uint16_t*)(w + L.place_off), (float*)(w + L.gval_off));
-        MIREC_LAUNCH_CHECK();
-    }
     return MIREC_OK;
 }
 
@@ -1108,9 +1114,13 @@ extern "C" int mirec_distill_grad(const float* X, int64_t n, const float* Y, int
     const DistillWorkspace L = distill_layout(n, m, f, k);
     if (const int rc = distill_check_ws("mirec_distill_grad", ws, ws_bytes, L.bytes)) return rc;
     char* w = (char*)ws;
-    hipLaunchKernelGGL(distill_dx_kernel, dim3(DI_PARTS), dim3(DI_THREADS), 0, stream, (const float*)(w + L.base_off), grad,
-                       temperature, n, f, dX, (const float*)(w + L.ref_off), (const float*)(w + L.mass_off),
-                       (const float*)(w + L.a_off), (float*)(w + L.row_off), (uint32_t*)(w + L.max_off) + 2 * DI_PARTS);
+    // (without dY the lists need no grouping)
+    hipLaunchKernelGGL(distill_prepare_kernel, dim3((unsigned)(DI_WEIGH_BLOCKS + (dY ? L.xtiles : 0))), dim3(DI_PREPARE_THREADS), 0,
+                       stream, (const float*)(w + L.base_off), grad, temperature, n, f, dX, (const float*)(w + L.ref_off),
+                       (const float*)(w + L.mass_off), (const float*)(w + L.a_off), (float*)(w + L.row_off),
+                       (uint32_t*)(w + L.max_off) + 2 * DI_PARTS, (const int32_t*)(w + L.count_off),
+                       (const int32_t*)(w + L.id_off), (const float*)(w + L.val_off), k, L.ytiles, (uint16_t*)(w + L.start_off),
+                       (uint16_t*)(w + L.place_off), (float*)(w + L.gval_off));
     MIREC_LAUNCH_CHECK();
     if (!dY) return MIREC_OK;
     const float step = (float)(1.4426950408889634 / (double)temperature);

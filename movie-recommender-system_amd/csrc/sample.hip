@@ -1093,20 +1093,14 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
 
 }  // namespace mirec
 
-extern "C" size_t mirec_sample_workspace_bytes(int64_t n, int64_t m, int dtype, int draws) {
-    (void)n, (void)m, (void)dtype, (void)draws;
-    return 0;
-}
-
 extern "C" int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m, int64_t row_stride, const int32_t* ids,
                             int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices,
                             const float* uniforms, int draws, int replacement, double temperature,
                             const float* row_temperature, int32_t top_k, const int32_t* row_top_k, double top_p,
                             const float* row_top_p, double min_p, const float* row_min_p, int32_t* out_ids,
-                            float* out_logprob, void* ws, size_t ws_bytes, mirec_stream_t stream_) {
+                            float* out_logprob, mirec_stream_t stream_) {
     using namespace mirec;
     hipStream_t stream = (hipStream_t)stream_;
-    (void)ws, (void)ws_bytes;
     MIREC_REQUIRE(n >= 0 && m >= 0 && draws >= 0, MIREC_E_INVALID, "mirec_sample: negative size");
     MIREC_REQUIRE(dtype == MIREC_F32 || dtype == MIREC_F16 || dtype == MIREC_BF16, MIREC_E_INVALID,
                   "mirec_sample: unknown score type %d", dtype);

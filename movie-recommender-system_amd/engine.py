@@ -501,6 +501,31 @@ def norm_order(Y: torch.Tensor, n_items: Optional[int] = None) -> torch.Tensor:
     return torch.argsort(Y[:ni].norm(dim=1), descending=True, stable=True).to(torch.int32)
 
 
+def _raw_stream(dev: torch.device) -> int:
+    """The current stream of ``dev`` as a number (``_stream_ptr`` without a stream object: 0.3 instead of 2.8 us, which
+    counts where a call is 3 us of device time)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+class _on_device:
+    """``torch.cuda.device`` for the rare case that ``dev`` is not the current device."""
+
+    def __init__(self, dev: torch.device):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 _SCORE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # MIREC_F32, MIREC_F16, MIREC_BF16
 
 
@@ -515,8 +540,7 @@ def _row_parameter(name: str, v, n: int, dtype: torch.dtype, dev: torch.device):
 
 def sample_scores(scores: torch.Tensor, uniforms: torch.Tensor, ids: Optional[torch.Tensor] = None,
                   mask: Optional[DeviceCSR] = None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
-                  replacement: bool = True, ws: Optional[torch.Tensor] = None,
-                  out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+                  replacement: bool = True, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
     """Draw items from every row of ``scores`` [n, m] (fp32, fp16 or bf16; rows may be strided): softmax at
     ``temperature`` (0: the best item), cut to the ``top_k`` best (0: all), then to the shortest best-first prefix
     that holds ``top_p`` of what is left, then to the items at least ``min_p`` times as likely as the best; one draw
@@ -568,16 +592,13 @@ def sample_scores(scores: torch.Tensor, uniforms: torch.Tensor, ids: Optional[to
     elif any(o.shape != (n, draws) or o.dtype != t or o.device != dev or not o.is_contiguous()
              for o, t in zip(out, (torch.int32, torch.float32))):
         raise ValueError("out must be contiguous tensors [rows, draws] of int32 and fp32 on the device of the scores")
-    need = int(lib.mirec_sample_workspace_bytes(n, m, _SCORE_TYPES[scores.dtype], draws))
-    if need and (ws is None or ws.numel() * ws.element_size() < need or ws.device != dev):
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(lib.mirec_sample(_ptr(scores), _SCORE_TYPES[scores.dtype], n, m, stride, _ptr(ids), ids_stride,
-                                    _ptr(None if mask is None else mask.indptr),
-                                    _ptr(None if mask is None else mask.indices), _ptr(uniforms), draws,
-                                    int(bool(replacement)), float(t1), _ptr(t_rows), min(int(k1), (1 << 31) - 1),
-                                    _ptr(k_rows), float(p1), _ptr(p_rows), float(q1), _ptr(q_rows), _ptr(out[0]),
-                                    _ptr(out[1]), _ptr(ws), need, _stream_ptr()), "mirec_sample")
+    with _on_device(dev):
+        _lib.check(lib.mirec_sample(_addr(scores), _SCORE_TYPES[scores.dtype], n, m, stride, _addr(ids), ids_stride,
+                                    _addr(None if mask is None else mask.indptr),
+                                    _addr(None if mask is None else mask.indices), _addr(uniforms), draws,
+                                    int(bool(replacement)), float(t1), _addr(t_rows), min(int(k1), (1 << 31) - 1),
+                                    _addr(k_rows), float(p1), _addr(p_rows), float(q1), _addr(q_rows), _addr(out[0]),
+                                    _addr(out[1]), _raw_stream(dev)), "mirec_sample")
     return out
 
 
@@ -606,10 +627,10 @@ def _distill_loss(X, Y, ids, scores, temperature, teacher_lse, with_grad, ws=Non
     need = int(lib.mirec_distill_workspace_bytes(n, m, f, k))
     if ws is None or ws.numel() * ws.element_size() < need or ws.device != X.device:
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device=X.device)
-    with torch.cuda.device(X.device):
-        _lib.check(lib.mirec_distill_loss(_ptr(X), n, _ptr(Y), m, f, _ptr(ids), _ptr(scores), k, float(temperature),
-                                          _ptr(teacher_lse), int(with_grad), _ptr(loss), _ptr(ws),
-                                          ws.numel() * ws.element_size(), _stream_ptr()), "mirec_distill_loss")
+    with _on_device(X.device):
+        _lib.check(lib.mirec_distill_loss(_addr(X), n, _addr(Y), m, f, _addr(ids), _addr(scores), k, float(temperature),
+                                          _addr(teacher_lse), int(with_grad), _addr(loss), _addr(ws),
+                                          ws.numel() * ws.element_size(), _raw_stream(X.device)), "mirec_distill_loss")
     return loss, ws
 
 
@@ -618,9 +639,9 @@ def _distill_grad(X, Y, k, temperature, grad, ws, need_x=True, need_y=True):
     n, f = X.shape
     dX = torch.empty_like(X) if need_x else None
     dY = torch.empty_like(Y) if need_y else None
-    with torch.cuda.device(X.device):
-        _lib.check(lib.mirec_distill_grad(_ptr(X), n, _ptr(Y), int(Y.shape[0]), f, int(k), float(temperature), _ptr(grad),
-                                          _ptr(dX), _ptr(dY), _ptr(ws), ws.numel() * ws.element_size(), _stream_ptr()),
+    with _on_device(X.device):
+        _lib.check(lib.mirec_distill_grad(_addr(X), n, _addr(Y), int(Y.shape[0]), f, int(k), float(temperature), _addr(grad),
+                                          _addr(dX), _addr(dY), _addr(ws), ws.numel() * ws.element_size(), _raw_stream(X.device)),
                    "mirec_distill_grad")
     return dX, dY
 

@@ -98,7 +98,7 @@ def call(scores=16, dtype=0, n=2, m=4, stride=4, ids=None, ids_stride=0, indptr=
     """mirec_sample with made-up device addresses: every call here is refused before anything is launched."""
     lib = _lib.require()
     rc = lib.mirec_sample(scores, dtype, n, m, stride, ids, ids_stride, indptr, indices, uniforms, draws, 1, T, None, k,
-                          None, p, None, q, None, out_ids, out_lp, None, 0, None)
+                          None, p, None, q, None, out_ids, out_lp, None)
     return rc, _lib.last_error()
 
 
