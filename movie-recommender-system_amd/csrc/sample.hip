@@ -24,7 +24,7 @@ constexpr int SM_SHORT = 256;                     // rows up to this length: one
 constexpr int64_t SM_FEW_ROWS = 256;              // no more rows than compute units: larger workgroups
 constexpr int SM_AHEAD = 2;                       // loads in flight ahead of the work
 constexpr int SM_BINS = 1024;                     // of a histogram over a row
-constexpr int SM_FEW = 256;                        // entries that one wavefront finishes
+constexpr int SM_FEW = 256;                        // entries that are compared with each other for every sum
 constexpr int SM_LIST = 512;                     // entries that are ranked against each other in LDS
 
 struct SampleParams {
@@ -458,8 +458,11 @@ struct Chunk {
 // What bounds it: the instructions per score (about 25 for a weight, 10 for a place in a histogram), then the chain of
 // barriers of a row, not the bytes: hence two rows of 512 threads side by side on a compute unit, or one of 1024 where
 // there are fewer rows than compute units.
+// Registers: few rows, of 1024 threads, run one or two workgroups to a compute unit and are faster with more registers
+// (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6); 512 threads are faster with 6 (mixed
+// requests 384 -> 350 us).
 template <int DT, int NT>
-__global__ __launch_bounds__(NT, 6) void sample_long_kernel(
+__global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,
     const int32_t* __restrict__ ids, int64_t ids_stride, const int64_t* __restrict__ mask_indptr,
     const int32_t* __restrict__ mask_indices, const float* __restrict__ uniforms, int draws, int replacement,
@@ -469,8 +472,9 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
     constexpr int BINS_PER = SM_BINS / NT;
     extern __shared__ uint32_t liked[];   // one bit per item, when there is a filter
     __shared__ __attribute__((aligned(16))) ulonglong2 list[SM_LIST];   // K and weight
-    __shared__ uint64_t mass_bins[SM_BINS];
+    __shared__ uint64_t mass_bins[SM_BINS], piece_mass[SM_BINS];
     __shared__ uint32_t count_bins[SM_BINS];
+    __shared__ uint64_t before_of[SM_LIST];
     __shared__ uint64_t part[2][NW];
     __shared__ uint64_t shared_key[2];
     __shared__ uint32_t shared_int[2];
@@ -652,7 +656,8 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
         };
 
         // A handful of items are to stay.  The top_k-th best of the threads' own best scores is not above the row's
-        // top_k-th best score, and few scores are above it: those go to a list, and one wavefront does the rest there.
+        // top_k-th best score, and few scores are above it: those go to a list, where every sum is formed by comparing each
+        // with each.
         if (cuts.top_k <= SM_FEW / 2) {
             for (int b = tid; b < SM_BINS; b += NT) count_bins[b] = 0;
             if (tid == 0) shared_int[1] = 0;
@@ -679,64 +684,78 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
             __syncthreads();
             const uint32_t have = shared_int[1];
             if (have <= SM_FEW) {
-                if (wave != 0) continue;
-                constexpr int SLOTS = SM_FEW / 64;
-                uint64_t K[SLOTS], w[SLOTS], run[SLOTS];
-                float f[SLOTS];
-#pragma unroll
-                for (int i = 0; i < SLOTS; ++i) {
-                    const uint32_t e = lane + 64 * i;
-                    K[i] = e < have ? list[e].x : 0ull;
-                    f[i] = sm_unorder((uint32_t)(K[i] >> 32));
-                    w[i] = 0;
-                    if (64 * i < (int)have && e < have) {
-                        w[i] = weight(f[i]);
-                        list[e].y = w[i];
+                // Entry e of the list to NT / SM_FEW threads, which share the entries it is compared with.
+                constexpr uint32_t SLICES = NT / SM_FEW;
+                const uint32_t e = tid % SM_FEW, slice = tid / SM_FEW;
+                uint64_t* sums = mass_bins;                 // by entry: the mass before it in rank order, then its running sum
+                uint64_t* runs = mass_bins + SM_FEW;
+                uint64_t K = 0, w = 0;
+                if (slice == 0) {
+                    sums[e] = runs[e] = 0;
+                    count_bins[e] = 0;
+                    if (e < have) {
+                        K = list[e].x;
+                        w = weight(sm_unorder((uint32_t)(K >> 32)));
+                        list[e].y = w;
+                    }
+                    if (e == 0) shared_key[0] = shared_key[1] = 0;
+                }
+                __syncthreads();
+                if (e < have) {
+                    K = list[e].x;
+                    uint32_t rank = 0;
+                    uint64_t before = 0;
+#pragma unroll 4
+                    for (uint32_t j = slice; j < have; j += SLICES) {
+                        const ulonglong2 x = list[j];
+                        rank += x.x > K ? 1u : 0u;
+                        before += x.x > K ? x.y : 0ull;
+                    }
+                    if (SLICES > 1) {
+                        atomicAdd(&count_bins[e], rank);
+                        atomicAdd((unsigned long long*)&sums[e], (unsigned long long)before);
+                    } else {
+                        count_bins[e] = rank;
+                        sums[e] = before;
                     }
                 }
-                asm volatile("" ::: "memory");
-                // place and mass before it, in rank order
-                uint32_t rank[SLOTS];
-                uint64_t before[SLOTS], mass = 0;
-#pragma unroll
-                for (int i = 0; i < SLOTS; ++i) {
-                    rank[i] = 0;
-                    before[i] = 0;
+                __syncthreads();
+                uint32_t rank = 0;
+                uint64_t before = 0;
+                if (slice == 0 && e < have) {
+                    rank = count_bins[e];
+                    before = sums[e];
+                    // the last entry that top_k leaves has all their mass up to and with it
+                    if (rank + 1 == (cuts.top_k < (int64_t)have ? (uint32_t)cuts.top_k : have)) shared_key[0] = before + w;
                 }
+                __syncthreads();
+                if (slice == 0 && e < have) {
+                    const uint64_t bound = cuts.top_p < 1.0 ? sm_bound(cuts.top_p, shared_key[0]) : ~0ull;
+                    w = rank < cuts.top_k && (rank == 0 || before < bound) && w >= cuts.floor_w ? w : 0ull;
+                    list[e].y = w;
+                }
+                __syncthreads();
+                if (e < have) {   // in index order: a larger complement is a smaller index
+                    uint64_t run = 0;
 #pragma unroll 4
-                for (uint32_t j = 0; j < have; ++j) {
-                    const ulonglong2 x = list[j];
-#pragma unroll
-                    for (int i = 0; i < SLOTS; ++i)
-                        if (64 * i < (int)have) {
-                            rank[i] += x.x > K[i] ? 1u : 0u;
-                            before[i] += x.x > K[i] ? x.y : 0ull;
-                        }
+                    for (uint32_t j = slice; j < have; j += SLICES) {
+                        const ulonglong2 x = list[j];
+                        run += (uint32_t)x.x >= (uint32_t)K ? x.y : 0ull;
+                    }
+                    if (SLICES > 1) atomicAdd((unsigned long long*)&runs[e], (unsigned long long)run);
+                    else runs[e] = run;
+                    atomicAdd((unsigned long long*)&shared_key[1], slice == 0 ? (unsigned long long)w : 0ull);
                 }
+                __syncthreads();
+                if (wave != 0) continue;
+                constexpr int SLOTS = SM_FEW / 64;
+                uint64_t total = shared_key[1], item_K[SLOTS], item_w[SLOTS], run[SLOTS];
 #pragma unroll
                 for (int i = 0; i < SLOTS; ++i) {
-                    w[i] = rank[i] < cuts.top_k ? w[i] : 0ull;
-                    mass += w[i];
-                }
-                const uint64_t bound = cuts.top_p < 1.0 ? sm_bound(cuts.top_p, sm_wave_sum(mass)) : ~0ull;
-                mass = 0;
-#pragma unroll
-                for (int i = 0; i < SLOTS; ++i) {
-                    w[i] = (rank[i] == 0 || before[i] < bound) && w[i] >= cuts.floor_w ? w[i] : 0ull;
-                    mass += w[i];
-                    const uint32_t e = lane + 64 * i;
-                    if (64 * i < (int)have && e < have) list[e].y = w[i];
-                    run[i] = 0;
-                }
-                uint64_t total = sm_wave_sum(mass);
-                asm volatile("" ::: "memory");
-                // running sums in index order: a larger complement is a smaller index
-#pragma unroll 4
-                for (uint32_t j = 0; j < have; ++j) {
-                    const ulonglong2 x = list[j];
-#pragma unroll
-                    for (int i = 0; i < SLOTS; ++i)
-                        if (64 * i < (int)have) run[i] += (uint32_t)x.x >= (uint32_t)K[i] ? x.y : 0ull;
+                    const bool real = lane + 64 * i < (int)have;
+                    item_K[i] = real ? list[lane + 64 * i].x : 0ull;
+                    item_w[i] = real ? list[lane + 64 * i].y : 0ull;
+                    run[i] = real ? runs[lane + 64 * i] : 0ull;
                 }
                 for (int d = 0; d < draws; ++d) {
                     if (total == 0) {
@@ -748,27 +767,25 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
                     }
                     const uint64_t t = sm_target(uniforms[row * draws + d], total);
                     uint64_t out_K = 0, out_w = 0;
-                    float out_f = 0.f;
 #pragma unroll
                     for (int i = 0; i < SLOTS; ++i) {
-                        const bool here = w[i] != 0 && run[i] > t && run[i] - w[i] <= t;
-                        out_K = here ? K[i] : out_K;
-                        out_w = here ? w[i] : out_w;
-                        out_f = here ? f[i] : out_f;
+                        const bool here = item_w[i] != 0 && run[i] > t && run[i] - item_w[i] <= t;
+                        out_K = here ? item_K[i] : out_K;
+                        out_w = here ? item_w[i] : out_w;
                     }
                     if (out_w != 0) {
                         const int32_t item = (int32_t)(0xffffffffu - (uint32_t)out_K);
                         out_ids[row * draws + d] = id ? id[item] : item;
-                        out_logprob[row * draws + d] = sm_logprob(out_f, best, cuts.step, total, bits);
+                        out_logprob[row * draws + d] = sm_logprob(sm_unorder((uint32_t)(out_K >> 32)), best, cuts.step, total, bits);
                     }
                     if (!replacement) {
                         const int l = __builtin_ctzll(__ballot(out_w != 0));
-                        const uint64_t gone = sm_lane(out_K, l), less = sm_lane(out_w, l);
+                        const uint64_t gone_K = sm_lane(out_K, l), less = sm_lane(out_w, l);
                         total -= less;
 #pragma unroll
                         for (int i = 0; i < SLOTS; ++i) {
-                            run[i] -= (uint32_t)gone >= (uint32_t)K[i] ? less : 0ull;
-                            w[i] = K[i] == gone ? 0ull : w[i];
+                            run[i] -= (uint32_t)gone_K >= (uint32_t)item_K[i] ? less : 0ull;
+                            item_w[i] = item_K[i] == gone_K ? 0ull : item_w[i];
                         }
                     }
                 }
@@ -788,6 +805,7 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
             for (int v = 1; v < V; ++v) most = fmaxf(most, q.score(v));
             return __any(most >= cut_f && most > -INFINITY);
         };
+        bool summed = false;   // piece_mass holds the kept mass of every piece
         // Moves `cut` to the item at the border: the target-th in order (by count), or the last item whose
         // predecessors hold less than the share top_p of what stayed so far.  Where the row has no border it stays.
         auto find_cut = [&](auto by_mass, uint64_t target, double top_p) {
@@ -847,29 +865,79 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
                     const uint64_t K = order_of(f, item);
                     return K >= lo && K <= hi && (int)((hi - K) >> shift) == b;
                 };
-                each([&](const C& q, int32_t first, int, int) {
+                if (BY_MASS && shift < 0) {
+                    // the members to the list, the mass of what is above the bin to its pieces: one pass for both
+                    uint64_t w = 0;
+                    each([&](const C& q, int32_t first, int p, int sub) {
+                        if (any_kept(q)) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const float f = q.score(v);
-                        if (member(f, first + v)) {
-                            const uint32_t e = atomicAdd(&shared_int[1], 1u);
-                            if (e < SM_LIST) list[e].x = order_of(f, first + v);
+                            for (int v = 0; v < V; ++v) {
+                                const float f = q.score(v);
+                                const uint32_t in = first_bin(f);
+                                const bool on = (in <= (uint32_t)b) & kept(f, first + v);
+                                if (__any(on)) {
+                                    const uint64_t wf = weight(f);
+                                    w += on & (in < (uint32_t)b) & (wf >= cuts.floor_w) ? wf : 0ull;
+                                }
+                                if (on && in == (uint32_t)b) {
+                                    const uint32_t e = atomicAdd(&shared_int[1], 1u);
+                                    if (e < SM_LIST) list[e].x = order_of(f, first + v);
+                                }
+                            }
                         }
-                    }
-                });
+                        if (sub == S - 1) {
+                            w = sm_wave_sum(w);
+                            if (lane == 0) piece_mass[p] = w;
+                            w = 0;
+                        }
+                    });
+                } else {
+                    each([&](const C& q, int32_t first, int, int) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            const float f = q.score(v);
+                            if (member(f, first + v)) {
+                                const uint32_t e = atomicAdd(&shared_int[1], 1u);
+                                if (e < SM_LIST) list[e].x = order_of(f, first + v);
+                            }
+                        }
+                    });
+                }
                 __syncthreads();
                 const uint32_t members = shared_int[1];
                 if (members <= SM_LIST) {
-                    for (uint32_t e = tid; e < members; e += NT) list[e].y = BY_MASS ? weight(sm_unorder((uint32_t)(list[e].x >> 32))) : 1ull;
+                    // every entry to `slices` threads, which share the entries it is compared with
+                    int span = 64;
+                    while (span < (int)members) span *= 2;
+                    const int slices = NT / span > 0 ? NT / span : 1;
+                    for (uint32_t e = tid; e < members; e += NT) {
+                        list[e].y = BY_MASS ? weight(sm_unorder((uint32_t)(list[e].x >> 32))) : 1ull;
+                        before_of[e] = base;
+                    }
+                    __syncthreads();
+                    for (uint32_t e0 = 0; e0 < members; e0 += NT) {
+                        const uint32_t e = e0 + (tid & (span - 1));
+                        if (e < members && (int)(tid / span) < slices) {
+                            const uint64_t K = list[e].x;
+                            uint64_t before = 0;
+#pragma unroll 4
+                            for (uint32_t j = tid / span; j < members; j += slices) before += list[j].x > K ? list[j].y : 0ull;
+                            atomicAdd((unsigned long long*)&before_of[e], (unsigned long long)before);
+                        }
+                    }
                     __syncthreads();
                     for (uint32_t e = tid; e < members; e += NT) {
                         const ulonglong2 x = list[e];
-                        uint64_t before = base;
-#pragma unroll 8
-                        for (uint32_t j = 0; j < members; ++j) before += list[j].x > x.x ? list[j].y : 0ull;
+                        const uint64_t before = before_of[e];
                         const bool stays = BY_MASS ? x.y > 0 && (before < bound || before == base) : before < target;
-                        if (stays) atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)x.x);
+                        if (stays) {
+                            atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)x.x);
+                            // (by mass in the first histogram: what lies above the bin is in the pieces already)
+                            if (BY_MASS && shift < 0 && x.y >= cuts.floor_w)
+                                atomicAdd((unsigned long long*)&piece_mass[(int32_t)(0xffffffffu - (uint32_t)x.x) / (WAVE_CHUNK * S)], (unsigned long long)x.y);
+                        }
                     }
+                    if (BY_MASS && shift < 0) summed = true;
                     __syncthreads();
                     cut_f = sm_unorder((uint32_t)(shared_key[0] >> 32));
                     cut_i = (int32_t)(0xffffffffu - (uint32_t)shared_key[0]);
@@ -909,6 +977,7 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
             }
         };
 
+        for (int p = tid; p < SM_BINS; p += NT) piece_mass[p] = 0;
         if (cuts.top_k < m) find_cut(std::false_type{}, (uint64_t)cuts.top_k, 0.0);
         if (cuts.top_p < 1.0) find_cut(std::true_type{}, 0ull, cuts.top_p);
 
@@ -918,9 +987,8 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
             return kept(f, item) & (w >= cuts.floor_w) ? w : 0ull;
         };
         const bool uncut = cut_f == -INFINITY && cuts.floor_w == 0;   // an excluded item has no weight
-        for (int p = tid; p < SM_BINS; p += NT) mass_bins[p] = 0;
         __syncthreads();
-        {
+        if (!summed) {
             uint64_t w = 0;
             each([&](const C& q, int32_t first, int p, int sub) {
                 if (uncut) {
@@ -932,7 +1000,7 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
                 }
                 if (sub == S - 1) {
                     w = sm_wave_sum(w);
-                    if (lane == 0) mass_bins[p] = w;
+                    if (lane == 0) piece_mass[p] = w;
                     w = 0;
                 }
             });
@@ -941,7 +1009,7 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
         uint64_t sum = 0, mine[BINS_PER];
 #pragma unroll
         for (int i = 0; i < BINS_PER; ++i) {
-            mine[i] = mass_bins[tid * BINS_PER + i];
+            mine[i] = piece_mass[tid * BINS_PER + i];
             sum += mine[i];
         }
         const uint64_t inc = sm_wave_scan(sum);
@@ -956,7 +1024,7 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
 #pragma unroll
         for (int i = 0; i < BINS_PER; ++i) {
             at += mine[i];
-            mass_bins[tid * BINS_PER + i] = at;
+            piece_mass[tid * BINS_PER + i] = at;
         }
         __syncthreads();
 
@@ -974,9 +1042,9 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
                 continue;
             }
             const uint64_t t = sm_target(uniforms[row * draws + d], total);
-            const int p16 = __builtin_ctzll(__ballot(mass_bins[lane * (SM_BINS / 64) + SM_BINS / 64 - 1] > t));
-            const int p = p16 * (SM_BINS / 64) + __builtin_ctzll(__ballot(lane >= SM_BINS / 64 || mass_bins[p16 * (SM_BINS / 64) + (lane & (SM_BINS / 64 - 1))] > t));
-            uint64_t run = p > 0 ? mass_bins[p - 1] : 0ull;
+            const int p16 = __builtin_ctzll(__ballot(piece_mass[lane * (SM_BINS / 64) + SM_BINS / 64 - 1] > t));
+            const int p = p16 * (SM_BINS / 64) + __builtin_ctzll(__ballot(lane >= SM_BINS / 64 || piece_mass[p16 * (SM_BINS / 64) + (lane & (SM_BINS / 64 - 1))] > t));
+            uint64_t run = p > 0 ? piece_mass[p - 1] : 0ull;
             for (int sub = 0; sub < S; ++sub) {
                 C q = load(p, sub);
                 const int32_t first = first_item(p, sub);
@@ -1020,7 +1088,7 @@ __global__ __launch_bounds__(NT, 6) void sample_long_kernel(
                     ++taken;
                     const uint64_t less = sm_lane(drawn, l);
                     total -= less;
-                    for (int j = p + lane; j < SM_BINS; j += 64) mass_bins[j] -= less;
+                    for (int j = p + lane; j < SM_BINS; j += 64) piece_mass[j] -= less;
                     asm volatile("" ::: "memory");
                 }
                 break;
