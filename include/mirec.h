@@ -269,6 +269,7 @@ int mirec_topk_ordered(const float* Q, int64_t nq, const float* Y, int64_t ni, i
  * out_ids int32[n, draws]: the item (ids[row, i] where ids are given, else i), or -1
  * where nothing is left; out_logprob fp32[n, draws]: the natural logarithm of the
  * probability the item was drawn with (-inf with id -1).
+ * An infinite score counts as FLT_MAX.
  * Excluded are scores that are NaN or not above the lowest finite value of their type
  * (what mirec_topk gives filtered items and empty slots), items of the row's filter
  * (mask_indptr / mask_indices as in mirec_topk, in any order; dense rows only, at most
@@ -311,8 +312,12 @@ int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m, int64_t ro
  * mirec_distill_grad writes the gradients of sum_b grad[b] * loss[b]: dX [n, f], dY
  * [m, f] (either may be null).  It reads what mirec_distill_loss with
  * with_grad != 0 left in `ws` for the same X, Y, lists and sizes, as often as needed.
- * f as in the ALS kernels (mirec_factor_width(f, 0)), k <= MIREC_DISTILL_MAX_LIST.
- * Sums and statistics are fp32 or wider.  The same inputs give the same bits.
+ * f as in the ALS kernels (mirec_factor_width(f, 0)), k <= MIREC_DISTILL_MAX_LIST,
+ * n and m <= 2^26, T in [1e-6, 1e6]; X, Y, dX and dY 16-byte aligned.
+ * Sums and statistics are fp32 or wider.  Products take the factors as two fp16 numbers
+ * each, scaled so that a matrix's largest entry is just below 2^15: 22 bits or more of
+ * entries within 2^-18 of the largest, 2^-40 of the largest absolutely below that.
+ * The same inputs give the same bits.
  * ws: mirec_distill_workspace_bytes(n, m, f, k) bytes, 256-byte aligned; calls that
  * overlap in time need one each. */
 #define MIREC_DISTILL_MAX_LIST 256

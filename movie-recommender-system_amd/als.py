@@ -47,6 +47,17 @@ def _hide_filtered(ids: torch.Tensor, scores: torch.Tensor, mask) -> torch.Tenso
     return torch.where(scores == _FILTERED, torch.full_like(ids, -1), ids)
 
 
+def _random_state(seed) -> np.random.RandomState:
+    return seed if isinstance(seed, np.random.RandomState) else np.random.RandomState(seed)
+
+
+def _adam(P: torch.Tensor, grad: torch.Tensor, m: torch.Tensor, v: torch.Tensor, step: int, rate: float) -> None:
+    """One step of Adam (Kingma and Ba) on ``P`` in place, with the usual 0.9, 0.999 and 1e-8."""
+    m.lerp_(grad, 0.1)
+    v.mul_(0.999).addcmul_(grad, grad, value=0.001)
+    P.addcdiv_(m, (v / (1.0 - 0.999 ** step)).sqrt_().add_(1e-8), value=-rate / (1.0 - 0.9 ** step))
+
+
 class _ServingState:
     """Device-resident state behind the per-request calls: nothing here is uploaded again per request."""
 
@@ -133,6 +144,13 @@ class AlternatingLeastSquares:
         self.dtype = np.dtype(np.float32)
         self._reset_caches()
 
+    def _start_factors(self, users: int, items: int) -> None:
+        rs = _random_state(self.random_state)
+        if self.user_factors is None:
+            self.user_factors = rs.rand(users, self.factors).astype(np.float32) * 0.01
+        if self.item_factors is None:
+            self.item_factors = rs.rand(items, self.factors).astype(np.float32) * 0.01
+
     # -------------------------------------------------------------------- fit
     def fit(self, user_items, show_progress: bool = True, callback=None) -> None:
         """implicit's ``fit``: cast to fp32, multiply the stored values by
@@ -144,12 +162,7 @@ class AlternatingLeastSquares:
         if Cui.nnz >= 2 ** 31:
             raise ValueError("more than 2^31 stored interactions in one matrix")
         dev = E.require_cuda(self.device)
-        rs = self.random_state if isinstance(self.random_state, np.random.RandomState) \
-            else np.random.RandomState(self.random_state)
-        if self.user_factors is None:
-            self.user_factors = rs.rand(users, self.factors).astype(np.float32) * 0.01
-        if self.item_factors is None:
-            self.item_factors = rs.rand(items, self.factors).astype(np.float32) * 0.01
+        self._start_factors(users, items)
         if self.user_factors.shape != (users, self.factors) or self.item_factors.shape != (items, self.factors):
             raise ValueError("user_factors / item_factors do not match the matrix shape")
         if not self.use_cg and Cui.nnz and float(np.abs(Cui.data).min()) * abs(self.alpha) < 1.0:
@@ -464,6 +477,95 @@ class AlternatingLeastSquares:
         with self._lock, torch.cuda.device(dev):
             y = self._solve_rows(sp.csr_matrix(item_users), self.user_factors, dev, self.factors).cpu().numpy()
         return y[0] if np.isscalar(itemid) else y
+
+    def sample(self, userid, user_items=None, N: int = 10, pool: int = 100, temperature: float = 1.0, top_p: float = 1.0,
+               min_p: float = 0.0, filter_already_liked_items: bool = True, random_state=None):
+        """N different items per user drawn from the ``pool`` (at most 224) best of ``recommend`` (same users,
+        ``user_items`` and filter): softmax of the scores at ``temperature`` (0: the best item alone), cut to the shortest best-first
+        prefix holding ``top_p`` of the mass and to items at least ``min_p`` times as likely as the best.  An item
+        drawn leaves before the next draw.  Returns (ids int32, log probabilities of the draws fp32) in the order
+        drawn, -1 and -inf where nothing is left; ``random_state`` (a seed or a RandomState) makes it repeatable."""
+        if self.user_factors is None or self.item_factors is None:
+            raise ValueError("model has not been fitted")
+        scalar = np.isscalar(userid)
+        uids = np.atleast_1d(np.asarray(userid)).astype(np.int64)
+        if uids.size and (uids.min() < 0 or uids.max() >= self.user_factors.shape[0]):
+            raise IndexError("a userid is out of range")
+        N, pool = int(N), min(int(pool), self.item_factors.shape[0])
+        if N < 1 or pool < 1:
+            raise ValueError("N and pool must be positive")
+        mask = None
+        if filter_already_liked_items:
+            if user_items is None and self._attached is not None:
+                user_items = self._attached[0][uids]
+            if not sp.isspmatrix_csr(user_items):
+                raise ValueError("user_items needs to be a CSR sparse matrix")
+            if user_items.shape[0] != len(uids):
+                raise ValueError("user_items must contain 1 row for every user in userids")
+            mask = user_items if user_items.has_sorted_indices else user_items.sorted_indices()
+        # 24 random bits: every number is exact in fp32 and below one
+        u = _random_state(random_state).randint(0, 1 << 24, size=(len(uids), N)).astype(np.float32) * np.float32(2.0 ** -24)
+        dev = E.require_cuda(self.device)
+        with self._lock, torch.cuda.device(dev):
+            st = self._serving_state(dev)
+            dmask = None if mask is None else E.DeviceCSR.from_scipy(mask, dev)
+            ids, scores = E.topk(st.X.index_select(0, torch.from_numpy(uids).to(dev)), st.Y, pool, dmask)
+            ids, logprob = E.sample_scores(scores, torch.from_numpy(u).to(dev), ids=ids, temperature=float(temperature),
+                                           top_p=float(top_p), min_p=float(min_p), replacement=False)
+            ids, logprob = ids.cpu().numpy(), logprob.cpu().numpy()
+        if scalar:
+            return ids[0], logprob[0]
+        return ids, logprob
+
+    def distill(self, teacher: "AlternatingLeastSquares", user_items=None, N: int = 100, temperature: float = 1.0,
+                epochs: int = 5, batch: int = 16384, learning_rate: float = 0.01) -> list:
+        """Train these factors on the lists of a fitted ``teacher`` of the same users and items (a wider model):
+        per user T^2 KL(p || q), p the softmax of the teacher's ``N`` (at most 224) best scores over ``temperature`` (without the
+        items of ``user_items``, where given) and q the softmax of this model's scores of all items.  ``epochs``
+        passes over the users in batches, Adam steps on both sides; starts from the factors that are set (``fit``'s
+        start otherwise).  Returns the mean loss of every epoch."""
+        if teacher.user_factors is None or teacher.item_factors is None:
+            raise ValueError("the teacher has not been fitted")
+        users, items = teacher.user_factors.shape[0], teacher.item_factors.shape[0]
+        N = min(int(N), items)
+        if N < 1 or int(epochs) < 0 or int(batch) < 1 or not learning_rate > 0.0:
+            raise ValueError("N, batch and learning_rate must be positive, epochs not negative")
+        mask = None
+        if user_items is not None:
+            mask = sp.csr_matrix(user_items)
+            if mask.shape != (users, items):
+                raise ValueError("user_items must have the teacher's users and items")
+            if not mask.has_sorted_indices:
+                mask = mask.sorted_indices()
+        self._start_factors(users, items)
+        if self.user_factors.shape != (users, self.factors) or self.item_factors.shape != (items, self.factors):
+            raise ValueError("user_factors / item_factors do not match the teacher's users and items")
+        dev = E.require_cuda(self.device)
+        W = E.factor_width(teacher.factors, for_scoring=True)
+        F = E.factor_width(self.factors)
+        with self._lock, torch.cuda.device(dev):
+            XT, YT = E.pad_factors(teacher.user_factors, W, dev), E.pad_factors(teacher.item_factors, W, dev)
+            dmask = None if mask is None else E.DeviceCSR.from_scipy(mask, dev)
+            batches = [(a, min(a + int(batch), users)) for a in range(0, users, int(batch))]
+            lists = [E.topk(XT[a:b], YT, N, None if dmask is None else dmask.rows(a, b)) for a, b in batches]
+            X, Y = E.pad_factors(self.user_factors, F, dev), E.pad_factors(self.item_factors, F, dev)
+            mX, vX, mY, vY = (torch.zeros_like(P) for P in (X, X, Y, Y))
+            need = max((int(_lib.require().mirec_distill_workspace_bytes(b - a, items, F, N)) for a, b in batches), default=0)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            losses, step = [], 0
+            for epoch in range(int(epochs)):
+                total = torch.zeros((), dtype=torch.float64, device=dev)
+                for (a, b), (ids, scores) in zip(batches, lists):
+                    step += 1
+                    loss, dX, dY = E.distill(X[a:b], Y, ids, scores, temperature=float(temperature), ws=ws)
+                    total += loss.sum(dtype=torch.float64)
+                    _adam(X[a:b], dX, mX[a:b], vX[a:b], epoch + 1, float(learning_rate))
+                    _adam(Y, dY, mY, vY, step, float(learning_rate))
+                losses.append(float(total) / max(users, 1))
+            self.user_factors = X[:, :self.factors].contiguous().cpu().numpy()
+            self.item_factors = Y[:, :self.factors].contiguous().cpu().numpy()
+            self._dev_items = self._item_norms = self._serving = None
+        return losses
 
     def recommend_all(self, user_items=None, N: int = 10, filter_already_liked_items: bool = True,
                       users: Optional[tuple] = None):

@@ -986,7 +986,8 @@ static int distill_check(const char* who, const float* X, int64_t n, const float
                   DI_LIST);
     MIREC_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, MIREC_E_INVALID,
                   "%s: temperature must lie in [1e-6, 1e6] (got %g)", who, (double)temperature);
-    MIREC_REQUIRE(n <= ((int64_t)1 << 28) && m <= ((int64_t)1 << 28), MIREC_E_UNSUPPORTED, "%s: more than 2^28 rows or items",
+    // (a launch has less than 2^32 threads: 1024 per 32 rows)
+    MIREC_REQUIRE(n <= ((int64_t)1 << 26) && m <= ((int64_t)1 << 26), MIREC_E_UNSUPPORTED, "%s: more than 2^26 rows or items",
                   who);
     MIREC_REQUIRE(n == 0 || m >= 1, MIREC_E_INVALID, "%s: the catalogue is empty", who);
     MIREC_REQUIRE(n == 0 || (X && Y), MIREC_E_INVALID, "%s: null argument", who);

@@ -447,8 +447,8 @@ struct Chunk {
 };
 
 // One workgroup of NT threads per row.  The row is cut into pieces of S chunks, a chunk is 16 bytes per lane; piece g NW + w
-// belongs to wavefront w, so pieces, chunks and lanes are in index order.  CH > 0: a wavefront's CH pieces (S = 1) stay in
-// its registers; CH = 0: each pass reads the row again, S makes at most SM_BINS pieces of it.
+// belongs to wavefront w, so pieces, chunks and lanes are in index order; S makes at most SM_BINS pieces of a row.  Each
+// pass reads the row again (from L2, mostly): rows held in registers spilled.
 //
 // A cut is the last item that stays (score and index).  It is found by a histogram whose bins are ordered like the items
 // -- first by the score's distance from the best, in 1/32 octaves of the weight, then, should a bin hold more than
@@ -484,17 +484,6 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
     const int64_t row_chunks = (m + WAVE_CHUNK - 1) / WAVE_CHUNK;
     const int S = (int)((row_chunks + SM_BINS - 1) / SM_BINS);
     const int pieces = (int)((row_chunks + S - 1) / S);   // at most SM_BINS
-
-    auto block_sum = [&](uint64_t v) -> uint64_t {
-        v = sm_wave_sum(v);
-        if (lane == 0) part[1][wave] = v;
-        __syncthreads();
-        v = part[1][0];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) v += part[1][w];
-        __syncthreads();
-        return v;
-    };
 
     for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
         const typename ScoreType<DT>::raw* s = scores + row * stride;

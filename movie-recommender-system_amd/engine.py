@@ -660,12 +660,15 @@ def distill(X: torch.Tensor, Y: torch.Tensor, ids: torch.Tensor, scores: torch.T
     most 256.
 
     Returns (loss [n], dX [n, f], dY [m, f]), the gradients of sum(grad * loss) (``grad`` fp32 [n]; None: ones).
-    The matrix of scores is never written.  ``ws`` lets a caller that takes many steps reuse its workspace."""
+    The matrix of scores is never written.  ``ws`` (contiguous, at least ``mirec_distill_workspace_bytes``, else a new
+    one is taken) lets a caller that takes many steps reuse its workspace; steps that overlap in time need one each."""
     _distill_inputs(X, Y, ids, scores, teacher_lse)
     if grad is None:
         grad = torch.ones(X.shape[0], dtype=torch.float32, device=X.device)
     elif grad.shape != (X.shape[0],) or grad.dtype != torch.float32 or grad.device != X.device or not grad.is_contiguous():
         raise ValueError("grad must hold one fp32 number per row of X")
+    if ws is not None and not ws.is_contiguous():
+        raise ValueError("ws must be contiguous")
     loss, ws = _distill_loss(X, Y, ids, scores, temperature, teacher_lse, True, ws)
     return (loss,) + _distill_grad(X, Y, ids.shape[1], temperature, grad, ws)
 
@@ -692,8 +695,12 @@ class _Distill(torch.autograd.Function):
 def distill_loss(X: torch.Tensor, Y: torch.Tensor, ids: torch.Tensor, scores: torch.Tensor, temperature: float = 1.0,
                  teacher_lse: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The loss of ``distill`` [n] as a differentiable function of ``X`` and ``Y`` (once; the lists and
-    ``teacher_lse`` are constants)."""
+    ``teacher_lse`` are constants).  Not for a stream that is being captured, unless no gradient is asked for: a
+    backward pass of autograd inside a capture ends the process if another graph of the same leaves is alive.
+    ``distill`` gives the same gradients without autograd and can be captured."""
     _distill_inputs(X, Y, ids, scores, teacher_lse)
+    if torch.is_grad_enabled() and (X.requires_grad or Y.requires_grad) and torch.cuda.is_current_stream_capturing():
+        raise _lib.MirecError("distill_loss with gradients cannot be captured: capture distill, which returns them")
     return _Distill.apply(X, Y, ids, scores, temperature, teacher_lse)
 
 

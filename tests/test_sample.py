@@ -1,9 +1,9 @@
 """Drawing items from scores: engine.sample_scores / mirec_sample against a float64 statement of its definition.
 
 A draw is checked by the interval of (0, 1) that belongs to the item: the device's running sum may sit off the float64 one
-by the weights' own error.  A weight is 2^f by a polynomial within 1.6e-14 of it, its exponent a product of float64 numbers below 2^7
-(2^-46 ln 2 of it at most) in float64 arithmetic (a dozen roundings, each 2^-53), rounded to S = min(51, 62 - ceil(log2 m)) fraction bits; with the
-largest weight 1 the borders of the normalised running sum are off by at most 2 (3e-13 + m 2^-(S+1)).  The logarithm of
+by the weights' own error.  A weight is 2^f by a polynomial within 1.6e-14 of it, its exponent
+a product of float64 numbers below 2^7 (2^-46 ln 2 of it at most) in float64 arithmetic (a dozen roundings, each 2^-53),
+rounded to S = min(51, 62 - ceil(log2 m)) fraction bits; with the largest weight 1 the borders of the normalised running sum are off by at most 2 (3e-13 + m 2^-(S+1)).  The logarithm of
 the probability carries the same and one rounding to fp32 (half a step: 2^-24 of it)."""
 
 import ctypes
@@ -196,6 +196,70 @@ def test_ties_rank_by_index(dev, m, levels, cut):
     u = torch.rand(4, 9, generator=g).to(dev)
     ids, lp = E.sample_scores(s, u, **cut)
     check(s, u, ids, lp, **cut)
+
+
+@gpu
+@pytest.mark.parametrize("cut", [dict(top_k=1), dict(top_k=129), dict(top_k=300), dict(top_k=700), dict(top_k=5000), dict(top_p=0.37),
+                                 dict(top_k=6000, top_p=0.37), dict(top_p=0.37, min_p=0.9999999), dict(top_k=200, top_p=0.9)])
+@pytest.mark.parametrize("n,m", [(2, 7000), (3, 20011)])
+@pytest.mark.parametrize("spread", [3e-7, 1e-4])
+def test_cuts_among_nearly_equal_scores(dev, n, m, spread, cut):
+    """All scores in one bin of the first histogram (1/32 octave): cuts by the finer ones, ties by index."""
+    s, u = make(m + n, n, m, "f32", 4, dev, spread)
+    s = s + 1.0
+    ids, lp = E.sample_scores(s, u, **cut)
+    check(s, u, ids, lp, **cut)
+
+
+@gpu
+@pytest.mark.parametrize("cut", [dict(), dict(top_k=20), dict(top_k=1000, top_p=0.8), dict(top_p=0.7), dict(min_p=0.3)])
+@pytest.mark.parametrize("n,m,dtype", [(1, 300_007, "f32"), (2, 1_000_003, "f16")])
+def test_rows_of_more_than_1024_chunks(dev, n, m, dtype, cut):
+    s, u = make(m, n, m, dtype, 3, dev)
+    ids, lp = E.sample_scores(s, u, replacement=False, **cut)
+    check(s, u, ids, lp, replacement=False, **cut)
+
+
+@gpu
+def test_a_model_draws_from_its_lists(dev):
+    """AlternatingLeastSquares.sample: every draw by the definition on the model's own list, repeatable, refusals."""
+    from scipy import sparse as sp
+    from movie_recommender_system_amd.als import AlternatingLeastSquares
+    g = np.random.default_rng(8)
+    model = AlternatingLeastSquares(factors=24)
+    with pytest.raises(ValueError):
+        model.sample(0, None)
+    model.user_factors, model.item_factors = (g.normal(0, 0.6, (c, 24)).astype(np.float32) for c in (60, 800))
+    liked = sp.random(60, 800, 0.1, format="csr", dtype=np.float32, random_state=4)
+    users = np.array([3, 59, 3, 0])
+    kw = dict(N=6, pool=50, temperature=0.4, top_p=0.95, min_p=0.01)
+    ids, lp = model.sample(users, liked[users], random_state=11, **kw)
+    again = model.sample(users, liked[users], random_state=np.random.RandomState(11), **kw)
+    assert np.array_equal(ids, again[0]) and np.array_equal(lp, again[1]) and ids.dtype == np.int32 and lp.dtype == np.float32
+    best, scores = model.recommend(users, liked[users], N=50)
+    u = np.random.RandomState(11).randint(0, 1 << 24, size=(4, 6)).astype(np.float32) * np.float32(2.0 ** -24)
+    check(torch.from_numpy(scores), torch.from_numpy(u), torch.from_numpy(ids), torch.from_numpy(lp), ids=torch.from_numpy(best),
+          T=0.4, top_p=0.95, min_p=0.01, replacement=False)
+    # one user; the attached matrix; temperature zero; a pool that the filter empties
+    model.attach_user_items(liked)
+    one, p1 = model.sample(3, N=6, pool=50, temperature=0.0, random_state=1)
+    assert one.shape == (6,) and one[0] == best[0, 0] and np.all(one[1:] == -1) and np.all(np.isneginf(p1[1:]))
+    with pytest.raises(_lib.MirecError):     # longer than the lists of the top-K kernels
+        model.sample([5], N=4, pool=10 ** 6, filter_already_liked_items=False, random_state=2)
+    wide, _ = model.sample([5], N=4, pool=224, filter_already_liked_items=False, random_state=2)
+    assert wide.shape == (1, 4) and np.all(wide >= 0)
+    everything = sp.csr_matrix(np.ones((1, 800), np.float32))
+    none, p0 = model.sample([5], everything, N=2, random_state=2)
+    assert np.all(none == -1) and np.all(np.isneginf(p0))
+    with pytest.raises(IndexError):
+        model.sample(60)
+    for bad in (dict(N=0), dict(pool=0)):
+        with pytest.raises(ValueError):
+            model.sample(1, **bad)
+    with pytest.raises(ValueError):
+        model.sample([1, 2], liked[:1])
+    with pytest.raises(_lib.MirecError):
+        model.sample(1, temperature=-1.0)
 
 
 @gpu
