@@ -127,12 +127,17 @@ __device__ __forceinline__ uint64_t sm_moved(uint64_t v) {   // 0 where no lane 
     return ((uint64_t)hi << 32) | lo;
 }
 
-__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {   // inclusive
+__device__ __forceinline__ uint64_t sm_half_scan(uint64_t v) {   // inclusive, over lanes 0 .. 31 and 32 .. 63
     v += sm_moved<0x111, 0xf>(v);   // shifted by 1, 2, 4, 8 within rows of 16 lanes
     v += sm_moved<0x112, 0xf>(v);
     v += sm_moved<0x114, 0xf>(v);
     v += sm_moved<0x118, 0xf>(v);
     v += sm_moved<0x142, 0xa>(v);   // lane 15 of a row to the next row: rows 1 and 3
+    return v;
+}
+
+__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
+    v = sm_half_scan(v);
     v += sm_moved<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
     return v;
 }
@@ -144,23 +149,32 @@ __device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {
 
 __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_lane(sm_wave_scan(v), 63); }
 
-__device__ __forceinline__ float sm_wave_max(float v) {
-#define SM_MAX_STEP(CTRL, ROWS)                                                                                        \
-    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(v), CTRL, ROWS, 0xf, false)))
-    SM_MAX_STEP(0x111, 0xf);
-    SM_MAX_STEP(0x112, 0xf);
-    SM_MAX_STEP(0x114, 0xf);
-    SM_MAX_STEP(0x118, 0xf);
-    SM_MAX_STEP(0x142, 0xa);
-    SM_MAX_STEP(0x143, 0xc);
-#undef SM_MAX_STEP
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float sm_max_moved(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(v), CTRL, ROWS, 0xf, false)));
 }
 
-// Where a number of [0, 1) falls in a total: floor(u * total), u moved into [0, 1 - 2^-53].
+__device__ __forceinline__ float sm_half_max(float v) {   // in lanes 31 and 63
+    v = sm_max_moved<0x111, 0xf>(v);
+    v = sm_max_moved<0x112, 0xf>(v);
+    v = sm_max_moved<0x114, 0xf>(v);
+    v = sm_max_moved<0x118, 0xf>(v);
+    return sm_max_moved<0x142, 0xa>(v);
+}
+
+__device__ __forceinline__ float sm_wave_max(float v) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sm_max_moved<0x143, 0xc>(sm_half_max(v))), 63));
+}
+
+// Where a number of [0, 1) falls in a total: floor(u * total), exactly (u is a 24-bit integer over a power of two); 0 for
+// NaN and below the range, total - 1 above it.
 __device__ __forceinline__ uint64_t sm_target(float u, uint64_t total) {
-    const double uc = u > 0.f ? fmin((double)u, 1.0 - 0x1p-53) : 0.0;
-    return __umul64hi(total, (uint64_t)(uc * 0x1p53) << 11);
+    const uint32_t b = __float_as_uint(fmaxf(u, 0.f)) & 0x7fffffffu, e = b >> 23;
+    const uint32_t M = (b & 0x7fffffu) | (e > 0 ? 0x800000u : 0u), q = 150 - (e > 0 ? e : 1);   // u = M 2^-q
+    const uint64_t lo = (uint64_t)M * (uint32_t)total, hi = (uint64_t)M * (uint32_t)(total >> 32) + (lo >> 32);
+    const uint64_t near = (hi << ((32 - q) & 63)) | ((uint32_t)lo >> (q & 31));   // 24 <= q < 32
+    const uint64_t far = hi >> (q - 32 < 63 ? q - 32 : 63);
+    return u >= 1.f ? total - 1 : q < 32 ? near : far;
 }
 
 // The least integer mass that is not below a share of a total.
@@ -201,49 +215,73 @@ __device__ __forceinline__ float sm_logprob(float score, double best, double ste
 
 // ------------------------------------------------------------------------------------------------------ short rows
 
-// One wavefront per row of at most 64 E items, all of it in registers: items E l .. E l + E - 1 in lane l, so that one scan
-// over the lanes gives every running sum.  A ranked list is in order already (one comparison of neighbours says so), and
-// then the running sum in index order is the running sum in rank order too: the scan serves the cuts and the draws.
-// Otherwise every item is compared with every other.  A wavefront takes `rows_each` rows, one after the other, and leaves
-// their draws in its lanes, one each, until there are 64 of them: logarithms and stores are then one for all.
-// What bounds it is the number of vector instructions per row.
-template <int DT, int E>
+// One wavefront per R rows of at most 64 E / R items, all of it in registers: items E l .. E l + E - 1 in lane l of the row's
+// lanes, so that one scan over the lanes gives every running sum.  A ranked list is in order already (one comparison of
+// neighbours says so), and then the running sum in index order is the running sum in rank order too: the scan serves the
+// cuts and the draws.  Otherwise every item is compared with every other.  The lanes of a row take `rows_each` rows, one after
+// the other, and keep their draws, one each, until all lanes have one: logarithms and stores are then one for all.
+// What bounds it is the number of vector instructions per row; most of them are for the row, not for its items, so that two
+// rows of up to 128 items share them.
+template <int DT, int E, int R>
 __global__ __launch_bounds__(256) void sample_short_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int m, int64_t stride, const int32_t* __restrict__ ids,
     int64_t ids_stride, const int64_t* __restrict__ mask_indptr, const int32_t* __restrict__ mask_indices,
     const float* __restrict__ uniforms, int draws, int replacement, int rows_each, SampleParams par, int bits,
     int32_t* __restrict__ out_ids, float* __restrict__ out_logprob) {
-    const int lane = threadIdx.x & 63;
+    constexpr int LANES = 64 / R;
+    const int lane = threadIdx.x & 63, half = R == 1 ? 0 : lane / LANES, sub = lane % LANES, first = E * sub;
     const double rounder = sm_rounder(bits);
-    const int64_t row0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * rows_each;
+    // Within a row's lanes: the value of a lane that is the same for both rows (`at`), or not (`pick`); of the last lane.
+    auto at32 = [&](uint32_t v, int l) -> uint32_t {
+        const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+        return R == 1 || half == 0 ? x : (uint32_t)__builtin_amdgcn_readlane((int)v, LANES + l);
+    };
+    auto at64 = [&](uint64_t v, int l) -> uint64_t { return ((uint64_t)at32((uint32_t)(v >> 32), l) << 32) | at32((uint32_t)v, l); };
+    auto pick32 = [&](uint32_t v, int l) -> uint32_t {
+        if (R == 1) return (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+        return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (half * LANES + l), (int)v);
+    };
+    auto pick64 = [&](uint64_t v, int l) -> uint64_t { return ((uint64_t)pick32((uint32_t)(v >> 32), l) << 32) | pick32((uint32_t)v, l); };
+    auto votes_of = [&](bool yes) -> uint64_t {
+        const uint64_t votes = __ballot(yes);
+        return R == 1 ? votes : half ? votes >> 32 : votes & 0xffffffffull;
+    };
+    auto first_vote = [&](uint64_t votes) -> int { return R == 1 ? __builtin_ctzll(votes) : __builtin_ctz((uint32_t)votes | 0x80000000u); };
+    auto scan64 = [&](uint64_t v) -> uint64_t { return R == 1 ? sm_wave_scan(v) : sm_half_scan(v); };
+
+    // the rows of these lanes, and one that is there for lanes without
+    const int64_t row0 = (((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * R + half) * rows_each;
     const int64_t row1 = row0 + rows_each < n ? row0 + rows_each : n;
+    int64_t row = row0 < n ? row0 : n - 1;
+    const typename ScoreType<DT>::raw* s = scores + row * stride;
+    const int32_t* list = ids ? ids + row * ids_stride : nullptr;
+    const float* uniform = uniforms + row * draws;
     // draws that are not written yet, in lanes 0 .. waiting - 1: number out0 + lane
     int waiting = 0;
     int64_t out0 = row0 * draws;
+    const int64_t out1 = row1 * draws;
     int32_t got = -1;
     float got_f = 0.f, got_best = 0.f;
     double got_step = 0.0;
     uint64_t got_total = 1;
     auto flush = [&]() {
-        if (lane < waiting) {
-            out_ids[out0 + lane] = got;
-            out_logprob[out0 + lane] = got >= 0 ? sm_logprob(got_f, (double)got_best, got_step, got_total, bits) : -INFINITY;
+        if (sub < waiting && out0 + sub < out1) {
+            out_ids[out0 + sub] = got;
+            out_logprob[out0 + sub] = got >= 0 ? sm_logprob(got_f, (double)got_best, got_step, got_total, bits) : -INFINITY;
         }
         out0 += waiting;
         waiting = 0;
     };
 
-    for (int64_t row = row0; row < row1; ++row) {
-        const typename ScoreType<DT>::raw* s = scores + row * stride;
-        const int first = E * lane;
+    for (int i = 0; i < rows_each && __any(row0 + i < row1); ++i) {
         float f[E];   // minus infinity where excluded; infinity counts as the largest finite score
         int32_t id[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             f[j] = first + j < m ? ScoreType<DT>::widen(s[first + j]) : -INFINITY;
-            id[j] = ids && first + j < m ? ids[row * ids_stride + first + j] : first + j;
+            id[j] = ids && first + j < m ? list[first + j] : first + j;
         }
-        const float u0 = lane < draws ? uniforms[row * draws + lane] : 0.f;
+        const float u0 = sub < draws ? uniform[sub] : 0.f;
 #pragma unroll
         for (int j = 0; j < E; ++j) f[j] = f[j] > ScoreType<DT>::lowest && id[j] >= 0 ? fminf(f[j], FLT_MAX) : -INFINITY;
         if (mask_indptr) {   // each lane looks for its items in the row's filter
@@ -256,16 +294,18 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
         float top = f[0];
 #pragma unroll
         for (int j = 1; j < E; ++j) top = fmaxf(top, f[j]);
-        top = sm_wave_max(top);
+        top = R == 1 ? sm_wave_max(top) : __uint_as_float(at32(__float_as_uint(sm_half_max(top)), LANES - 1));
         const RowCuts cut = sm_cuts(par, row, m, bits);
+        const int k = (int)cut.top_k;   // (at most m)
         const float best32 = top > -INFINITY ? top : 0.f;
         const double best = (double)best32;
         uint64_t w[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) w[j] = sm_weight(f[j], best, cut.step, rounder);
 
-        // in order if no item is better than the one before it (the next lane's first: minus infinity after lane 63)
+        // in order if no item is better than the one before it (the next lane's first: minus infinity after the last lane)
         float before_f = __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(f[0]), 0x130, 0xf, 0xf, false));
+        if (R > 1) before_f = sub == LANES - 1 ? -INFINITY : before_f;
         bool ordered = true;
 #pragma unroll
         for (int j = E - 1; j >= 0; --j) {
@@ -277,30 +317,35 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
             uint64_t sum = w[0];
 #pragma unroll
             for (int j = 1; j < E; ++j) sum += w[j];
-            const uint64_t inc = sm_wave_scan(sum);
+            const uint64_t inc = scan64(sum);
             run[E - 1] = inc;
 #pragma unroll
             for (int j = E - 1; j > 0; --j) run[j - 1] = run[j] - w[j];
-            return sm_lane(inc, 63);
+            return at64(inc, LANES - 1);
         };
         uint64_t total;
         if (__all(ordered)) {
-            if (cut.top_k < m) {
+            if (__any(k < m)) {
 #pragma unroll
-                for (int j = 0; j < E; ++j) w[j] = first + j < cut.top_k ? w[j] : 0ull;
+                for (int j = 0; j < E; ++j) w[j] = first + j < k ? w[j] : 0ull;
             }
             total = scan();
-            if (cut.top_p < 1.0 || cut.floor_w > 0) {
+            if (__any(cut.top_p < 1.0 || cut.floor_w > 0)) {
                 const uint64_t bound = cut.top_p < 1.0 ? sm_bound(cut.top_p, total) : ~0ull;
-                uint64_t last = 0;   // a prefix stays: the running sum at its end
+                // A prefix stays: the running sum at its end.  (What a draw looks for is the first running sum above a number
+                // below that: the items behind it may keep their weights.)
+                uint64_t last = 0;
+                const uint64_t least = cut.floor_w > 1 ? cut.floor_w : 1;
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
-                    const bool stays = (first + j == 0 || run[j] - w[j] < bound) && w[j] >= cut.floor_w && w[j] != 0;
-                    w[j] = stays ? w[j] : 0ull;
+                    const uint64_t before = j > 0 ? run[j - 1] : run[0] - w[0];
+                    const bool stays = (first + j == 0 || before < bound) && w[j] >= least;
                     last = stays ? run[j] : last;
                 }
-                const uint64_t votes = __ballot(last != 0);
-                total = votes ? sm_lane(last, 63 - __builtin_clzll(votes)) : 0ull;
+                const uint64_t votes = votes_of(last != 0);
+                const int l = R == 1 ? 63 - __builtin_clzll(votes | 1) : 31 - __builtin_clz((uint32_t)votes | 1);
+                const uint64_t mass = pick64(last, l);
+                total = votes ? mass : 0ull;
             }
         } else {
             uint32_t rank[E];
@@ -310,12 +355,12 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
                 rank[j] = 0;
                 before[j] = 0;
             }
-            if (cut.top_k < m || cut.top_p < 1.0) {
+            if (__any(k < m || cut.top_p < 1.0)) {
                 for (int l = 0; E * l < m; ++l)
 #pragma unroll
                     for (int q = 0; q < E; ++q) {
-                        const float g = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[q]), l));
-                        const uint64_t gw = sm_lane(w[q], l);
+                        const float g = __uint_as_float(at32(__float_as_uint(f[q]), l));
+                        const uint64_t gw = at64(w[q], l);
 #pragma unroll
                         for (int j = 0; j < E; ++j) {
                             const bool ahead = g > f[j] || (g == f[j] && E * l + q < first + j);
@@ -327,55 +372,55 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
             uint64_t mass = 0;
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                if (rank[j] >= cut.top_k) w[j] = 0;
+                if (rank[j] >= (uint32_t)k) w[j] = 0;
                 mass += w[j];
             }
-            const uint64_t bound = cut.top_p < 1.0 ? sm_bound(cut.top_p, sm_wave_sum(mass)) : ~0ull;
+            mass = at64(scan64(mass), LANES - 1);
+            const uint64_t bound = cut.top_p < 1.0 ? sm_bound(cut.top_p, mass) : ~0ull;
 #pragma unroll
             for (int j = 0; j < E; ++j)
                 if (!((rank[j] == 0 || before[j] < bound) && w[j] >= cut.floor_w)) w[j] = 0;
             total = scan();
         }
 
-        for (int d0 = 0; d0 < draws; d0 += 64) {
-            const int cnt = draws - d0 < 64 ? draws - d0 : 64;
-            const float u = d0 == 0 ? u0 : lane < cnt ? uniforms[row * draws + d0 + lane] : 0.f;
-            if (waiting + cnt > 64) flush();
+        for (int d0 = 0; d0 < draws; d0 += LANES) {
+            const int cnt = draws - d0 < LANES ? draws - d0 : LANES;
+            const float u = d0 == 0 ? u0 : sub < cnt ? uniform[d0 + sub] : 0.f;
+            if (waiting + cnt > LANES) flush();
             const uint64_t targets = sm_target(u, total);
             for (int d = 0; d < cnt; ++d, ++waiting) {
-                if (total == 0) {
-                    if (lane == waiting) got = -1;
+                if (!__any(total != 0)) {
+                    if (sub == waiting) got = -1;
                     continue;
                 }
-                const uint64_t t = replacement ? sm_lane(targets, d)
-                                               : sm_target(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(u), d)), total);
+                const uint64_t t = replacement ? at64(targets, d) : sm_target(__uint_as_float(at32(__float_as_uint(u), d)), total);
                 // the first lane whose last running sum is above the number, and its first item for which that holds
-                const int l = __builtin_ctzll(__ballot(run[E - 1] > t));
+                const int l = first_vote(votes_of(run[E - 1] > t));
                 int j_of = E - 1;
-#pragma unroll
-                for (int j = E - 2; j >= 0; --j) j_of = run[j] > t ? j : j_of;
                 int32_t my_id = id[E - 1];
                 float my_f = f[E - 1];
 #pragma unroll
                 for (int j = E - 2; j >= 0; --j) {
-                    my_id = j_of == j ? id[j] : my_id;
-                    my_f = j_of == j ? f[j] : my_f;
+                    const bool above = run[j] > t;
+                    j_of = above ? j : j_of;
+                    my_id = above ? id[j] : my_id;
+                    my_f = above ? f[j] : my_f;
                 }
-                const int32_t item = __builtin_amdgcn_readlane(my_id, l);
-                const float score = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_f), l));
-                if (lane == waiting) {
-                    got = item;
+                const int32_t item = (int32_t)pick32((uint32_t)my_id, l);
+                const float score = __uint_as_float(pick32(__float_as_uint(my_f), l));
+                if (sub == waiting) {
+                    got = total != 0 ? item : -1;
                     got_f = score;
                     got_best = best32;
                     got_step = cut.step;
                     got_total = total;
                 }
                 if (!replacement) {   // the item leaves: every running sum from it on is lower by its weight
-                    const int at = E * l + __builtin_amdgcn_readlane(j_of, l);
+                    const int at = E * l + (int)pick32((uint32_t)j_of, l);
                     uint64_t mine = 0;
 #pragma unroll
                     for (int j = 0; j < E; ++j) mine = first + j == at ? w[j] : mine;
-                    const uint64_t gone = sm_lane(mine, l);
+                    const uint64_t leaves = pick64(mine, l), gone = total != 0 ? leaves : 0ull;
                     total -= gone;
 #pragma unroll
                     for (int j = 0; j < E; ++j) {
@@ -384,6 +429,12 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
                     }
                 }
             }
+        }
+        if (row + 1 < row1) {   // (lanes without a further row stay where they are; what they draw is not written)
+            ++row;
+            s += stride;
+            if (ids) list += ids_stride;
+            uniform += draws;
         }
     }
     flush();
@@ -1093,17 +1144,17 @@ static int sample_bits(int64_t m) {
     return 62 - b < 51 ? 62 - b : 51;
 }
 
-template <int DT, int E>
+template <int DT, int E, int R>
 static int launch_short(const typename ScoreType<DT>::raw* scores, int64_t n, int m, int64_t stride, const int32_t* ids,
                         int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
                         int draws, int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
                         hipStream_t stream) {
-    // a row per wavefront until the chip is full (256 compute units of 28 wavefronts), then runs of up to 64
-    int64_t rows_each = n / (256 * 28);
+    // each row its lanes until the chip is full (256 compute units of 28 wavefronts), then runs of up to 64 rows
+    int64_t rows_each = n / (256 * 28 * R);
     rows_each = rows_each < 1 ? 1 : rows_each > 64 ? 64 : rows_each;
-    const int64_t blocks = (n + 4 * rows_each - 1) / (4 * rows_each);
+    const int64_t blocks = (n + 4 * R * rows_each - 1) / (4 * R * rows_each);
     MIREC_REQUIRE(blocks < ((int64_t)1 << 24), MIREC_E_UNSUPPORTED, "mirec_sample: more than 2^32 rows");
-    hipLaunchKernelGGL((sample_short_kernel<DT, E>), dim3((unsigned)blocks), dim3(256), 0, stream, scores, n, m, stride, ids,
+    hipLaunchKernelGGL((sample_short_kernel<DT, E, R>), dim3((unsigned)blocks), dim3(256), 0, stream, scores, n, m, stride, ids,
                        ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, (int)rows_each, par, bits, out_ids,
                        out_logprob);
     MIREC_LAUNCH_CHECK();
@@ -1139,9 +1190,13 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
                          hipStream_t stream) {
     const typename ScoreType<DT>::raw* scores = (const typename ScoreType<DT>::raw*)scores_;
 #define MIREC_SAMPLE_ARGS stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids, out_logprob, stream
-    if (m <= 64) return launch_short<DT, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
-    if (m <= 128) return launch_short<DT, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
-    if (m <= SM_SHORT) return launch_short<DT, 4>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    // Ranked lists are in order and cost what a row costs: two share a wavefront (262144 of 50 items: 107 -> 81 us).  Dense
+    // rows cost their comparisons: a wavefront each (one of 100 items: 33 us shared, 16 us alone).
+    if (ids && m <= 64) return launch_short<DT, 2, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    if (ids && m <= 128) return launch_short<DT, 4, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    if (m <= 64) return launch_short<DT, 1, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    if (m <= 128) return launch_short<DT, 2, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    if (m <= SM_SHORT) return launch_short<DT, 4, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (n <= SM_FEW_ROWS && m > 8192) return launch_long<DT, 1024>(scores, n, m, MIREC_SAMPLE_ARGS);
     if (m > 8192) return launch_long<DT, 512>(scores, n, m, MIREC_SAMPLE_ARGS);
     return launch_long<DT, 256>(scores, n, m, MIREC_SAMPLE_ARGS);
