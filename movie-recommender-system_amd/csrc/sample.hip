@@ -20,7 +20,7 @@ namespace mirec {
 constexpr int SM_MAX_DRAWS = MIREC_SAMPLE_MAX_DRAWS;
 constexpr int64_t SM_MAX_MASKED_ITEMS = MIREC_SAMPLE_MAX_MASKED_ITEMS;   // the filter of a row is a bitmap in LDS
 constexpr double SM_MIN_TEMPERATURE = 1e-37;      // below: greedy
-constexpr int SM_SHORT = 256;                     // rows up to this length: one wavefront each
+constexpr int SM_SHORT = 256;                     // rows up to this length: in the registers of a wavefront
 constexpr int64_t SM_FEW_ROWS = 256;              // no more rows than compute units: larger workgroups
 constexpr int SM_AHEAD = 2;                       // loads in flight ahead of the work
 constexpr int SM_BINS = 1024;                     // of a histogram over a row
@@ -234,7 +234,9 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
     // Within a row's lanes: the value of a lane that is the same for both rows (`at`), or not (`pick`); of the last lane.
     auto at32 = [&](uint32_t v, int l) -> uint32_t {
         const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)v, l);
-        return R == 1 || half == 0 ? x : (uint32_t)__builtin_amdgcn_readlane((int)v, LANES + l);
+        if (R == 1) return x;
+        const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)v, LANES + l);
+        return half ? y : x;
     };
     auto at64 = [&](uint64_t v, int l) -> uint64_t { return ((uint64_t)at32((uint32_t)(v >> 32), l) << 32) | at32((uint32_t)v, l); };
     auto pick32 = [&](uint32_t v, int l) -> uint32_t {
@@ -273,19 +275,41 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
         waiting = 0;
     };
 
+    // A row is read while the one before it is worked on.
+    typename ScoreType<DT>::raw next_s[E];
+    int32_t next_id[E];
+    float next_u = 0.f;
+    auto fetch = [&]() {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (first + j < m) {
+                next_s[j] = s[first + j];
+                if (ids) next_id[j] = list[first + j];
+            }
+        if (sub < draws) next_u = uniform[sub];
+    };
+    fetch();
     for (int i = 0; i < rows_each && __any(row0 + i < row1); ++i) {
         float f[E];   // minus infinity where excluded; infinity counts as the largest finite score
         int32_t id[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            f[j] = first + j < m ? ScoreType<DT>::widen(s[first + j]) : -INFINITY;
-            id[j] = ids && first + j < m ? list[first + j] : first + j;
+            const float v = ScoreType<DT>::widen(next_s[j]);
+            id[j] = ids ? next_id[j] : first + j;
+            f[j] = first + j < m && v > ScoreType<DT>::lowest && id[j] >= 0 ? fminf(v, FLT_MAX) : -INFINITY;
         }
-        const float u0 = sub < draws ? uniform[sub] : 0.f;
-#pragma unroll
-        for (int j = 0; j < E; ++j) f[j] = f[j] > ScoreType<DT>::lowest && id[j] >= 0 ? fminf(f[j], FLT_MAX) : -INFINITY;
+        const float u0 = next_u;
+        const float* row_u = uniform;
+        const int64_t this_row = row;
+        if (row + 1 < row1) {   // (lanes without a further row stay where they are; what they draw is not written)
+            ++row;
+            s += stride;
+            if (ids) list += ids_stride;
+            uniform += draws;
+        }
+        if (i + 1 < rows_each) fetch();
         if (mask_indptr) {   // each lane looks for its items in the row's filter
-            for (int64_t e = mask_indptr[row]; e < mask_indptr[row + 1]; ++e) {
+            for (int64_t e = mask_indptr[this_row]; e < mask_indptr[this_row + 1]; ++e) {
                 const int32_t it = mask_indices[e];
 #pragma unroll
                 for (int j = 0; j < E; ++j) f[j] = it == first + j ? -INFINITY : f[j];
@@ -295,7 +319,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
 #pragma unroll
         for (int j = 1; j < E; ++j) top = fmaxf(top, f[j]);
         top = R == 1 ? sm_wave_max(top) : __uint_as_float(at32(__float_as_uint(sm_half_max(top)), LANES - 1));
-        const RowCuts cut = sm_cuts(par, row, m, bits);
+        const RowCuts cut = sm_cuts(par, this_row, m, bits);
         const int k = (int)cut.top_k;   // (at most m)
         const float best32 = top > -INFINITY ? top : 0.f;
         const double best = (double)best32;
@@ -363,7 +387,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
                         const uint64_t gw = at64(w[q], l);
 #pragma unroll
                         for (int j = 0; j < E; ++j) {
-                            const bool ahead = g > f[j] || (g == f[j] && E * l + q < first + j);
+                            const bool ahead = (g > f[j]) | ((g == f[j]) & (E * l + q < first + j));
                             rank[j] += ahead ? 1u : 0u;
                             before[j] += ahead ? gw : 0ull;
                         }
@@ -385,7 +409,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
 
         for (int d0 = 0; d0 < draws; d0 += LANES) {
             const int cnt = draws - d0 < LANES ? draws - d0 : LANES;
-            const float u = d0 == 0 ? u0 : sub < cnt ? uniform[d0 + sub] : 0.f;
+            const float u = d0 == 0 ? u0 : sub < cnt ? row_u[d0 + sub] : 0.f;
             if (waiting + cnt > LANES) flush();
             const uint64_t targets = sm_target(u, total);
             for (int d = 0; d < cnt; ++d, ++waiting) {
@@ -429,12 +453,6 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
                     }
                 }
             }
-        }
-        if (row + 1 < row1) {   // (lanes without a further row stay where they are; what they draw is not written)
-            ++row;
-            s += stride;
-            if (ids) list += ids_stride;
-            uniform += draws;
         }
     }
     flush();
@@ -1190,11 +1208,11 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
                          hipStream_t stream) {
     const typename ScoreType<DT>::raw* scores = (const typename ScoreType<DT>::raw*)scores_;
 #define MIREC_SAMPLE_ARGS stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids, out_logprob, stream
-    // Ranked lists are in order and cost what a row costs: two share a wavefront (262144 of 50 items: 107 -> 81 us).  Dense
-    // rows cost their comparisons: a wavefront each (one of 100 items: 33 us shared, 16 us alone).
-    if (ids && m <= 64) return launch_short<DT, 2, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
+    // Two rows to a wavefront where a row has at most two items a lane then (262144 lists of 50: 107 -> 76 us).  Up to 128
+    // items ranked lists, which are in order, still gain (of 100: 139 -> 107 us); dense rows cost their comparisons and are
+    // sooner done with a wavefront each (one of 100: 17 us shared, 11 us alone; 262144: 1.28 ms either way).
+    if (m <= 64) return launch_short<DT, 2, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (ids && m <= 128) return launch_short<DT, 4, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
-    if (m <= 64) return launch_short<DT, 1, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= 128) return launch_short<DT, 2, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= SM_SHORT) return launch_short<DT, 4, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (n <= SM_FEW_ROWS && m > 8192) return launch_long<DT, 1024>(scores, n, m, MIREC_SAMPLE_ARGS);
