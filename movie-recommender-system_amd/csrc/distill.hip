@@ -193,11 +193,14 @@ __device__ __forceinline__ uint32_t di_pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
 }
 
-// (a, b) -> packed pairs hi, mid; both roundings to nearest, the remainder is exact.
+// (a, b) -> packed pairs hi, mid; both roundings to nearest, the remainder is exact (one instruction for the widening of hi
+// and the difference).
 __device__ __forceinline__ void di_split(float a, float b, uint32_t& hi, uint32_t& mid) {
     hi = di_pack(a, b);
-    const f16x2 h = __builtin_bit_cast(f16x2, hi);
-    mid = di_pack(a - (float)h[0], b - (float)h[1]);
+    float ra, rb;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hi), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hi), "v"(b));
+    mid = di_pack(ra, rb);
 }
 
 // One workgroup per tile: tiles of X first, then tiles of Y.  Rows behind the last are zero.
@@ -585,13 +588,22 @@ __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* _
     const int64_t begin = di_run_begin(blockIdx.x + 1, steps, runs), block = begin / xtiles, s0 = block * xtiles, s1 = s0 + xtiles;
     const int64_t w0 = blockIdx.x, before = di_run_begin(w0, steps, runs);   // the run that ends inside the block
     if (begin == s0 || before > s0) return;
-    int64_t w1 = w0 + 1;   // one past the last run with a part of the block
-    while (w1 < runs && di_run_begin(w1, steps, runs) < s1) ++w1;
+    // one past the last run with a part of the block: the first whose steps begin behind it
+    int64_t w1 = (s1 * runs + steps - 1) / steps;
+    w1 = w1 < runs ? w1 : runs;
     const int first_slot = before == s0 ? 0 : 1;
     const int64_t rows = m - block * DI_OWN < DI_OWN ? m - block * DI_OWN : DI_OWN;
     for (int64_t e = ((int64_t)blockIdx.y * DI_THREADS + threadIdx.x) * 4; e < rows * f; e += (int64_t)gridDim.y * DI_THREADS * 4) {
         f32x4 v = *reinterpret_cast<const f32x4*>(slots + (2 * w0 + first_slot) * DI_OWN * f + e);
-        for (int64_t w = w0 + 1; w < w1; ++w) v += *reinterpret_cast<const f32x4*>(slots + 2 * w * DI_OWN * f + e);
+        for (int64_t w = w0 + 1; w < w1; w += 4) {   // four parts asked for at once
+            f32x4 part[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (w + u < w1) part[u] = *reinterpret_cast<const f32x4*>(slots + 2 * (w + u) * DI_OWN * f + e);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (w + u < w1) v += part[u];
+        }
         *reinterpret_cast<f32x4*>(dY + block * DI_OWN * f + e) = v;
     }
 }
