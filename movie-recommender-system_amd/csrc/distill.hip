@@ -633,7 +633,7 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
     float* sp = reinterpret_cast<float*>(sid + kp);                 // p
     float* slogp = sp + kp;
     int32_t* mid = reinterpret_cast<int32_t*>(slogp + kp);          // merged
-    float* mz = reinterpret_cast<float*>(mid + kp);                 // logits, then the coefficients of y in dX
+    float* mz = reinterpret_cast<float*>(mid + kp);                 // logits
     float* mp = reinterpret_cast<float*>(key);
     float* mlogp = mp + kp;
     __shared__ float red[NWV][F];
@@ -772,7 +772,9 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
             }
         }
         __syncthreads();
-        // the student's logits on the list
+        // The student's logits and probabilities on the list, and the items' sums under both distributions: a factor row is
+        // read once.
+        f32x2 sum_py[PIECES] = {}, sum_qy[PIECES] = {};
         for (int e0 = group; e0 - group < merged; e0 += 4 * ROWS) {
             f32x2 y[4][PIECES];
 #pragma unroll
@@ -793,18 +795,33 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
                 }
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
-                if (sub == 0 && e < merged) mz[e] = z;
+                const double lq = (double)z * inv_t - log_mass;
+                const float q = expf((float)lq), p = mp[e < merged ? e : 0];
+                if (e < merged) {
+                    if (sub == 0) {
+                        mz[e] = z;
+                        sp[e] = q;
+                    }
+                    if (base) {
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                sum_py[i][j] = __builtin_fmaf(p, y[u][i][j], sum_py[i][j]);
+                                if (teacher_lse) sum_qy[i][j] = __builtin_fmaf(q, y[u][i][j], sum_qy[i][j]);
+                            }
+                    }
+                }
             }
         }
         __syncthreads();
         double kl = 0.0, sum_p = 0.0, sum_q = 0.0;
         for (int e = tid; e < merged; e += NT) {
             const double logq = (double)mz[e] * inv_t - log_mass;
-            const float p = mp[e], q = expf((float)logq);
+            const float p = mp[e], q = sp[e];
             if (!(p <= 0.f)) kl += (double)p * ((double)mlogp[e] - logq);   // (a NaN probability stays in the sum)
             sum_p += (double)p;
             sum_q += (double)q;
-            sp[e] = q;
         }
         kl = block_sum(kl, 0);
         float a = 1.f;
@@ -825,25 +842,27 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
         for (int e = tid; e < merged; e += NT) {
             id_out[b * k + e] = mid[e];
             val_out[b * k + e] = sp[e] - mp[e];
-            mz[e] = (1.f - a) * sp[e] - mp[e];
         }
-        __syncthreads();
-        // dX but for its weight: listed items and the ranges' sums under the softmax, by their coefficients
-        f32x2 sum[PIECES] = {};
-        for (int e0 = group; e0 - group < merged + ranges; e0 += 4 * ROWS) {
+        // dX but for its weight: (1 - A) sum q y - sum p y over the list, and A times the ranges' sums
+        f32x2 sum[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) sum[i][j] = __builtin_fmaf(1.f - a, sum_qy[i][j], -sum_py[i][j]);
+        for (int r0 = group; r0 - group < ranges; r0 += 4 * ROWS) {
             f32x2 y[4][PIECES];
             float w[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int e = e0 + u * ROWS, r = e - merged;
-                w[u] = e < merged ? mz[e] : r < ranges ? a * range_w[r] : 0.f;
-                const float* v = (e < merged ? Y + (int64_t)mid[e] * F : psum + ((r < ranges ? r : 0) * n + b) * F) + 2 * sub;
+                const int r = r0 + u * ROWS;
+                w[u] = r < ranges ? a * range_w[r] : 0.f;
+                const float* v = psum + ((r < ranges ? r : 0) * n + b) * F + 2 * sub;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) y[u][i] = *reinterpret_cast<const f32x2*>(v + 32 * i);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const bool real = e0 + u * ROWS < merged + ranges;
+                const bool real = r0 + u * ROWS < ranges;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
                     sum[i][0] = real ? __builtin_fmaf(w[u], y[u][i][0], sum[i][0]) : sum[i][0];
