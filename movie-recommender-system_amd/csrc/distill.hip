@@ -108,7 +108,7 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.mass_off = take((size_t)n * 4);         // sum_j 2^(z_bj log2 e - M_b)
     w.a_off = take((size_t)n * 4);            // A_b
     w.count_off = take((size_t)n * 4);        // entries of the merged list
-    w.id_off = take((size_t)n * k * 4);       // merged list, ascending ids
+    w.id_off = take((size_t)n * k * 4);       // merged list
     w.val_off = take((size_t)n * k * 4);      // q - p of those
     // the same by (row tile, item tile): where a group begins, the entries' places in their 32 x 32 block, q - p
     w.start_off = take((size_t)w.xtiles * (w.ytiles + 1) * 2);
@@ -625,17 +625,19 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
     float* __restrict__ base) {
     constexpr int PIECES = F / 32;     // 8-byte pieces of a factor row per lane
     constexpr int ROWS = NT / 16;      // factor rows that the workgroup reads side by side
-    constexpr int NWV = NT / 64;
+    constexpr int NWV = NT / 64, PER = DI_LIST / NT;
     extern __shared__ __attribute__((aligned(16))) char list_lds[];
     const int kp = (k + 63) & ~63;
-    uint64_t* key = reinterpret_cast<uint64_t*>(list_lds);          // item and place; later p and log p of the merged entries
-    int32_t* sid = reinterpret_cast<int32_t*>(key + kp);            // by ascending item
-    float* sp = reinterpret_cast<float*>(sid + kp);                 // p
-    float* slogp = sp + kp;
-    int32_t* mid = reinterpret_cast<int32_t*>(slogp + kp);          // merged
-    float* mz = reinterpret_cast<float*>(mid + kp);                 // logits
-    float* mp = reinterpret_cast<float*>(key);
+    uint64_t* key = reinterpret_cast<uint64_t*>(list_lds);          // item and place, where an item is listed twice
+    int32_t* table = reinterpret_cast<int32_t*>(key);               // before that: the items, hashed
+    float* mp = reinterpret_cast<float*>(key);                      // after that: p and log p of the merged entries
     float* mlogp = mp + kp;
+    int32_t* sid = reinterpret_cast<int32_t*>(key + kp);            // by ascending item
+    float* sp = reinterpret_cast<float*>(sid + kp);                 // p, then q
+    int32_t* mid = reinterpret_cast<int32_t*>(sp + kp);             // merged
+    float* mz = reinterpret_cast<float*>(mid + kp);                 // log p, then logits
+    int slots = 2 * kp;                                             // of the table: a power of two
+    while (slots & (slots - 1)) slots &= slots - 1;
     __shared__ float red[NWV][F];
     __shared__ float range_w[64];
     __shared__ float row_ref, row_mass;
@@ -677,34 +679,54 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
                 mass_out[b] = row_mass;
             }
         }
-        // the entries that count, the best of them and their mass
+        // The entries that count, the best of them, and whether two name the same item (a hash table, open addressing: at
+        // least a quarter of it stays empty).
+        int32_t my_id[PER];   // entry tid + NT i; -1: left out
+        float my_s[PER];
         float top = -INFINITY;
         int valid = 0;
-        for (int e = tid; e < kp; e += NT) {
-            const int32_t id = e < k ? ids[b * k + e] : -1;
-            const float s = e < k ? scores[b * k + e] : 0.f;
-            const bool ok = id >= 0 && id < m && s > -FLT_MAX;
-            key[e] = ok ? ((uint64_t)id << 8) | (uint64_t)e : ~0ull;
-            slogp[e] = s;
-            if (ok) top = fmaxf(top, s);
-            valid += ok ? 1 : 0;
+        bool twice = false;
+        for (int e = tid; e < slots; e += NT) table[e] = -1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = tid + NT * i;
+            my_id[i] = e < k ? ids[b * k + e] : -1;
+            my_s[i] = e < k ? scores[b * k + e] : 0.f;
+            if (!(my_id[i] >= 0 && my_id[i] < m && my_s[i] > -FLT_MAX)) my_id[i] = -1;
+            if (my_id[i] >= 0) top = fmaxf(top, my_s[i]);
+            valid += my_id[i] >= 0 ? 1 : 0;
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (my_id[i] >= 0) {
+                uint32_t at = ((uint32_t)my_id[i] * 2654435769u >> 16) & (uint32_t)(slots - 1);
+                for (;;) {
+                    const int32_t there = atomicCAS(&table[at], -1, my_id[i]);
+                    twice = twice || there == my_id[i];
+                    if (there == -1 || there == my_id[i]) break;
+                    at = (at + 1) & (uint32_t)(slots - 1);
+                }
+            }
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) {
             top = fmaxf(top, __shfl_xor(top, d, 64));
             valid += __shfl_xor(valid, d, 64);
         }
+        int again = __any(twice) ? 1 : 0;
         if (NWV > 1) {
             if (lane == 0) {
                 sp[wave] = top;
-                parti[wave] = valid;
+                parti[wave] = 2 * valid + again;
             }
             __syncthreads();
             top = sp[0];
-            valid = parti[0];
+            valid = parti[0] >> 1;
+            again = parti[0] & 1;
             for (int w = 1; w < NWV; ++w) {
                 top = fmaxf(top, sp[w]);
-                valid += parti[w];
+                valid += parti[w] >> 1;
+                again |= parti[w] & 1;
             }
         }
         __syncthreads();
@@ -725,50 +747,73 @@ __global__ __launch_bounds__(NT) void distill_list_kernel(
             teacher = (double)teacher_lse[b] - (double)top * inv_t;
         } else {
             double mass = 0.0;
-            for (int e = tid; e < kp; e += NT)
-                if (key[e] != ~0ull) mass += slogp[e] == top ? 1.0 : (double)expf((float)(((double)slogp[e] - (double)top) * inv_t));
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (my_id[i] >= 0) mass += my_s[i] == top ? 1.0 : (double)expf((float)(((double)my_s[i] - (double)top) * inv_t));
             teacher = log(block_sum(mass, 0));
         }
-        for (int e = tid; e < kp; e += NT) {
-            const uint64_t mine = key[e];
-            if (mine == ~0ull) continue;
-            int rank = 0;
-            const ulonglong2* kv = reinterpret_cast<const ulonglong2*>(key);
-#pragma unroll 8
-            for (int j = 0; j < kp / 2; ++j) rank += (kv[j].x < mine ? 1 : 0) + (kv[j].y < mine ? 1 : 0);
-            const float s = slogp[e];
-            const float lp = (float)((s == top ? 0.0 : ((double)s - (double)top) * inv_t) - teacher);
-            sid[rank] = (int32_t)(mine >> 8);
-            mz[rank] = lp;
-            sp[rank] = expf(lp);
-        }
-        __syncthreads();
-        // entries of one item become one
-        int merged = 0;
-        for (int e0 = 0; e0 < valid; e0 += NT) {
-            const int e = e0 + tid;
-            const bool head = e < valid && (e == 0 || sid[e] != sid[e - 1]);
-            const uint64_t votes = __ballot(head);
-            int at = merged + __popcll(votes & ((1ull << lane) - 1));
+        auto logp_of = [&](float s) -> float { return (float)((s == top ? 0.0 : ((double)s - (double)top) * inv_t) - teacher); };
+        // where the chosen entries of this step go: behind `done`, in order
+        auto place_of = [&](bool chosen, int& done) -> int {
+            const uint64_t votes = __ballot(chosen);
+            int at = done + __popcll(votes & ((1ull << lane) - 1));
             if (NWV > 1) {
                 if (lane == 0) parti[wave] = __popcll(votes);
                 __syncthreads();
                 for (int w = 0; w < NWV; ++w) {
                     at += w < wave ? parti[w] : 0;
-                    merged += parti[w];
+                    done += parti[w];
                 }
                 __syncthreads();
             } else {
-                merged += __popcll(votes);
+                done += __popcll(votes);
             }
-            if (head) {
-                float p = sp[e], lp = mz[e];
-                int j = e + 1;
-                for (; j < valid && sid[j] == sid[e]; ++j) p += sp[j];
-                if (j > e + 1) lp = logf(p);
-                mid[at] = sid[e];
-                mp[at] = p;
-                mlogp[at] = lp;
+            return at;
+        };
+        int merged = 0;
+        if (!again) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int at = place_of(my_id[i] >= 0, merged);
+                if (my_id[i] >= 0) {
+                    const float lp = logp_of(my_s[i]);
+                    mid[at] = my_id[i];
+                    mp[at] = expf(lp);
+                    mlogp[at] = lp;
+                }
+            }
+        } else {   // by ascending item; entries of one item become one
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (tid + NT * i < kp) key[tid + NT * i] = my_id[i] >= 0 ? ((uint64_t)my_id[i] << 8) | (uint64_t)(tid + NT * i) : ~0ull;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (my_id[i] < 0) continue;
+                const uint64_t mine = key[tid + NT * i];
+                int rank = 0;
+                const ulonglong2* kv = reinterpret_cast<const ulonglong2*>(key);
+#pragma unroll 8
+                for (int j = 0; j < kp / 2; ++j) rank += (kv[j].x < mine ? 1 : 0) + (kv[j].y < mine ? 1 : 0);
+                const float lp = logp_of(my_s[i]);
+                sid[rank] = my_id[i];
+                mz[rank] = lp;
+                sp[rank] = expf(lp);
+            }
+            __syncthreads();
+            for (int e0 = 0; e0 < valid; e0 += NT) {
+                const int e = e0 + tid;
+                const bool head = e < valid && (e == 0 || sid[e] != sid[e - 1]);
+                const int at = place_of(head, merged);
+                if (head) {
+                    float p = sp[e], lp = mz[e];
+                    int j = e + 1;
+                    for (; j < valid && sid[j] == sid[e]; ++j) p += sp[j];
+                    if (j > e + 1) lp = logf(p);
+                    mid[at] = sid[e];
+                    mp[at] = p;
+                    mlogp[at] = lp;
+                }
             }
         }
         __syncthreads();
@@ -1063,7 +1108,7 @@ static int launch_forward(const DistillWorkspace& L, char* w, const float* X, in
     MIREC_LAUNCH_CHECK();
     const int nt = n >= DI_MANY_ROWS ? 64 : 256;
     hipLaunchKernelGGL(nt == 64 ? (distill_list_kernel<F, 64>) : (distill_list_kernel<F, 256>),
-                       dim3((unsigned)(n < 262144 ? n : 262144)), dim3(nt), (size_t)((k + 63) & ~63) * 28, stream, X, n, Y, m,
+                       dim3((unsigned)(n < 262144 ? n : 262144)), dim3(nt), (size_t)((k + 63) & ~63) * 24, stream, X, n, Y, m,
                        ids, scores, k, temperature, teacher_lse, (int)ranges, (const float*)(w + L.pref_off),
                        (const float*)(w + L.pmass_off), (const float*)(w + L.part_off), parts, loss, (float*)(w + L.ref_off),
                        (float*)(w + L.mass_off), (float*)(w + L.a_off), (int32_t*)(w + L.count_off), (int32_t*)(w + L.id_off),
