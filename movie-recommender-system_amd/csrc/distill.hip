@@ -43,6 +43,7 @@ constexpr int DI_PREPARE_THREADS = 1024;
 constexpr int DI_WEIGH_BLOCKS = 64;
 constexpr int DI_BINS = 4096;                     // item tiles that di_group counts at a time
 constexpr int DI_CUS = 256;                       // workgroups that run at once
+constexpr int DI_FEW_TILES = 4;                   // of rows: the backward pass does not cut its blocks of items
 constexpr float DI_HEADROOM = 7.f;                // log2 of a probability's scale when its row's reference is current
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -102,7 +103,9 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.ytiles = (m + 31) / 32;
     const int64_t xblocks = (n + DI_OWN - 1) / DI_OWN, yblocks = (m + DI_OWN - 1) / DI_OWN;
     w.splits_x = distill_splits(xblocks, w.ytiles);
-    w.runs = yblocks * w.xtiles < DI_CUS ? yblocks * w.xtiles : DI_CUS;
+    // (few row tiles: whole blocks of items, nothing to join.  128 rows of 27000 items at 128 columns: 84 us with the blocks
+    // cut, 71 whole; 256 rows of 7207 items at 96 columns: 56 and 64)
+    w.runs = w.xtiles <= DI_FEW_TILES && yblocks < DI_CUS ? yblocks : yblocks * w.xtiles < DI_CUS ? yblocks * w.xtiles : DI_CUS;
     w.max_off = take(3 * DI_PARTS * 4);       // partial maxima of |X|, |Y|, |grad|
     w.ref_off = take((size_t)n * 4);          // M_b: log2 reference of a row's mass
     w.mass_off = take((size_t)n * 4);         // sum_j 2^(z_bj log2 e - M_b)
@@ -614,9 +617,10 @@ __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* _
 // same item merged (their probabilities add); the row's loss; its dX but for the weight.  Latency, not bandwidth, is
 // what a row costs (a chain of a dozen dependent steps): factor rows are read by sixteen lanes each, four rows of a
 // group of lanes in flight, and what does not depend on each other is asked for at once.  NT threads: 256 finish a row
-// soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) many rows: DI_MANY_ROWS.
+// soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) many rows: DI_MANY_ROWS (4096 lists of
+// 100 at 128 columns: 34 us, of which the factor rows, 0.2 GB from L2, are a third).
 template <int F, int NT>
-__global__ __launch_bounds__(NT) void distill_list_kernel(
+__global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list_kernel(
     const float* __restrict__ X, int64_t n, const float* __restrict__ Y, int64_t m, const int32_t* __restrict__ ids,
     const float* __restrict__ scores, int k, float temperature, const float* __restrict__ teacher_lse, int ranges,
     const float* __restrict__ pref, const float* __restrict__ pmass, const float* __restrict__ psum,
@@ -1130,7 +1134,7 @@ static int launch_backward(const DistillWorkspace& L, char* w, int64_t n, int64_
                        (const float*)(w + L.row_off), (const uint16_t*)(w + L.start_off), L.ytiles,
                        (const uint16_t*)(w + L.place_off), (const float*)(w + L.gval_off), k, dY, slots);
     MIREC_LAUNCH_CHECK();
-    if (L.runs > 1) {
+    if (blocks % L.runs != 0) {   // (else every run is of whole blocks)
         hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)(L.runs - 1), (F / 32) * 4), dim3(DI_THREADS), 0, stream, slots, steps,
                            L.runs, L.xtiles, m, F, dY);
         MIREC_LAUNCH_CHECK();
