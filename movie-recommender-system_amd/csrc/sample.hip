@@ -221,7 +221,8 @@ __device__ __forceinline__ float sm_logprob(float score, double best, double ste
 // cuts and the draws.  Otherwise every item is compared with every other.  The lanes of a row take `rows_each` rows, one after
 // the other, and keep their draws, one each, until all lanes have one: logarithms and stores are then one for all.
 // What bounds it is the number of vector instructions per row; most of them are for the row, not for its items, so that two
-// rows of up to 128 items share them.
+// rows of up to 128 items share them.  Measured: 262144 lists of 100 under top_p and min_p 110 us (2 TB/s of scores and ids;
+// the bytes alone 53 us), of 50 76 us, one list 3.4 us.
 template <int DT, int E, int R>
 __global__ __launch_bounds__(256) void sample_short_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int m, int64_t stride, const int32_t* __restrict__ ids,
@@ -525,8 +526,9 @@ struct Chunk {
 // item -- and by ranking the items of the bin that the border falls into against each other.
 //
 // What bounds it: the instructions per score (about 25 for a weight, 10 for a place in a histogram), then the chain of
-// barriers of a row, not the bytes: hence two rows of 512 threads side by side on a compute unit, or one of 1024 where
-// there are fewer rows than compute units.
+// barriers of a row, not the bytes (read once, 1024 rows of 27000 would take 27 us): hence rows of 512 threads side by side
+// on a compute unit, or one of 1024 where there are no more rows than compute units.  Measured: 1024 x 27000 under top_p
+// 115 us, 512 x 200000 bf16 uncut, 8 draws, 151 us (1.3 TB/s of scores), one row of 27000 under top_k 18 us.
 // Registers: few rows, of 1024 threads, run one or two workgroups to a compute unit and are faster with more registers
 // (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6); 512 threads are faster with 6 (mixed
 // requests 384 -> 350 us).
