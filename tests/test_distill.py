@@ -237,6 +237,18 @@ def test_the_same_item_twice_adds_up(dev, tail):
 
 
 @gpu
+@pytest.mark.parametrize("k", [1, 64, 65, 192, 256])
+@pytest.mark.parametrize("n", [40, 2100])
+@pytest.mark.parametrize("twice", [False, True])
+def test_lists_of_every_length(dev, k, n, twice):
+    """The list kernel of few and of many rows; in every third row some items are listed again."""
+    X, Y, ids, scores, _, grad = problem(71, n, 300, 32, k, dev, ragged=True)
+    if twice:
+        ids[::3, k // 2:] = torch.where(ids[::3, k // 2:] >= 0, ids[::3, :k - k // 2], -1)
+    compare(X, Y, ids, scores, 1.0, None, grad, E.distill(X, Y, ids, scores, grad=grad))
+
+
+@gpu
 def test_a_list_of_the_whole_catalogue(dev):
     """With every item listed the class of the others is empty on both sides."""
     X, Y, ids, scores, tlse, grad = problem(8, 20, 100, 32, 100, dev)

@@ -337,6 +337,55 @@ def test_ranked_lists(dev, k, replacement):
 
 
 @gpu
+@pytest.mark.parametrize("k", [300, 1000, 9000])
+@pytest.mark.parametrize("replacement", [True, False])
+def test_long_and_unordered_lists(dev, k, replacement):
+    """Lists longer than the short rows' kernels take, in any order, with empty slots in between."""
+    g = torch.Generator().manual_seed(k)
+    s = torch.randn(6, k, generator=g)
+    ids = torch.stack([torch.randperm(20000, generator=g)[:k] for _ in range(6)]).to(torch.int32)
+    ids[torch.rand(6, k, generator=g) < 0.3] = -1
+    ids[5] = -1
+    u = torch.rand(6, 5, generator=g)
+    s, ids, u = s.to(dev), ids.to(dev), u.to(dev)
+    for cut in (dict(), dict(top_k=5), dict(top_p=0.7, min_p=0.001), dict(top_k=200)):
+        got, lp = E.sample_scores(s, u, ids=ids, replacement=replacement, **cut)
+        check(s, u, got, lp, ids=ids, replacement=replacement, **cut)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 32, 33, 64, 65, 100, 128, 129, 256])
+@pytest.mark.parametrize("lists", [False, True])
+def test_rows_that_share_a_wavefront(dev, m, lists):
+    """Many short rows: each draws what it draws alone, whatever shares its wavefront (parameters and filters per row, rows
+    that are in order beside rows that are not)."""
+    n = 29993
+    g = torch.Generator().manual_seed(m)
+    s = torch.randn(n, m, generator=g)
+    s = torch.where(torch.rand(n, 1, generator=g) < 0.6, torch.sort(s, dim=1, descending=True).values, s).to(dev)
+    u = torch.rand(n, 3, generator=g).to(dev)
+    T = (0.2 + torch.rand(n, generator=g)).to(dev)
+    k = torch.randint(0, 80, (n,), generator=g, dtype=torch.int32).to(dev)
+    p = (torch.rand(n, generator=g) * 1.3).to(dev)
+    rows, csr = filter_rows(m, n, m, 0.3, dev)
+    ids = (torch.randint(0, 1 << 20, (n, m), generator=g, dtype=torch.int32) * 1024 + torch.arange(m, dtype=torch.int32)).to(dev)
+    ids[::7, ::3] = -1
+    for replacement in (True, False):
+        kw = dict(temperature=T, top_k=k, top_p=p, replacement=replacement)
+        got, lp = E.sample_scores(s, u, **kw, **(dict(ids=ids) if lists else dict(mask=csr)))
+        for r in (0, 1, 2, 3, 777, 14976, 14977, n - 2, n - 1):
+            one = slice(r, r + 1)
+            extra = dict(ids=ids[one]) if lists else dict(mask=E.DeviceCSR(csr.indptr[r:r + 2], csr.indices, csr.data, (1, m)))
+            alone = E.sample_scores(s[one], u[one], temperature=T[one], top_k=k[one], top_p=p[one], replacement=replacement, **extra)
+            assert torch.equal(got[one], alone[0]) and torch.equal(lp[one], alone[1]), r
+        pick = torch.arange(0, n, 997)
+        at = pick.to(dev)
+        pc = p[at].cpu().clamp(max=1.0)
+        check(s[at], u[at], got[at], lp[at], ids=ids[at] if lists else None, liked=None if lists else [rows[r] for r in pick.tolist()],
+              T=T[at].cpu(), top_k=k[at].cpu(), top_p=pc, replacement=replacement)
+
+
+@gpu
 @pytest.mark.parametrize("m", [5, 300, 3001, 30000])
 def test_without_replacement_no_item_twice(dev, m):
     n, draws = 5, 12
