@@ -489,13 +489,8 @@ struct Chunk {
     // Whether a score is not below the largest finite magnitude: it may be one that is excluded, or infinite.
     __device__ __forceinline__ bool unsettled() const {
         if constexpr (DT == MIREC_F32) {
-            uint32_t most = word[0] & 0x7fffffffu;
-#pragma unroll
-            for (int i = 1; i < 4; ++i) {
-                const uint32_t a = word[i] & 0x7fffffffu;
-                most = a > most ? a : most;
-            }
-            return most >= 0x7f7fffffu;
+            // (a sum of magnitudes is not below any of them, and a NaN where one is; that it can be too large costs time only)
+            return !((fabsf(raw(0)) + fabsf(raw(1))) + (fabsf(raw(2)) + fabsf(raw(3))) < FLT_MAX);
         } else {
             sm_u16x2 most = __builtin_bit_cast(sm_u16x2, word[0] & 0x7fff7fffu);
 #pragma unroll
@@ -532,7 +527,7 @@ struct Chunk {
 // Registers: few rows, of 1024 threads, run one or two workgroups to a compute unit and are faster with more registers
 // (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6); 512 threads are faster with 6 (mixed
 // requests 384 -> 350 us).
-template <int DT, int NT>
+template <int DT, int NT, bool LISTS>
 __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,
     const int32_t* __restrict__ ids, int64_t ids_stride, const int64_t* __restrict__ mask_indptr,
@@ -555,13 +550,14 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
     const int64_t row_chunks = (m + WAVE_CHUNK - 1) / WAVE_CHUNK;
     const int S = (int)((row_chunks + SM_BINS - 1) / SM_BINS);
     const int pieces = (int)((row_chunks + S - 1) / S);   // at most SM_BINS
+    const int items = (int)m, last_whole = items - WAVE_CHUNK;   // (items <= 2^30; where the last whole chunk may begin)
 
     for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
         const typename ScoreType<DT>::raw* s = scores + row * stride;
-        const int32_t* id = ids ? ids + row * ids_stride : nullptr;
+        const int32_t* id = LISTS ? ids + row * ids_stride : nullptr;
         __syncthreads();   // the row before is done with the shared arrays
         if (mask_indptr) {
-            for (int64_t w = tid; w < (m + 31) / 32; w += NT) liked[w] = 0;
+            for (int w = tid; w < pieces * S * (WAVE_CHUNK / 32); w += NT) liked[w] = 0;
             __syncthreads();
             for (int64_t e = mask_indptr[row] + tid; e < mask_indptr[row + 1]; e += NT) {
                 const int64_t it = mask_indices[e];
@@ -571,43 +567,45 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
         }
         // a lane's first item of chunk `sub` of piece p
         auto first_item = [&](int p, int sub) -> int32_t { return (p * S + sub) * WAVE_CHUNK + lane * V; };
-        // its 16 bytes (minus infinity behind the row's end), and what is excluded set to minus infinity
+        // its 16 bytes (minus infinity behind the row's end); whether a chunk ends inside the row is asked once for all lanes
         auto load = [&](int p, int sub) -> C {
-            const int32_t i = first_item(p, sub);
+            const int begin = (p * S + sub) * WAVE_CHUNK;
             C q;
-#pragma unroll
-            for (int v = 0; v < 4; ++v) q.word[v] = DT == MIREC_F32 ? 0xff800000u : DT == MIREC_BF16 ? 0xff80ff80u : 0xfc00fc00u;
-            if (i + V <= m) {
-                const sm_words x = *reinterpret_cast<const sm_words*>(s + i);
+            if (begin <= last_whole) {
+                const sm_words x = *reinterpret_cast<const sm_words*>(s + begin + lane * V);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) q.word[v] = x[v];
-            } else if (i < m) {
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (i + v < m) {
-                        if constexpr (DT == MIREC_F32) q.word[v] = __float_as_uint(s[i + v]);
-                        else {
-                            const uint32_t raw = __builtin_bit_cast(uint16_t, s[i + v]);
-                            q.word[v >> 1] = v & 1 ? (q.word[v >> 1] & 0xffffu) | (raw << 16) : (q.word[v >> 1] & 0xffff0000u) | raw;
-                        }
-                    }
+                return q;
             }
+            const int i = begin + lane * V;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) q.word[v] = DT == MIREC_F32 ? 0xff800000u : DT == MIREC_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (i + v < items) {
+                    if constexpr (DT == MIREC_F32) q.word[v] = __float_as_uint(s[i + v]);
+                    else {
+                        const uint32_t raw = __builtin_bit_cast(uint16_t, s[i + v]);
+                        q.word[v >> 1] = v & 1 ? (q.word[v >> 1] & 0xffffu) | (raw << 16) : (q.word[v >> 1] & 0xffff0000u) | raw;
+                    }
+                }
             return q;
         };
+        // what is excluded set to minus infinity
         auto filter = [&](C& q, int32_t i) {
             if (__any(q.unsettled())) q.settle();
             if (mask_indptr) {
-                const uint32_t out = i < m ? (liked[i >> 5] >> (i & 31)) & ((1u << V) - 1) : 0u;
+                const uint32_t out = (liked[i >> 5] >> (i & 31)) & ((1u << V) - 1);
                 if (__any(out != 0)) {
 #pragma unroll
                     for (int v = 0; v < V; ++v)
                         if ((out >> v) & 1u) q.exclude(v);
                 }
             }
-            if (id) {
+            if constexpr (LISTS) {
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (i + v < m && id[i + v] < 0) q.exclude(v);
+                    if (i + v < items && id[i + v] < 0) q.exclude(v);
             }
         };
         // f(chunk, the lane's first item, its piece, number within the piece) for every chunk of this wavefront, in order,
@@ -835,7 +833,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
                     }
                     if (out_w != 0) {
                         const int32_t item = (int32_t)(0xffffffffu - (uint32_t)out_K);
-                        out_ids[row * draws + d] = id ? id[item] : item;
+                        out_ids[row * draws + d] = LISTS ? id[item] : item;
                         out_logprob[row * draws + d] = sm_logprob(sm_unorder((uint32_t)(out_K >> 32)), best, cuts.step, total, bits);
                     }
                     if (!replacement) {
@@ -1140,7 +1138,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
                     float f = 0.f;
 #pragma unroll
                     for (int v = 0; v < V; ++v) f = at_v == v ? q.score(v) : f;
-                    out_ids[row * draws + d] = id ? id[item] : item;
+                    out_ids[row * draws + d] = LISTS ? id[item] : item;
                     out_logprob[row * draws + d] = sm_logprob(f, best, cuts.step, total, bits);
                     if (!replacement) gone[taken] = item;
                 }
@@ -1181,7 +1179,7 @@ static int launch_short(const typename ScoreType<DT>::raw* scores, int64_t n, in
     return MIREC_OK;
 }
 
-template <int DT, int NT>
+template <int DT, int NT, bool LISTS>
 static int launch_long(const typename ScoreType<DT>::raw* scores, int64_t n, int64_t m, int64_t stride, const int32_t* ids,
                        int64_t ids_stride, const int64_t* mask_indptr, const int32_t* mask_indices, const float* uniforms,
                        int draws, int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
@@ -1191,12 +1189,15 @@ static int launch_long(const typename ScoreType<DT>::raw* scores, int64_t n, int
     bool* done = once.slot();
     MIREC_REQUIRE(done, MIREC_E_HIP, "mirec_sample: cannot read the current device");
     if (!*done) {
-        MIREC_HIP(hipFuncSetAttribute((const void*)sample_long_kernel<DT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        MIREC_HIP(hipFuncSetAttribute((const void*)sample_long_kernel<DT, NT, LISTS>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)(SM_MAX_MASKED_ITEMS / 8)));
         *done = true;
     }
-    const size_t lds = mask_indptr ? (size_t)((m + 31) / 32) * 4 : 0;
-    hipLaunchKernelGGL((sample_long_kernel<DT, NT>), dim3((unsigned)(n < 262144 ? n : 262144)), dim3(NT), lds, stream, scores,
+    // (a bit for every item of whole pieces; at SM_MAX_MASKED_ITEMS these end with the row)
+    constexpr int64_t CHUNK_ITEMS = 64 * Chunk<DT>::V;
+    const int64_t chunks = (m + CHUNK_ITEMS - 1) / CHUNK_ITEMS, per = (chunks + SM_BINS - 1) / SM_BINS;
+    const size_t lds = mask_indptr ? (size_t)((chunks + per - 1) / per * per * (CHUNK_ITEMS / 8)) : 0;
+    hipLaunchKernelGGL((sample_long_kernel<DT, NT, LISTS>), dim3((unsigned)(n < 262144 ? n : 262144)), dim3(NT), lds, stream, scores,
                        n, m, stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids,
                        out_logprob);
     MIREC_LAUNCH_CHECK();
@@ -1217,9 +1218,10 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
     if (ids && m <= 128) return launch_short<DT, 4, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= 128) return launch_short<DT, 2, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= SM_SHORT) return launch_short<DT, 4, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
-    if (n <= SM_FEW_ROWS && m > 8192) return launch_long<DT, 1024>(scores, n, m, MIREC_SAMPLE_ARGS);
-    if (m > 8192) return launch_long<DT, 512>(scores, n, m, MIREC_SAMPLE_ARGS);
-    return launch_long<DT, 256>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (ids) return m > 8192 ? launch_long<DT, 512, true>(scores, n, m, MIREC_SAMPLE_ARGS) : launch_long<DT, 256, true>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (n <= SM_FEW_ROWS && m > 8192) return launch_long<DT, 1024, false>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (m > 8192) return launch_long<DT, 512, false>(scores, n, m, MIREC_SAMPLE_ARGS);
+    return launch_long<DT, 256, false>(scores, n, m, MIREC_SAMPLE_ARGS);
 #undef MIREC_SAMPLE_ARGS
 }
 
