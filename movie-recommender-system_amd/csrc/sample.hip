@@ -118,28 +118,30 @@ __device__ __forceinline__ double sm_log2(double x) {
     return __builtin_fma(r * (1.0 - 0.5 * r), 1.4426950408889634, l);
 }
 
-// ---- 64-bit sums over a wavefront, by data-parallel moves between lanes (no LDS)
+// ---- sums and maxima over a wavefront, by data-parallel moves between lanes (no LDS)
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t sm_moved(uint64_t v) {   // 0 where no lane is moved from
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
-    return ((uint64_t)hi << 32) | lo;
-}
+// One step: v of another lane is added where the move reaches from a lane that is there (elsewhere the instruction does
+// nothing).  Written out because the compiler moves and adds separately: seven instructions a step instead of two, a third
+// of what a piece of a long row costs.  A data-parallel read of a register needs two wait states behind its write.
+#define SM_ADD_STEP(MOVE)                                       \
+    "s_nop 0\n"                                                 \
+    "v_add_co_u32_dpp %0, vcc, %0, %0 " MOVE " bank_mask:0xf\n"  \
+    "v_addc_co_u32_dpp %1, vcc, %1, %1, vcc " MOVE " bank_mask:0xf\n"
 
 __device__ __forceinline__ uint64_t sm_half_scan(uint64_t v) {   // inclusive, over lanes 0 .. 31 and 32 .. 63
-    v += sm_moved<0x111, 0xf>(v);   // shifted by 1, 2, 4, 8 within rows of 16 lanes
-    v += sm_moved<0x112, 0xf>(v);
-    v += sm_moved<0x114, 0xf>(v);
-    v += sm_moved<0x118, 0xf>(v);
-    v += sm_moved<0x142, 0xa>(v);   // lane 15 of a row to the next row: rows 1 and 3
-    return v;
+    uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    asm("s_nop 0\n"                                              // shifted by 1, 2, 4, 8 within rows of 16 lanes,
+        SM_ADD_STEP("row_shr:1 row_mask:0xf") SM_ADD_STEP("row_shr:2 row_mask:0xf") SM_ADD_STEP("row_shr:4 row_mask:0xf")
+        SM_ADD_STEP("row_shr:8 row_mask:0xf") SM_ADD_STEP("row_bcast:15 row_mask:0xa")   // lane 15 of a row to rows 1 and 3
+        "s_nop 1" : "+v"(lo), "+v"(hi) : : "vcc");
+    return ((uint64_t)hi << 32) | lo;
 }
 
 __device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
     v = sm_half_scan(v);
-    v += sm_moved<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
-    return v;
+    uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    asm("s_nop 0\n" SM_ADD_STEP("row_bcast:31 row_mask:0xc") "s_nop 1" : "+v"(lo), "+v"(hi) : : "vcc");   // lane 31 to rows 2 and 3
+    return ((uint64_t)hi << 32) | lo;
 }
 
 __device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {
@@ -149,21 +151,18 @@ __device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {
 
 __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_lane(sm_wave_scan(v), 63); }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float sm_max_moved(float v) {
-    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(v), CTRL, ROWS, 0xf, false)));
-}
+#define SM_MAX_STEP(MOVE) "s_nop 1\nv_max_f32_dpp %0, %0, %0 " MOVE " bank_mask:0xf\n"
 
 __device__ __forceinline__ float sm_half_max(float v) {   // in lanes 31 and 63
-    v = sm_max_moved<0x111, 0xf>(v);
-    v = sm_max_moved<0x112, 0xf>(v);
-    v = sm_max_moved<0x114, 0xf>(v);
-    v = sm_max_moved<0x118, 0xf>(v);
-    return sm_max_moved<0x142, 0xa>(v);
+    asm(SM_MAX_STEP("row_shr:1 row_mask:0xf") SM_MAX_STEP("row_shr:2 row_mask:0xf") SM_MAX_STEP("row_shr:4 row_mask:0xf")
+        SM_MAX_STEP("row_shr:8 row_mask:0xf") SM_MAX_STEP("row_bcast:15 row_mask:0xa") "s_nop 1" : "+v"(v));
+    return v;
 }
 
 __device__ __forceinline__ float sm_wave_max(float v) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sm_max_moved<0x143, 0xc>(sm_half_max(v))), 63));
+    v = sm_half_max(v);
+    asm(SM_MAX_STEP("row_bcast:31 row_mask:0xc") "s_nop 1" : "+v"(v));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // Where a number of [0, 1) falls in a total: floor(u * total), exactly (u is a 24-bit integer over a power of two); 0 for
@@ -221,7 +220,7 @@ __device__ __forceinline__ float sm_logprob(float score, double best, double ste
 // cuts and the draws.  Otherwise every item is compared with every other.  The lanes of a row take `rows_each` rows, one after
 // the other, and keep their draws, one each, until all lanes have one: logarithms and stores are then one for all.
 // What bounds it is the number of vector instructions per row; most of them are for the row, not for its items, so that two
-// rows of up to 128 items share them.  Measured: 262144 lists of 100 under top_p and min_p 110 us (2 TB/s of scores and ids;
+// rows of up to 128 items share them.  Measured: 262144 lists of 100 under top_p and min_p 107 us (2 TB/s of scores and ids;
 // the bytes alone 53 us), of 50 76 us, one list 3.4 us.
 template <int DT, int E, int R>
 __global__ __launch_bounds__(256) void sample_short_kernel(
@@ -520,10 +519,11 @@ struct Chunk {
 // SM_LIST items, by equal ranges of K = (monotone image of the score, complemented index), which is larger for a better
 // item -- and by ranking the items of the bin that the border falls into against each other.
 //
-// What bounds it: the instructions per score (about 25 for a weight, 10 for a place in a histogram), then the chain of
-// barriers of a row, not the bytes (read once, 1024 rows of 27000 would take 27 us): hence rows of 512 threads side by side
-// on a compute unit, or one of 1024 where there are no more rows than compute units.  Measured: 1024 x 27000 under top_p
-// 115 us, 512 x 200000 bf16 uncut, 8 draws, 151 us (1.3 TB/s of scores), one row of 27000 under top_k 18 us.
+// What bounds it: where the rows in flight exceed L2 each pass reads them at the rate of memory (two passes over 4096 x 27000
+// in 186 us, 4.75 TB/s), and a weight is 21 instructions (nine of them its polynomial); under top_p both take about 280 of
+// the 340 us of those rows.  Hence as few passes as possible, and rows of 512 threads side by side on a compute unit, or one
+// of 1024 where there are no more rows than compute units.  Measured: 1024 x 27000 under top_p 111 us, 512 x 200000 bf16 uncut,
+// 8 draws, 149 us, one row of 27000 under top_k 17 us.
 // Registers: few rows, of 1024 threads, run one or two workgroups to a compute unit and are faster with more registers
 // (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6); 512 threads are faster with 6 (mixed
 // requests 384 -> 350 us).
