@@ -42,11 +42,12 @@ constexpr int DI_NW = 8;                          // wavefronts of a workgroup o
 constexpr int DI_OWN = 32 * DI_NW;                // rows it owns
 constexpr int DI_PARTS = 256;                     // partial maxima of a matrix
 constexpr int DI_MAX_THREADS = 1024;              // of the workgroups that find them
+constexpr int DI_RANGES = 256;                    // most ranges that the items are cut into in the forward pass
 constexpr int DI_PREPARE_THREADS = 1024;
 constexpr int DI_WEIGH_BLOCKS = 64;
 constexpr int DI_BINS = 4096;                     // item tiles that di_group counts at a time
 constexpr int DI_CUS = 256;                       // workgroups that run at once
-constexpr int DI_FEW_TILES = 4;                   // of rows: the backward pass does not cut its blocks of items
+constexpr int DI_JOIN_STEPS = 4;                  // of the backward pass: what joining cut blocks takes
 constexpr float DI_HEADROOM = 7.f;                // log2 of a probability's scale when its row's reference is current
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -83,7 +84,7 @@ struct DistillWorkspace {
 static int distill_splits(int64_t blocks, int64_t tiles) {
     int best = 1;
     double cost = 1e300;
-    for (int64_t s = 1; s <= 64 && s <= tiles; ++s) {
+    for (int64_t s = 1; s <= DI_RANGES && s <= tiles; ++s) {
         const double rounds = (double)((blocks * s + DI_CUS - 1) / DI_CUS);
         const double c = rounds * ((double)((tiles + s - 1) / s) + 4.0) + (s > 1 ? 0.05 * (double)(blocks * s) : 0.0);
         if (c < cost) {
@@ -106,9 +107,11 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.ytiles = (m + 31) / 32;
     const int64_t xblocks = (n + DI_OWN - 1) / DI_OWN, yblocks = (m + DI_OWN - 1) / DI_OWN;
     w.splits_x = distill_splits(xblocks, w.ytiles);
-    // (few row tiles: whole blocks of items, nothing to join.  128 rows of 27000 items at 128 columns: 84 us with the blocks
-    // cut, 71 whole; 256 rows of 7207 items at 96 columns: 56 and 64)
-    w.runs = w.xtiles <= DI_FEW_TILES && yblocks < DI_CUS ? yblocks : yblocks * w.xtiles < DI_CUS ? yblocks * w.xtiles : DI_CUS;
+    // Cut the blocks of items where that saves more steps than the join of their parts costs.  (256 rows of 7207 items at 96
+    // columns, 8 row tiles and 29 blocks: 56 us cut, 64 whole; 128 of 27000 at 128 columns, 4 and 106: 84 and 71; 512 of 60000, 16
+    // and 235: 170 and 154.)
+    const int64_t steps = yblocks * w.xtiles, whole = (yblocks + DI_CUS - 1) / DI_CUS * w.xtiles;
+    w.runs = whole <= (steps + DI_CUS - 1) / DI_CUS + DI_JOIN_STEPS ? yblocks : steps < DI_CUS ? steps : DI_CUS;
     w.max_off = take(3 * DI_PARTS * 4);       // partial maxima of |X|, |Y|, |grad|
     w.ref_off = take((size_t)n * 4);          // M_b: log2 reference of a row's mass
     w.mass_off = take((size_t)n * 4);         // sum_j 2^(z_bj log2 e - M_b)
@@ -126,7 +129,7 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.yimg_off = take((size_t)w.ytiles * 256 * f);
     w.pref_off = take((size_t)w.splits_x * n * 4);
     w.pmass_off = take((size_t)w.splits_x * n * 4);
-    const size_t px = (size_t)w.splits_x * n * f * 4, py = (size_t)w.runs * 2 * DI_OWN * f * 4;
+    const size_t px = (size_t)w.splits_x * n * f * 4, py = w.runs == yblocks ? 0 : (size_t)w.runs * 2 * DI_OWN * f * 4;
     w.part_off = take(px > py ? px : py);     // partial means, later parts of dY
     w.bytes = at;
     return w;
@@ -345,8 +348,8 @@ __device__ __forceinline__ void di_accumulate(const char* tile, const f32x16& w,
 
 // Workgroup index -> (owned block, range of the streamed side): the workgroups of an XCD (every eighth index) take
 // neighbouring work, range by range, so that what streams through an XCD's L2 is shared by its compute units.
-__device__ __forceinline__ int64_t di_work_index() {
-    const int64_t total = gridDim.x, per = total / 8, i = blockIdx.x;
+__device__ __forceinline__ uint32_t di_work_index() {
+    const uint32_t total = gridDim.x, per = total / 8, i = blockIdx.x;
     return i < per * 8 ? (i % 8) * per + i / 8 : i;
 }
 
@@ -361,8 +364,8 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
     constexpr int FETCH = GRAD ? D::BYTES : 2 * D::PLANE, STAGES = D::STAGES_FORWARD;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int64_t work = di_work_index();
-    const int64_t range = work / blocks, block = work % blocks;
+    const uint32_t work = di_work_index();
+    const int64_t range = work / (uint32_t)blocks, block = work % (uint32_t)blocks;
     const int64_t t0 = range * tiles_per_range;
     const int64_t t1 = t0 + tiles_per_range < ytiles ? t0 + tiles_per_range : ytiles;
     const int64_t own0 = block * DI_OWN + wave * 32;
@@ -432,7 +435,10 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
 }
 
 // First of the steps that workgroup w of `runs` takes.
-__host__ __device__ __forceinline__ int64_t di_run_begin(int64_t w, int64_t steps, int64_t runs) { return w * steps / runs; }
+__device__ __forceinline__ int64_t di_quotient(int64_t a, int64_t b) {   // (a 64-bit division takes half a microsecond)
+    return a < ((int64_t)1 << 32) ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+__device__ __forceinline__ int64_t di_run_begin(int64_t w, int64_t steps, int64_t runs) { return di_quotient(w * steps, runs); }
 
 // The gradients of the items: 32 of them per wavefront, 256 per workgroup, against all tiles of rows.  The steps (block of
 // items, row tile) are numbered block by block and cut into equal runs, one per workgroup, whatever the number of
@@ -501,7 +507,8 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
     float* fix = reinterpret_cast<float*>(lds + STAGES * (D::BYTES + 512)) + wave * (64 * 20 + 64);
     uint32_t* fix_bits = reinterpret_cast<uint32_t*>(fix + 64 * 20);
     fix_bits[lane] = 0;
-    Step now = {(int)(run0 / xtiles), (int)(run0 % xtiles)};
+    const int block0 = (int)di_quotient(run0, xtiles);
+    Step now = {block0, (int)(run0 - block0 * xtiles)};
     fetch_extent(now);
     Step ahead = now;   // the next tile to copy
 #pragma unroll
@@ -591,27 +598,27 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
 // run; it takes the block that its run begins inside of, if no run before it does.
 __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* __restrict__ slots, int64_t steps, int64_t runs,
                                                                   int64_t xtiles, int64_t m, int f, float* __restrict__ dY) {
-    const int64_t begin = di_run_begin(blockIdx.x + 1, steps, runs), block = begin / xtiles, s0 = block * xtiles, s1 = s0 + xtiles;
+    const int64_t begin = di_run_begin(blockIdx.x + 1, steps, runs), block = di_quotient(begin, xtiles), s0 = block * xtiles, s1 = s0 + xtiles;
     const int64_t w0 = blockIdx.x, before = di_run_begin(w0, steps, runs);   // the run that ends inside the block
     if (begin == s0 || before > s0) return;
     // one past the last run with a part of the block: the first whose steps begin behind it
-    int64_t w1 = (s1 * runs + steps - 1) / steps;
+    int64_t w1 = di_quotient(s1 * runs + steps - 1, steps);
     w1 = w1 < runs ? w1 : runs;
     const int first_slot = before == s0 ? 0 : 1;
     const int64_t rows = m - block * DI_OWN < DI_OWN ? m - block * DI_OWN : DI_OWN;
-    for (int64_t e = ((int64_t)blockIdx.y * DI_THREADS + threadIdx.x) * 4; e < rows * f; e += (int64_t)gridDim.y * DI_THREADS * 4) {
-        f32x4 v = *reinterpret_cast<const f32x4*>(slots + (2 * w0 + first_slot) * DI_OWN * f + e);
-        for (int64_t w = w0 + 1; w < w1; w += 4) {   // four parts asked for at once
-            f32x4 part[4];
+    const int64_t e = ((int64_t)blockIdx.y * DI_THREADS + threadIdx.x) * 4;   // (the grid covers a block)
+    if (e >= rows * f) return;
+    f32x4 v = *reinterpret_cast<const f32x4*>(slots + (2 * w0 + first_slot) * DI_OWN * f + e);
+    for (int64_t w = w0 + 1; w < w1; w += 8) {   // eight parts asked for at once
+        f32x4 part[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (w + u < w1) part[u] = *reinterpret_cast<const f32x4*>(slots + 2 * (w + u) * DI_OWN * f + e);
+        for (int u = 0; u < 8; ++u)
+            if (w + u < w1) part[u] = *reinterpret_cast<const f32x4*>(slots + 2 * (w + u) * DI_OWN * f + e);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (w + u < w1) v += part[u];
-        }
-        *reinterpret_cast<f32x4*>(dY + block * DI_OWN * f + e) = v;
+        for (int u = 0; u < 8; ++u)
+            if (w + u < w1) v += part[u];
     }
+    *reinterpret_cast<f32x4*>(dY + block * DI_OWN * f + e) = v;
 }
 
 // ------------------------------------------------------------------------------------------------------- the lists
@@ -646,7 +653,7 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
     int slots = 2 * kp;                                             // of the table: a power of two
     while (slots & (slots - 1)) slots &= slots - 1;
     __shared__ float red[NWV][F];
-    __shared__ float range_w[64];
+    __shared__ float range_w[DI_RANGES];
     __shared__ float row_ref, row_mass;
     __shared__ double partd[2][NWV];
     __shared__ int parti[NWV];
@@ -670,15 +677,25 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) x[i] = *reinterpret_cast<const f32x2*>(X + b * F + 2 * (sub + 16 * i));
         __syncthreads();   // the row before is done with the shared arrays
-        if (wave == 0) {   // at most 64 ranges: one lane each
-            const float r = lane < ranges ? pref[lane * n + b] : -INFINITY;
-            const float pm = lane < ranges ? pmass[lane * n + b] : 0.f;
-            float top = r;
+        if (wave == 0) {   // the ranges' references and masses, some of them to a lane
+            float r[DI_RANGES / 64], pm[DI_RANGES / 64], top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < DI_RANGES / 64; ++i) {
+                const int at = lane + 64 * i;
+                r[i] = at < ranges ? pref[at * n + b] : -INFINITY;
+                pm[i] = at < ranges ? pmass[at * n + b] : 0.f;
+                top = fmaxf(top, r[i]);
+            }
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-            const float w = lane < ranges ? __builtin_amdgcn_exp2f(r - top) : 0.f;
-            const float sum = wave_sum(pm * w);
-            range_w[lane] = ldexpf(w / sum, -sy);
+#pragma unroll
+            for (int i = 0; i < DI_RANGES / 64; ++i) {
+                r[i] = lane + 64 * i < ranges ? __builtin_amdgcn_exp2f(r[i] - top) : 0.f;
+                sum = __builtin_fmaf(pm[i], r[i], sum);
+            }
+            sum = wave_sum(sum);
+#pragma unroll
+            for (int i = 0; i < DI_RANGES / 64; ++i) range_w[lane + 64 * i] = ldexpf(r[i] / sum, -sy);
             if (lane == 0) {
                 row_ref = top;
                 row_mass = ldexpf(sum, -(int)DI_HEADROOM);
@@ -953,15 +970,31 @@ __device__ __forceinline__ void di_group(int64_t tile, const int32_t* __restrict
     const int64_t row0 = tile * 32;
     const int rows = (int)(n - row0 < 32 ? n - row0 : 32);
     uint16_t* tile_start = start + tile * (ytiles + 1);
+    // this thread's entries: item tile (-1: not an entry), place in the 32 x 32 block, value
+    constexpr int HELD = 32 * DI_LIST / DI_PREPARE_THREADS;
+    int32_t in[HELD], spot[HELD];
+    float v[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int e = tid + i * DI_PREPARE_THREADS;
+        in[i] = -1;
+        if (e < rows * k) {
+            const int r = e / k;
+            const int32_t id = list_id[row0 * k + e];
+            v[i] = list_val[row0 * k + e];
+            spot[i] = r * 32 + (id & 31);
+            in[i] = e - r * k < count[row0 + r] ? id >> 5 : -1;
+        }
+    }
     int base = 0;
     for (int64_t t0 = 0; t0 < ytiles; t0 += DI_BINS) {
         for (int i = tid; i < DI_BINS; i += DI_PREPARE_THREADS) bins[i] = 0;
         __syncthreads();
-        for (int e = tid; e < rows * k; e += DI_PREPARE_THREADS)
-            if (e % k < count[row0 + e / k]) {
-                const int64_t t = list_id[row0 * k + e] / 32 - t0;
-                if (t >= 0 && t < DI_BINS) atomicAdd(&bins[t], 1);
-            }
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int64_t t = in[i] - t0;
+            if (in[i] >= 0 && t >= 0 && t < DI_BINS) atomicAdd(&bins[t], 1);
+        }
         __syncthreads();
         int sum = 0;
         for (int i = 0; i < PER; ++i) sum += bins[tid * PER + i];
@@ -985,16 +1018,15 @@ __device__ __forceinline__ void di_group(int64_t tile, const int32_t* __restrict
             at += c;
         }
         __syncthreads();
-        for (int e = tid; e < rows * k; e += DI_PREPARE_THREADS)
-            if (e % k < count[row0 + e / k]) {
-                const int32_t id = list_id[row0 * k + e];
-                const int64_t t = id / 32 - t0;
-                if (t >= 0 && t < DI_BINS) {
-                    const int64_t to = row0 * k + atomicAdd(&bins[t], 1);
-                    place[to] = (uint16_t)(e / k * 32 + (id & 31));
-                    val[to] = list_val[row0 * k + e];
-                }
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int64_t t = in[i] - t0;
+            if (in[i] >= 0 && t >= 0 && t < DI_BINS) {
+                const int64_t to = row0 * k + atomicAdd(&bins[t], 1);
+                place[to] = (uint16_t)spot[i];
+                val[to] = v[i];
             }
+        }
         __syncthreads();
     }
     if (tid == 0) tile_start[ytiles] = (uint16_t)base;
@@ -1138,7 +1170,7 @@ static int launch_backward(const DistillWorkspace& L, char* w, int64_t n, int64_
                        (const uint16_t*)(w + L.place_off), (const float*)(w + L.gval_off), k, dY, slots);
     MIREC_LAUNCH_CHECK();
     if (blocks % L.runs != 0) {   // (else every run is of whole blocks)
-        hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)(L.runs - 1), (F / 32) * 4), dim3(DI_THREADS), 0, stream, slots, steps,
+        hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)(L.runs - 1), DI_OWN * F / (4 * DI_THREADS)), dim3(DI_THREADS), 0, stream, slots, steps,
                            L.runs, L.xtiles, m, F, dY);
         MIREC_LAUNCH_CHECK();
     }
