@@ -80,13 +80,13 @@ struct DistillWorkspace {
 };
 
 // Into how many ranges to cut the streamed tiles: the fewest rounds of 256 workgroups, each paying for its start (four
-// tiles' time) and for the partial results (written and read once more: 0.05 of a tile's time per owned block).
+// tiles' time) and for the partial results (written and read once more: 0.025 of a tile's time per owned block).
 static int distill_splits(int64_t blocks, int64_t tiles) {
     int best = 1;
     double cost = 1e300;
     for (int64_t s = 1; s <= DI_RANGES && s <= tiles; ++s) {
         const double rounds = (double)((blocks * s + DI_CUS - 1) / DI_CUS);
-        const double c = rounds * ((double)((tiles + s - 1) / s) + 4.0) + (s > 1 ? 0.05 * (double)(blocks * s) : 0.0);
+        const double c = rounds * ((double)((tiles + s - 1) / s) + 4.0) + (s > 1 ? 0.025 * (double)(blocks * s) : 0.0);
         if (c < cost) {
             cost = c;
             best = (int)s;
