@@ -36,7 +36,7 @@
 namespace mirec {
 
 constexpr int DI_LIST = MIREC_DISTILL_MAX_LIST;   // longest list
-constexpr int64_t DI_MANY_ROWS = 2048;            // from here on a wavefront per row in distill_list_kernel
+constexpr int64_t DI_MANY_ROWS = 1024;            // beyond: a wavefront per row in distill_list_kernel
 constexpr int DI_THREADS = 256;
 constexpr int DI_NW = 8;                          // wavefronts of a workgroup of the two passes
 constexpr int DI_OWN = 32 * DI_NW;                // rows it owns
@@ -79,13 +79,13 @@ struct DistillWorkspace {
     int64_t runs;      // workgroups of the backward pass
 };
 
-// Into how many ranges to cut the streamed tiles: the fewest rounds of 256 workgroups, each paying for its start (four
+// Into how many ranges to cut the streamed tiles: the fewest rounds of workgroups, each paying for its start (four
 // tiles' time) and for the partial results (written and read once more: 0.025 of a tile's time per owned block).
-static int distill_splits(int64_t blocks, int64_t tiles) {
+static int distill_splits(int64_t blocks, int64_t tiles, int64_t places) {
     int best = 1;
     double cost = 1e300;
     for (int64_t s = 1; s <= DI_RANGES && s <= tiles; ++s) {
-        const double rounds = (double)((blocks * s + DI_CUS - 1) / DI_CUS);
+        const double rounds = (double)((blocks * s + places - 1) / places);
         const double c = rounds * ((double)((tiles + s - 1) / s) + 4.0) + (s > 1 ? 0.025 * (double)(blocks * s) : 0.0);
         if (c < cost) {
             cost = c;
@@ -106,12 +106,15 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.xtiles = (n + 31) / 32;
     w.ytiles = (m + 31) / 32;
     const int64_t xblocks = (n + DI_OWN - 1) / DI_OWN, yblocks = (m + DI_OWN - 1) / DI_OWN;
-    w.splits_x = distill_splits(xblocks, w.ytiles);
+    // workgroups of the two passes that run at once (2000 x 20000 at 32 columns: backward 43 us with one on a compute unit, 35 with
+    // two; at 64 columns two gain nothing)
+    const int64_t places = f <= 32 ? 2 * DI_CUS : DI_CUS;
+    w.splits_x = distill_splits(xblocks, w.ytiles, places);
     // Cut the blocks of items where that saves more steps than the join of their parts costs.  (256 rows of 7207 items at 96
     // columns, 8 row tiles and 29 blocks: 56 us cut, 64 whole; 128 of 27000 at 128 columns, 4 and 106: 84 and 71; 512 of 60000, 16
     // and 235: 170 and 154.)
-    const int64_t steps = yblocks * w.xtiles, whole = (yblocks + DI_CUS - 1) / DI_CUS * w.xtiles;
-    w.runs = whole <= (steps + DI_CUS - 1) / DI_CUS + DI_JOIN_STEPS ? yblocks : steps < DI_CUS ? steps : DI_CUS;
+    const int64_t steps = yblocks * w.xtiles, whole = (yblocks + places - 1) / places * w.xtiles;
+    w.runs = whole <= (steps + places - 1) / places + DI_JOIN_STEPS ? yblocks : steps < places ? steps : places;
     w.max_off = take(3 * DI_PARTS * 4);       // partial maxima of |X|, |Y|, |grad|
     w.ref_off = take((size_t)n * 4);          // M_b: log2 reference of a row's mass
     w.mass_off = take((size_t)n * 4);         // sum_j 2^(z_bj log2 e - M_b)
@@ -627,8 +630,9 @@ __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* _
 // same item merged (their probabilities add); the row's loss; its dX but for the weight.  Latency, not bandwidth, is
 // what a row costs (a chain of a dozen dependent steps): factor rows are read by sixteen lanes each, four rows of a
 // group of lanes in flight, and what does not depend on each other is asked for at once.  NT threads: 256 finish a row
-// soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) many rows: DI_MANY_ROWS (4096 lists of
-// 100 at 128 columns: 34 us, of which the factor rows, 0.2 GB from L2, are a third).
+// soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) more rows than run at once with 256
+// (DI_MANY_ROWS: 1024 lists of 50 at 64 columns 12 and 16 us, 1500 of 200 at 192 columns 52 and 40).  4096 lists of 100 at 128
+// columns: 34 us, of which the factor rows, 0.2 GB from L2, are a third.
 template <int F, int NT>
 __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list_kernel(
     const float* __restrict__ X, int64_t n, const float* __restrict__ Y, int64_t m, const int32_t* __restrict__ ids,
@@ -1145,7 +1149,7 @@ static int launch_forward(const DistillWorkspace& L, char* w, const float* X, in
                        w + L.ximg_off, n, blocks, w + L.yimg_off, m, L.ytiles, per, step, parts, (float*)(w + L.pref_off),
                        (float*)(w + L.pmass_off), (float*)(w + L.part_off));
     MIREC_LAUNCH_CHECK();
-    const int nt = n >= DI_MANY_ROWS ? 64 : 256;
+    const int nt = n > DI_MANY_ROWS ? 64 : 256;
     hipLaunchKernelGGL(nt == 64 ? (distill_list_kernel<F, 64>) : (distill_list_kernel<F, 256>),
                        dim3((unsigned)(n < 262144 ? n : 262144)), dim3(nt), (size_t)((k + 63) & ~63) * 24, stream, X, n, Y, m,
                        ids, scores, k, temperature, teacher_lse, (int)ranges, (const float*)(w + L.pref_off),
