@@ -276,8 +276,8 @@ __global__ __launch_bounds__(256) void sample_short_kernel(
     };
 
     // A row is read while the one before it is worked on.
-    typename ScoreType<DT>::raw next_s[E];
-    int32_t next_id[E];
+    typename ScoreType<DT>::raw next_s[E] = {};
+    int32_t next_id[E] = {};
     float next_u = 0.f;
     auto fetch = [&]() {
 #pragma unroll
