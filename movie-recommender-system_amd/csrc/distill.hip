@@ -72,8 +72,8 @@ struct DistillTile {
 
 // Workspace of a call pair (host side): what mirec_distill_loss leaves for mirec_distill_grad, and scratch.
 struct DistillWorkspace {
-    size_t max_off, ref_off, mass_off, a_off, count_off, id_off, val_off, start_off, place_off, gval_off, row_off, base_off, ximg_off, yimg_off, pref_off,
-        pmass_off, part_off, bytes;
+    size_t max_off, ref_off, mass_off, a_off, count_off, id_off, val_off, start_off, place_off, gval_off, row_off, base_off;
+    size_t ximg_off, yimg_off, pref_off, pmass_off, part_off, bytes;
     int64_t xtiles, ytiles;
     int splits_x;      // ranges that Y is cut into in the forward pass
     int64_t runs;      // workgroups of the backward pass
@@ -583,8 +583,8 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
         const int64_t item = own0 + (lane & 31);
         if (active && item < m) {
             // a part of a block goes to slot 0 where the run begins with it, else to slot 1
-            float* out = t0 == 0 && t1 == xt ? dY + item * F
-                                                 : slots + ((2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * DI_OWN + wave * 32 + (lane & 31)) * F;
+            const int64_t slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
+            float* out = t0 == 0 && t1 == xt ? dY + item * F : slots + (slot * DI_OWN + wave * 32 + (lane & 31)) * F;
 #pragma unroll
             for (int u = 0; u < F / 32; ++u)
 #pragma unroll
@@ -601,7 +601,8 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
 // run; it takes the block that its run begins inside of, if no run before it does.
 __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* __restrict__ slots, int64_t steps, int64_t runs,
                                                                   int64_t xtiles, int64_t m, int f, float* __restrict__ dY) {
-    const int64_t begin = di_run_begin(blockIdx.x + 1, steps, runs), block = di_quotient(begin, xtiles), s0 = block * xtiles, s1 = s0 + xtiles;
+    const int64_t begin = di_run_begin(blockIdx.x + 1, steps, runs), block = di_quotient(begin, xtiles);
+    const int64_t s0 = block * xtiles, s1 = s0 + xtiles;
     const int64_t w0 = blockIdx.x, before = di_run_begin(w0, steps, runs);   // the run that ends inside the block
     if (begin == s0 || before > s0) return;
     // one past the last run with a part of the block: the first whose steps begin behind it
@@ -1048,7 +1049,10 @@ __device__ __forceinline__ void di_weigh(int block, const float* __restrict__ ba
     for (int64_t b0 = threadIdx.x; b0 < n; b0 += 8 * DI_PREPARE_THREADS) {
         uint32_t u[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = b0 + i * DI_PREPARE_THREADS < n ? __float_as_uint(grad[b0 + i * DI_PREPARE_THREADS]) & 0x7fffffffu : 0u;
+        for (int i = 0; i < 8; ++i) {
+            const int64_t b = b0 + i * DI_PREPARE_THREADS;
+            u[i] = b < n ? __float_as_uint(grad[b]) & 0x7fffffffu : 0u;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = u[i] > top ? u[i] : top;
     }
@@ -1062,12 +1066,13 @@ __device__ __forceinline__ void di_weigh(int block, const float* __restrict__ ba
     for (int w = 0; w < DI_PREPARE_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
     if (block == 0 && threadIdx.x < DI_PARTS) parts[threadIdx.x] = top;
     const int sg = di_exponent_of(top);
+    const int64_t mine = (int64_t)block * DI_PREPARE_THREADS + threadIdx.x, stride = (int64_t)DI_WEIGH_BLOCKS * DI_PREPARE_THREADS;
     if (dX)
-        for (int64_t e = ((int64_t)block * DI_PREPARE_THREADS + threadIdx.x) * 4; e < n * f; e += (int64_t)DI_WEIGH_BLOCKS * DI_PREPARE_THREADS * 4) {
+        for (int64_t e = mine * 4; e < n * f; e += stride * 4) {
             const float g = grad[e / f] * temperature;
             *reinterpret_cast<f32x4*>(dX + e) = *reinterpret_cast<const f32x4*>(base + e) * g;
         }
-    for (int64_t b = (int64_t)block * DI_PREPARE_THREADS + threadIdx.x; b < ((n + 31) & ~(int64_t)31); b += (int64_t)DI_WEIGH_BLOCKS * DI_PREPARE_THREADS) {
+    for (int64_t b = mine; b < ((n + 31) & ~(int64_t)31); b += stride) {
         float* to = rows + b / 32 * 128 + b % 32;
         const float g = b < n ? ldexpf(grad[b], sg) : 0.f;
         to[0] = b < n ? -ref[b] : 0.f;
@@ -1174,7 +1179,8 @@ static int launch_backward(const DistillWorkspace& L, char* w, int64_t n, int64_
                        (const uint16_t*)(w + L.place_off), (const float*)(w + L.gval_off), k, dY, slots);
     MIREC_LAUNCH_CHECK();
     if (blocks % L.runs != 0) {   // (else every run is of whole blocks)
-        hipLaunchKernelGGL(distill_join_kernel, dim3((unsigned)(L.runs - 1), DI_OWN * F / (4 * DI_THREADS)), dim3(DI_THREADS), 0, stream, slots, steps,
+        const dim3 grid((unsigned)(L.runs - 1), DI_OWN * F / (4 * DI_THREADS));
+        hipLaunchKernelGGL(distill_join_kernel, grid, dim3(DI_THREADS), 0, stream, slots, steps,
                            L.runs, L.xtiles, m, F, dY);
         MIREC_LAUNCH_CHECK();
     }

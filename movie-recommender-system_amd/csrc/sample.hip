@@ -22,6 +22,7 @@ constexpr int64_t SM_MAX_MASKED_ITEMS = MIREC_SAMPLE_MAX_MASKED_ITEMS;   // the 
 constexpr double SM_MIN_TEMPERATURE = 1e-37;      // below: greedy
 constexpr int SM_SHORT = 256;                     // rows up to this length: in the registers of a wavefront
 constexpr int64_t SM_FEW_ROWS = 256;              // no more rows than compute units: larger workgroups
+constexpr int64_t SM_SOME_ROWS = 768;             // no more rows than three workgroups to a compute unit
 constexpr int SM_AHEAD = 2;                       // loads in flight ahead of the work
 constexpr int SM_BINS = 1024;                     // of a histogram over a row
 constexpr int SM_FEW = 256;                        // entries that are compared with each other for every sum
@@ -521,8 +522,8 @@ struct Chunk {
 //
 // What bounds it: where the rows in flight exceed L2 each pass reads them at the rate of memory (two passes over 4096 x 27000
 // in 186 us, 4.75 TB/s), and a weight is 21 instructions (nine of them its polynomial); under top_p both take about 280 of
-// the 340 us of those rows.  Hence as few passes as possible, and rows of 512 threads side by side on a compute unit, or one
-// of 1024 where there are no more rows than compute units.  Measured: 1024 x 27000 under top_p 111 us, 512 x 200000 bf16 uncut,
+// the 340 us of those rows.  Hence as few passes as possible, and four rows of 256 threads side by side on a compute unit, or
+// fewer of more threads where there are fewer rows.  Measured: 1024 x 27000 under top_p 111 us, 512 x 200000 bf16 uncut,
 // 8 draws, 149 us, one row of 27000 under top_k 17 us.
 // Registers: few rows, of 1024 threads, run one or two workgroups to a compute unit and are faster with more registers
 // (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6); 512 threads are faster with 6 (mixed
@@ -723,7 +724,9 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
             if (own_top > -INFINITY) atomicAdd(&count_bins[first_bin(own_top)], 1u);
             __syncthreads();
             uint64_t all;
-            const int found = find_bin(count_bins, 0, [&](uint64_t at, uint64_t mine, uint64_t) { return at < (uint64_t)cuts.top_k && at + mine >= (uint64_t)cuts.top_k; }, all);
+            const uint64_t target = (uint64_t)cuts.top_k;
+            const int found = find_bin(count_bins, 0, [&](uint64_t at, uint64_t mine, uint64_t) { return at < target && at + mine >= target; },
+                                       all);
             const uint32_t last_bin = found >= 0 ? (uint32_t)found : SM_BINS - 1;   // (fewer threads with scores: all of them)
             each([&](const C& q, int32_t first, int, int) {
                 float most = q.score(0);
@@ -915,7 +918,8 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
                         return mine > 0 && (at < bound || at == base);
                     }, all);
                 else
-                    b = find_bin(count_bins, base, [&](uint64_t at, uint64_t mine, uint64_t) { return at < target && at + mine >= target; }, all);
+                    b = find_bin(count_bins, base, [&](uint64_t at, uint64_t mine, uint64_t) { return at < target && at + mine >= target; },
+                                 all);
                 if (b < 0) return;   // by count: fewer items than the target
                 base = shared_key[1];
                 auto member = [&](float f, int32_t item) -> bool {
@@ -992,7 +996,8 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
                             atomicMin((unsigned long long*)&shared_key[0], (unsigned long long)x.x);
                             // (by mass in the first histogram: what lies above the bin is in the pieces already)
                             if (BY_MASS && shift < 0 && x.y >= cuts.floor_w)
-                                atomicAdd((unsigned long long*)&piece_mass[(int32_t)(0xffffffffu - (uint32_t)x.x) / (WAVE_CHUNK * S)], (unsigned long long)x.y);
+                                atomicAdd((unsigned long long*)&piece_mass[(int32_t)(0xffffffffu - (uint32_t)x.x) / (WAVE_CHUNK * S)],
+                                          (unsigned long long)x.y);
                         }
                     }
                     if (BY_MASS && shift < 0) summed = true;
@@ -1101,7 +1106,8 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
             }
             const uint64_t t = sm_target(uniforms[row * draws + d], total);
             const int p16 = __builtin_ctzll(__ballot(piece_mass[lane * (SM_BINS / 64) + SM_BINS / 64 - 1] > t));
-            const int p = p16 * (SM_BINS / 64) + __builtin_ctzll(__ballot(lane >= SM_BINS / 64 || piece_mass[p16 * (SM_BINS / 64) + (lane & (SM_BINS / 64 - 1))] > t));
+            const uint64_t upto16 = piece_mass[p16 * (SM_BINS / 64) + (lane & (SM_BINS / 64 - 1))];
+            const int p = p16 * (SM_BINS / 64) + __builtin_ctzll(__ballot(lane >= SM_BINS / 64 || upto16 > t));
             uint64_t run = p > 0 ? piece_mass[p - 1] : 0ull;
             for (int sub = 0; sub < S; ++sub) {
                 C q = load(p, sub);
@@ -1210,7 +1216,8 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
                          int replacement, const SampleParams& par, int bits, int32_t* out_ids, float* out_logprob,
                          hipStream_t stream) {
     const typename ScoreType<DT>::raw* scores = (const typename ScoreType<DT>::raw*)scores_;
-#define MIREC_SAMPLE_ARGS stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids, out_logprob, stream
+#define MIREC_SAMPLE_ARGS \
+    stride, ids, ids_stride, mask_indptr, mask_indices, uniforms, draws, replacement, par, bits, out_ids, out_logprob, stream
     // Two rows to a wavefront where a row has at most two items a lane then (262144 lists of 50: 107 -> 76 us).  Up to 128
     // items ranked lists, which are in order, still gain (of 100: 139 -> 107 us); dense rows cost their comparisons and are
     // sooner done with a wavefront each (one of 100: 17 us shared, 11 us alone; 262144: 1.28 ms either way).
@@ -1218,9 +1225,13 @@ static int launch_sample(const void* scores_, int64_t n, int64_t m, int64_t stri
     if (ids && m <= 128) return launch_short<DT, 4, 2>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= 128) return launch_short<DT, 2, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
     if (m <= SM_SHORT) return launch_short<DT, 4, 1>(scores, n, (int)m, MIREC_SAMPLE_ARGS);
-    if (ids) return m > 8192 ? launch_long<DT, 512, true>(scores, n, m, MIREC_SAMPLE_ARGS) : launch_long<DT, 256, true>(scores, n, m, MIREC_SAMPLE_ARGS);
+    // Threads to a row: as few as fill the chip, since a row's barriers cost by the thread (256 / 512 threads, uncut: 1024 x 27000
+    // 47 / 53 us, 4096 x 12000 74 / 92 us; under top_k 50: 41 / 60 and 86 / 132 us); few long rows need more (512 x 200000 under
+    // top_p 831 / 612 us; with 1024 threads 256 x 27000 under top_p 36 us, with 512 47).
+    if (ids && n <= SM_SOME_ROWS && m > 16384) return launch_long<DT, 512, true>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (ids) return launch_long<DT, 256, true>(scores, n, m, MIREC_SAMPLE_ARGS);
     if (n <= SM_FEW_ROWS && m > 8192) return launch_long<DT, 1024, false>(scores, n, m, MIREC_SAMPLE_ARGS);
-    if (m > 8192) return launch_long<DT, 512, false>(scores, n, m, MIREC_SAMPLE_ARGS);
+    if (n <= SM_SOME_ROWS && m > 16384) return launch_long<DT, 512, false>(scores, n, m, MIREC_SAMPLE_ARGS);
     return launch_long<DT, 256, false>(scores, n, m, MIREC_SAMPLE_ARGS);
 #undef MIREC_SAMPLE_ARGS
 }

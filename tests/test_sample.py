@@ -1,10 +1,10 @@
 """Drawing items from scores: engine.sample_scores / mirec_sample against a float64 statement of its definition.
 
 A draw is checked by the interval of (0, 1) that belongs to the item: the device's running sum may sit off the float64 one
-by the weights' own error.  A weight is 2^f by a polynomial within 1.6e-14 of it, its exponent
-a product of float64 numbers below 2^7 (2^-46 ln 2 of it at most) in float64 arithmetic (a dozen roundings, each 2^-53),
-rounded to S = min(51, 62 - ceil(log2 m)) fraction bits; with the largest weight 1 the borders of the normalised running sum are off by at most 2 (3e-13 + m 2^-(S+1)).  The logarithm of
-the probability carries the same and one rounding to fp32 (half a step: 2^-24 of it)."""
+by the weights' own error.  A weight is 2^f by a polynomial within 1.6e-14 of it, its exponent a product of float64 numbers
+below 2^7 (2^-46 ln 2 of it at most) in float64 arithmetic (a dozen roundings, each 2^-53), rounded to S = min(51, 62 -
+ceil(log2 m)) fraction bits; with the largest weight 1 the borders of the normalised running sum are off by at most 2 (3e-13
++ m 2^-(S+1)).  The logarithm of the probability carries the same and one rounding to fp32 (half a step: 2^-24 of it)."""
 
 import ctypes
 import math
