@@ -523,11 +523,11 @@ struct Chunk {
 // What bounds it: where the rows in flight exceed L2 each pass reads them at the rate of memory (two passes over 4096 x 27000
 // in 186 us, 4.75 TB/s), and a weight is 21 instructions (nine of them its polynomial); under top_p both take about 280 of
 // the 340 us of those rows.  Hence as few passes as possible, and four rows of 256 threads side by side on a compute unit, or
-// fewer of more threads where there are fewer rows.  Measured: 1024 x 27000 under top_p 111 us, 512 x 200000 bf16 uncut,
+// fewer of more threads where there are fewer rows.  Measured: 1024 x 27000 under top_p 104 us, 512 x 200000 bf16 uncut,
 // 8 draws, 149 us, one row of 27000 under top_k 17 us.
 // Registers: few rows, of 1024 threads, run one or two workgroups to a compute unit and are faster with more registers
-// (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6); 512 threads are faster with 6 (mixed
-// requests 384 -> 350 us).
+// (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6).  512 threads ask for 6; of 256 threads LDS
+// admits four rows, and a fifth (histogram, list and draws in one place) gains under top_p what it loses under top_k.
 template <int DT, int NT, bool LISTS>
 __global__ __launch_bounds__(NT, NT == 1024 ? 4 : 6) void sample_long_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,
