@@ -24,11 +24,11 @@ def listed():
         # one user's request over the whole catalogue, the user's liked items filtered
         dict(SAMPLE, name="sample: one user", rows=1, items=27000, liked=50, temperature=0.7, top_k=50, top_p=0.9),
         # a few hundred requests in half precision over a small catalogue of an odd size, three items each
-        dict(SAMPLE, name="sample: f16 min-p", rows=300, items=7207, dtype="f16", draws=3, temperature=1.3, min_p=0.05),
+        dict(SAMPLE, name="sample: f16, min-p", rows=300, items=7207, dtype="f16", draws=3, temperature=1.3, min_p=0.05),
         # a batch of users, nucleus sampling over everything they have not seen
         dict(SAMPLE, name="sample: nucleus", rows=1024, items=27000, liked=50, temperature=0.7, top_p=0.95),
         # sampled negatives for training: several draws per user from the untruncated softmax, large catalogue
-        dict(SAMPLE, name="sample: negatives bf16", rows=512, items=200000, dtype="bf16", draws=8),
+        dict(SAMPLE, name="sample: negatives, bf16", rows=512, items=200000, dtype="bf16", draws=8),
         # an offline pass over the ranked lists of many users
         dict(SAMPLE, name="sample: many lists", rows=262144, items=100, lists=True, temperature=0.5, top_p=0.9, min_p=0.02),
         # requests of many callers in one batch, each with parameters of its own
@@ -40,7 +40,7 @@ def listed():
         # odd sizes, lists of different lengths (some empty), a width between the usual ones
         dict(DISTILL, name="distill: ragged lists", rows=777, items=7207, f=96, listed=37, ragged=True, temperature=1.5),
         # a large step at the benchmark's width, the teacher's mass outside its list kept as one class
-        dict(DISTILL, name="distill: f=128 tail", rows=4096, items=27000, f=128, listed=100, tail=True, temperature=2.0),
+        dict(DISTILL, name="distill: f=128, tail", rows=4096, items=27000, f=128, listed=100, tail=True, temperature=2.0),
         # the large catalogue
         dict(DISTILL, name="distill: 200 k items", rows=2048, items=200000, f=128, listed=20),
     ]
