@@ -123,15 +123,17 @@ __device__ __forceinline__ double sm_log2(double x) {
 
 // One step: v of another lane is added where the move reaches from a lane that is there (elsewhere the instruction does
 // nothing).  Written out because the compiler moves and adds separately: seven instructions a step instead of two, a third
-// of what a piece of a long row costs.  A data-parallel read of a register needs two wait states behind its write.
+// of what a piece of a long row costs.  A data-parallel read of a register needs two wait states behind its write, and so
+// does reading vcc as a carry behind the vector instruction that wrote it (the compiler puts an s_nop 1 there, too): the
+// wait between the two instructions of a step is enough for both.
 #define SM_ADD_STEP(MOVE)                                       \
-    "s_nop 0\n"                                                 \
     "v_add_co_u32_dpp %0, vcc, %0, %0 " MOVE " bank_mask:0xf\n"  \
+    "s_nop 1\n"                                                 \
     "v_addc_co_u32_dpp %1, vcc, %1, %1, vcc " MOVE " bank_mask:0xf\n"
 
 __device__ __forceinline__ uint64_t sm_half_scan(uint64_t v) {   // inclusive, over lanes 0 .. 31 and 32 .. 63
     uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
-    asm("s_nop 0\n"                                              // shifted by 1, 2, 4, 8 within rows of 16 lanes,
+    asm("s_nop 1\n"                                              // shifted by 1, 2, 4, 8 within rows of 16 lanes,
         SM_ADD_STEP("row_shr:1 row_mask:0xf") SM_ADD_STEP("row_shr:2 row_mask:0xf") SM_ADD_STEP("row_shr:4 row_mask:0xf")
         SM_ADD_STEP("row_shr:8 row_mask:0xf") SM_ADD_STEP("row_bcast:15 row_mask:0xa")   // lane 15 of a row to rows 1 and 3
         "s_nop 1" : "+v"(lo), "+v"(hi) : : "vcc");
@@ -141,7 +143,7 @@ __device__ __forceinline__ uint64_t sm_half_scan(uint64_t v) {   // inclusive, o
 __device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
     v = sm_half_scan(v);
     uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
-    asm("s_nop 0\n" SM_ADD_STEP("row_bcast:31 row_mask:0xc") "s_nop 1" : "+v"(lo), "+v"(hi) : : "vcc");   // lane 31 to rows 2 and 3
+    asm("s_nop 1\n" SM_ADD_STEP("row_bcast:31 row_mask:0xc") "s_nop 1" : "+v"(lo), "+v"(hi) : : "vcc");   // lane 31 to rows 2 and 3
     return ((uint64_t)hi << 32) | lo;
 }
 

@@ -8,6 +8,8 @@ ceil(log2 m)) fraction bits; with the largest weight 1 the borders of the normal
 
 import ctypes
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -129,6 +131,38 @@ def test_the_wrapper_refuses_on_the_host():
         E.sample_scores(s.double(), torch.zeros(2, 1))
     with pytest.raises(ValueError):
         E.sample_scores(s[0], torch.zeros(2, 1))
+
+
+def waits_missing(source):
+    """Instructions written out in a HIP source that read vcc as a carry, or a register by a data-parallel move, less than
+    two wait states behind the vector instruction that wrote it.  The macros' steps follow each other, so every step is
+    read twice in a row."""
+    bad = []
+    for block in re.findall(r"#define SM_\w+_STEP(?:.*\\\n)*.*", source):
+        step = [i.strip() for text in re.findall(r'"((?:[^"\\]|\\.)*)"', block) for i in text.split("\\n")]
+        step = [i for i in step if re.match(r"[sv]_", i)]
+        written = {}     # register -> wait states since
+        for ins in step * 2:
+            nop = re.match(r"s_nop (\d+)", ins)
+            if nop:
+                written = {r: w + int(nop.group(1)) + 1 for r, w in written.items()}
+                continue
+            name, ops = ins.split(None, 1)
+            ops = re.findall(r"%\d|\bvcc\b", ops)
+            outs = 2 if "_co_" in name else 1
+            bad += [ins for r in ops[outs:] if written.get(r, 9) < 2]
+            written = {r: w + 1 for r, w in written.items()}
+            written.update({r: 0 for r in ops[:outs]})
+    return bad
+
+
+def test_cross_lane_steps_keep_their_wait_states():
+    text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "sample.hip")).read()
+    assert len(re.findall(r"#define SM_\w+_STEP", text)) == 2
+    assert waits_missing(text) == []
+    # what the check is for: a carry read directly behind its write, a move directly behind a write
+    assert waits_missing('#define SM_A_STEP(M) "s_nop 0\\n" "v_add_co_u32_dpp %0, vcc, %0, %0 " M "\\n" "v_addc_co_u32_dpp %1, vcc, %1, %1, vcc " M "\\n"')
+    assert waits_missing('#define SM_B_STEP(M) "s_nop 0\\nv_max_f32_dpp %0, %0, %0 " M "\\n"')
 
 
 # ------------------------------------------------------------------------------------------------------- on the GPU
