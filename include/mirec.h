@@ -305,7 +305,10 @@ int mirec_sample(const void* scores, int dtype, int64_t n, int64_t m, int64_t ro
  *   loss_b = T^2 sum_list p (log p - log q).
  * teacher_lse (fp32 [n] or null): log sum exp of ALL the teacher's scores over T; then
  * p = exp(scores / T - teacher_lse), and what the list leaves of both distributions is
- * one class more in the sum (the student's share of it is taken to be at least 2^-24).
+ * one class more in the sum.  The student's share q_r of it is summed over the items off
+ * the list, so that it is as exact as one probability however small; p_r / q_r, in loss
+ * and gradient, takes it to be at least 2^-24.  The teacher's p_r is 1 - sum p of fp32
+ * probabilities (0 if that is negative).
  * List entries with an id outside 0 .. m-1 or a score that is NaN or not above -FLT_MAX
  * are left out; entries that name the same item add up; a row without entries has loss
  * and gradient zero.

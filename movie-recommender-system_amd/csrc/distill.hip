@@ -7,18 +7,26 @@
 //   exp(t / T - lse) with the teacher's log-sum-exp given: what the list leaves, p_r = 1 - sum p, is one class more,
 //   which the student gives q_r = 1 - sum over the list of q)
 //   loss_b = T^2 [ sum_list p (log p - log q) + p_r (log p_r - log q_r) ]
-//   d loss_b / d (x_b . y_j) = T (q_j - p_j) on the list, T A_b q_j elsewhere, A_b = 1 - p_r / q_r (1 without the class)
+//   d loss_b / d (x_b . y_j) = T (q_j - p_j) on the list, T (1 - p_r / q_r) q_j elsewhere (T q_j without the class)
 //
-// so with mean_b = sum_j q_bj y_j
-//   dX_b = grad_b T [ A_b mean_b + sum_list ((1 - A_b) q_k - p_k) y_k ],   dY_j = sum_b grad_b T g_bj x_b,
-//   g_bj = A_b q_bj, or q_k - p_k where j is on row b's list.
+// Without the class, with mean_b = sum_j q_bj y_j over all items
+//   dX_b = grad_b T [ mean_b - sum_list p_k y_k ],   dY_j = sum_b grad_b T g_bj x_b,
+//   g_bj = q_bj, or q_k - p_k where j is on row b's list.
+// With it nothing is formed as a difference of near values (a student that is nearly certain of its list leaves a q_r of
+// 1e-6, less than the fp32 error of one): the pass over the items leaves the listed ones out, so that its mass and mean
+// are those of the rest, S_b = sum e_bj and mean_b = sum e_bj y_j / S_b over j off the list, e the exponentials; the
+// list's own logits complete the log-sum-exp, q_r = S_b / (S_b + sum_list e), and
+//   dX_b = grad_b T [ (q_r - p_r) mean_b + sum_list (q_k - p_k) y_k ],   g_bj = (q_r - p_r) e_bj / S_b off the list.
 //
 // The two passes over the n x m logits have one form: a wavefront owns 32 rows of one side (in registers), the other
 // side streams through LDS in tiles of 32 rows, a tile's 32 x 32 logits come off the matrix cores with the owned rows
 // as columns, so that a lane holds 16 logits of ONE owned row, become probabilities in registers and go straight back
 // into the matrix cores as the operand that weights the streamed rows: the streamed side's image is laid out for that
 // (below) and no logit passes through LDS or memory.
-//   distill_forward_kernel   owns rows of X, streams Y: running maximum, mass and mean of the items (dX's dense part)
+//   distill_forward_kernel   owns rows of X, streams Y: running maximum, mass and mean of the items (dX's dense part); with
+//                            the class the listed items' logits become minus infinity, found by the lists' entries
+//                            grouped by (row tile, item tile) before the pass (4096 x 27000 at 128, lists of 100: 164 us
+//                            without, 179 with; grouping 6 us beside the largest magnitudes)
 //   distill_backward_kernel  owns rows of Y, streams X: dY; the logits are formed a second time (three of twelve
 //                            matrix products) because keeping them would write and read n m of them
 // What bounds them: the matrix cores from 128 columns on (2048 x 200000 at 128: 0.53 and 0.62 ms, 1.10 PFLOP/s of plane
@@ -41,9 +49,9 @@ constexpr int DI_THREADS = 256;
 constexpr int DI_NW = 8;                          // wavefronts of a workgroup of the two passes
 constexpr int DI_OWN = 32 * DI_NW;                // rows it owns
 constexpr int DI_PARTS = 256;                     // partial maxima of a matrix
-constexpr int DI_MAX_THREADS = 1024;              // of the workgroups that find them
+constexpr int DI_MAX_THREADS = 1024;              // of the workgroups that find them and group lists
 constexpr int DI_RANGES = 256;                    // most ranges that the items are cut into in the forward pass
-constexpr int DI_PREPARE_THREADS = 1024;
+constexpr int DI_PREPARE_THREADS = DI_MAX_THREADS;
 constexpr int DI_WEIGH_BLOCKS = 64;
 constexpr int DI_BINS = 4096;                     // item tiles that di_group counts at a time
 constexpr int DI_CUS = 256;                       // workgroups that run at once
@@ -117,12 +125,13 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
     w.runs = whole <= (steps + places - 1) / places + DI_JOIN_STEPS ? yblocks : steps < places ? steps : places;
     w.max_off = take(3 * DI_PARTS * 4);       // partial maxima of |X|, |Y|, |grad|
     w.ref_off = take((size_t)n * 4);          // M_b: log2 reference of a row's mass
-    w.mass_off = take((size_t)n * 4);         // sum_j 2^(z_bj log2 e - M_b)
-    w.a_off = take((size_t)n * 4);            // A_b
+    w.mass_off = take((size_t)n * 4);         // sum_j 2^(z_bj log2 e - M_b), over all items or those off the list
+    w.a_off = take((size_t)n * 4);            // what the mean counts for: 1, or q_r - p_r
     w.count_off = take((size_t)n * 4);        // entries of the merged list
     w.id_off = take((size_t)n * k * 4);       // merged list
     w.val_off = take((size_t)n * k * 4);      // q - p of those
-    // the same by (row tile, item tile): where a group begins, the entries' places in their 32 x 32 block, q - p
+    // the same by (row tile, item tile): where a group begins, the entries' places in their 32 x 32 block, q - p (before that,
+    // with teacher_lse: the lists' entries for the forward pass, in place of q - p)
     w.start_off = take((size_t)w.xtiles * (w.ytiles + 1) * 2);
     w.place_off = take((size_t)n * k * 2);
     w.gval_off = take((size_t)n * k * 4);
@@ -140,18 +149,16 @@ static DistillWorkspace distill_layout(int64_t n, int64_t m, int f, int k) {
 
 // ------------------------------------------------------------------------------------------------ operand images
 
-// Largest magnitude of up to two arrays (blockIdx.y), as DI_PARTS partial maxima of bit patterns each (a NaN's is
-// above every number's).
-__global__ __launch_bounds__(DI_MAX_THREADS) void distill_absmax_kernel(const float* __restrict__ a, int64_t na,
-                                                                    const float* __restrict__ b, int64_t nb,
-                                                                    uint32_t* __restrict__ parts) {
+// Largest magnitude of two arrays, as DI_PARTS partial maxima of bit patterns each (a NaN's is above every number's).
+__device__ __forceinline__ void di_absmax(int block, const float* __restrict__ a, int64_t na, const float* __restrict__ b, int64_t nb,
+                                          uint32_t* __restrict__ parts) {
     __shared__ uint32_t part[DI_MAX_THREADS / 64];
-    const float* v = blockIdx.y ? b : a;
-    const int64_t cnt = blockIdx.y ? nb : na;
+    const float* v = block >= DI_PARTS ? b : a;
+    const int64_t cnt = block >= DI_PARTS ? nb : na;
     uint32_t top = 0;
     constexpr int64_t step = (int64_t)DI_PARTS * DI_MAX_THREADS * 4;
     // (the widths are multiples of 32: no tail; a thread past the end reads its first value again)
-    for (int64_t e = ((int64_t)blockIdx.x * DI_MAX_THREADS + threadIdx.x) * 4; e < cnt; e += 4 * step) {
+    for (int64_t e = ((int64_t)(block % DI_PARTS) * DI_MAX_THREADS + threadIdx.x) * 4; e < cnt; e += 4 * step) {
         f32x4 q[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const f32x4*>(v + (e + u * step < cnt ? e + u * step : e));
@@ -172,7 +179,7 @@ __global__ __launch_bounds__(DI_MAX_THREADS) void distill_absmax_kernel(const fl
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < DI_MAX_THREADS / 64; ++w) top = part[w] > top ? part[w] : top;
-        parts[blockIdx.y * DI_PARTS + blockIdx.x] = top;
+        parts[block] = top;
     }
 }
 
@@ -201,6 +208,9 @@ __device__ __forceinline__ int di_scale_exponent(const uint32_t* __restrict__ pa
     return di_exponent_of(top);
 }
 
+// What an entry of a list must be to count.
+__device__ __forceinline__ bool di_counts(int32_t id, float score, int64_t m) { return id >= 0 && id < m && score > -FLT_MAX; }
+
 __device__ __forceinline__ uint32_t di_pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
 }
@@ -213,6 +223,102 @@ __device__ __forceinline__ void di_split(float a, float b, uint32_t& hi, uint32_
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hi), "v"(a));
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hi), "v"(b));
     mid = di_pack(ra, rb);
+}
+
+// One workgroup per tile of 32 rows: their lists' entries grouped by item tile, and where every item tile's group begins.
+// A group's order does not matter: its entries are places of one 32 x 32 block.  Item tiles are counted in LDS, DI_BINS at a
+// time.  MERGED: lists as distill_list_kernel leaves them, `count` entries a row, written as place (row in the tile, column in the
+// item tile) and value (q - p); else the caller's lists, written to `word` for distill_forward_kernel.
+static_assert(((int64_t)1 << 26) / 32 < (1 << 22) - 1, "an item tile fits 22 bits, below the mark of no entry");
+template <bool MERGED>
+__device__ __forceinline__ void di_group(int64_t tile, const int32_t* __restrict__ count, const int32_t* __restrict__ list_id,
+                                         const float* __restrict__ list_val, int64_t n, int64_t m, int k, int64_t ytiles,
+                                         uint16_t* __restrict__ start, uint16_t* __restrict__ place, float* __restrict__ val,
+                                         uint32_t* __restrict__ word) {
+    __shared__ int32_t bins[DI_BINS];
+    __shared__ int32_t part[DI_PREPARE_THREADS / 64];
+    constexpr int PER = DI_BINS / DI_PREPARE_THREADS;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t row0 = tile * 32;
+    const int rows = (int)(n - row0 < 32 ? n - row0 : 32);
+    uint16_t* tile_start = start + tile * (ytiles + 1);
+    // this thread's entries: item tile (-1: not an entry), place in the 32 x 32 block, value
+    constexpr int HELD = 32 * DI_LIST / DI_PREPARE_THREADS;
+    int32_t in[HELD], spot[HELD];
+    float v[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int e = tid + i * DI_PREPARE_THREADS;
+        in[i] = -1;
+        if (e < rows * k) {
+            const int r = e / k;
+            const int32_t id = list_id[row0 * k + e];
+            v[i] = list_val[row0 * k + e];
+            spot[i] = r * 32 + (id & 31);
+            const bool entry = MERGED ? e - r * k < count[row0 + r] : di_counts(id, v[i], m);
+            in[i] = entry ? id >> 5 : -1;
+        }
+    }
+    int base = 0;
+    for (int64_t t0 = 0; t0 < ytiles; t0 += DI_BINS) {
+        for (int i = tid; i < DI_BINS; i += DI_PREPARE_THREADS) bins[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int64_t t = in[i] - t0;
+            if (in[i] >= 0 && t >= 0 && t < DI_BINS) atomicAdd(&bins[t], 1);
+        }
+        __syncthreads();
+        int sum = 0;
+        for (int i = 0; i < PER; ++i) sum += bins[tid * PER + i];
+        int inc = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(inc, d, 64);
+            inc += lane >= d ? o : 0;
+        }
+        if (lane == 63) part[wave] = inc;
+        __syncthreads();
+        int at = base + inc - sum;
+        for (int w = 0; w < DI_PREPARE_THREADS / 64; ++w) {
+            at += w < wave ? part[w] : 0;
+            base += part[w];
+        }
+        for (int i = 0; i < PER; ++i) {
+            const int c = bins[tid * PER + i];
+            bins[tid * PER + i] = at;
+            if (t0 + tid * PER + i < ytiles) tile_start[t0 + tid * PER + i] = (uint16_t)at;
+            at += c;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int64_t t = in[i] - t0;
+            if (in[i] >= 0 && t >= 0 && t < DI_BINS) {
+                const int64_t to = row0 * k + atomicAdd(&bins[t], 1);
+                if (MERGED) {
+                    place[to] = (uint16_t)spot[i];
+                    val[to] = v[i];
+                } else {
+                    word[to] = (uint32_t)in[i] << 10 | (uint32_t)spot[i];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (tid == 0) tile_start[ytiles] = (uint16_t)base;
+}
+
+// What the images and the forward pass wait for: workgroups 0 .. 2 DI_PARTS - 1 find the largest magnitudes, the others (only
+// with teacher_lse) group the lists.
+__global__ __launch_bounds__(DI_MAX_THREADS) void distill_scan_kernel(
+    const float* __restrict__ X, const float* __restrict__ Y, int f, uint32_t* __restrict__ parts, const int32_t* __restrict__ ids,
+    const float* __restrict__ scores, int64_t n, int64_t m, int k, int64_t ytiles, uint16_t* __restrict__ start,
+    uint32_t* __restrict__ word) {
+    if (blockIdx.x < 2 * DI_PARTS)
+        di_absmax((int)blockIdx.x, X, n * f, Y, m * f, parts);
+    else
+        di_group<false>((int64_t)blockIdx.x - 2 * DI_PARTS, nullptr, ids, scores, n, m, k, ytiles, start, nullptr, nullptr, word);
 }
 
 // One workgroup per tile: tiles of X first, then tiles of Y.  Rows behind the last are zero.
@@ -357,12 +463,15 @@ __device__ __forceinline__ uint32_t di_work_index() {
 }
 
 // Rows [32 w, 32 w + 32) of the block per wavefront against a range of item tiles: reference, mass and (GRAD) the
-// weighted sum of the items, per row and range.
-template <int F, bool GRAD>
+// weighted sum of the items, per row and range.  REST: of the items that are not on the row's list (a reference of minus
+// infinity where that leaves none).  `listed` holds a row tile's entries by ascending item tile, (item tile, row, column)
+// in 22, 5 and 5 bits; a wavefront holds 64 of them at a time, one per lane, and sets a bit for each that falls into the
+// current tile in the word of the lane that holds its logit.
+template <int F, bool GRAD, bool REST>
 __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
     const char* __restrict__ ximg, int64_t n, int64_t blocks, const char* __restrict__ yimg, int64_t m, int64_t ytiles,
-    int64_t tiles_per_range, float step, const uint32_t* __restrict__ parts, float* __restrict__ pref,
-    float* __restrict__ pmass, float* __restrict__ psum) {
+    int64_t tiles_per_range, float step, const uint32_t* __restrict__ parts, int k, const uint16_t* __restrict__ start,
+    const uint32_t* __restrict__ listed, float* __restrict__ pref, float* __restrict__ pmass, float* __restrict__ psum) {
     typedef DistillTile<F> D;
     constexpr int FETCH = GRAD ? D::BYTES : 2 * D::PLANE, STAGES = D::STAGES_FORWARD;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -382,6 +491,19 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
         if (t0 + i < t1) di_fetch<FETCH>(yimg + (t0 + i) * D::BYTES, lds + i * FETCH);
     f32x16 acc[F / 32] = {};
     float ref = -INFINITY, mass = 0.f;
+    uint32_t* out_bits = reinterpret_cast<uint32_t*>(lds + STAGES * FETCH) + wave * 64;
+    const uint32_t* entry = listed;
+    int entries = 0;                      // from `entry` on
+    uint32_t held = ~0u, next = ~0u;      // these 64 and the 64 behind them (no entry: behind every tile)
+    if (REST && active) {
+        out_bits[lane] = 0;
+        const uint16_t* at = start + own0 / 32 * (ytiles + 1);
+        const int e0 = at[t0];
+        entries = at[t1] - e0;
+        entry += own0 * k + e0;
+        if (lane < entries) held = entry[lane];
+        if (lane + 64 < entries) next = entry[lane + 64];
+    }
     int cur = 0;   // the buffer of the current tile
     for (int64_t t = t0; t < t1; ++t, cur = cur + 1 < STAGES ? cur + 1 : 0) {
         const char* tile = lds + cur * FETCH;
@@ -389,7 +511,33 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
         __syncthreads();   // this tile has arrived, and every wavefront is done with the one before it
         if (t + STAGES - 1 < t1) di_fetch<FETCH>(yimg + (t + STAGES - 1) * D::BYTES, lds + (cur > 0 ? cur - 1 : STAGES - 1) * FETCH);
         if (!active) continue;
+        bool some = false;   // of this tile's items is on a list
+        uint32_t bits = 0;   // which of this lane's
+        if (REST) {
+            for (;;) {
+                const bool here = held >> 10 == (uint32_t)t;
+                if (__any(here)) {
+                    some = true;
+                    const int r = held >> 5 & 31, c_of = held & 31;
+                    if (here) atomicOr(&out_bits[r + 32 * ((c_of >> 2) & 1)], 1u << (4 * (c_of >> 3) + (c_of & 3)));
+                }
+                if ((uint32_t)__builtin_amdgcn_readlane((int)held, 63) >> 10 > (uint32_t)t) break;
+                entry += 64;
+                entries -= 64;
+                held = next;
+                next = lane + 64 < entries ? entry[lane + 64] : ~0u;
+            }
+            if (some) {
+                asm volatile("" ::: "memory");   // written by other lanes of this wavefront, in order
+                bits = out_bits[lane];
+                out_bits[lane] = 0;
+            }
+        }
         f32x16 z = di_logits<F>(tile, own);
+        if (REST && some) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = (bits >> r) & 1u ? -INFINITY : z[r];
+        }
         if (t == ytiles - 1 && (m & 31)) {   // rows behind the last item
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -410,7 +558,7 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
             }
             ref = now;
         }
-        const float off = DI_HEADROOM - ref;
+        const float off = REST && ref == -INFINITY ? 0.f : DI_HEADROOM - ref;   // (no item so far: all terms are zero)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[r], c, off));
         float sum = 0.f;
@@ -460,7 +608,8 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int64_t run0 = di_run_begin(blockIdx.x, steps, gridDim.x), run1 = di_run_begin(blockIdx.x + 1, steps, gridDim.x);
     const int sx = di_scale_exponent(parts), sy = di_scale_exponent(parts + DI_PARTS);
-    const int sg = di_scale_exponent(parts + 2 * DI_PARTS);   // the weights of the rows; |q - p| and |A q| are at most 1
+    // the weights of the rows; |q - p| is at most 1, and so is |q_r - p_r| e / S: S sums the e off the list
+    const int sg = di_scale_exponent(parts + 2 * DI_PARTS);
     const float c = ldexpf(step, -sx - sy);
 
     const float back = ldexpf(temperature, -sx - sg);
@@ -566,7 +715,7 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
                 for (int i = 0; i < 4; ++i)
                     z[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[4 * g + i], c, off[i])) * w[i];
             }
-            // where an item is on a row's list, its gradient is not A q but q - p
+            // where an item is on a row's list its gradient is q - p (with the class, what stands there may have overflowed)
             if (have > 0) {
                 asm volatile("" ::: "memory");   // written by other lanes of this wavefront, in order
                 const uint32_t bits = fix_bits[lane];
@@ -627,15 +776,17 @@ __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* _
 
 // ------------------------------------------------------------------------------------------------------- the lists
 
-// One workgroup per row: joins the row's partial results; the list without its excluded entries, entries that name the
-// same item merged (their probabilities add); the row's loss; its dX but for the weight.  Latency, not bandwidth, is
+// One workgroup per row: joins the row's partial results (REST: with teacher_lse, those of the items off the list); the list
+// without its excluded entries, entries that name the same item merged (their probabilities add); the row's loss; its dX
+// but for the weight.  Latency, not bandwidth, is
 // what a row costs (a chain of a dozen dependent steps): factor rows are read by sixteen lanes each, four rows of a
 // group of lanes in flight, and what does not depend on each other is asked for at once.  NT threads: 256 finish a row
 // soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) more rows than run at once with 256
 // (DI_MANY_ROWS: 1024 lists of 50 at 64 columns 12 and 16 us, 1500 of 200 at 192 columns 52 and 40).  4096 lists of 100 at 128
-// columns: 34 us, of which the factor rows, 0.2 GB from L2, are a third.
-template <int F, int NT>
-__global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list_kernel(
+// columns with the class 48 us, of which the factor rows, 0.2 GB from L2, are a third.  REST: two sums of the list's items in
+// registers, three wavefronts per SIMD from 96 columns on (four spill: 50 us).
+template <int F, int NT, bool REST>
+__global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? (REST && F > 64 ? 3 : 4) : 2) void distill_list_kernel(
     const float* __restrict__ X, int64_t n, const float* __restrict__ Y, int64_t m, const int32_t* __restrict__ ids,
     const float* __restrict__ scores, int k, float temperature, const float* __restrict__ teacher_lse, int ranges,
     const float* __restrict__ pref, const float* __restrict__ pmass, const float* __restrict__ psum,
@@ -665,6 +816,17 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = tid >> 4, sub = tid & 15;
     const double inv_t = 1.0 / (double)temperature;
     const int sy = di_scale_exponent(parts + DI_PARTS);
+    auto block_max = [&](double v) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) v = fmax(v, __shfl_xor(v, d, 64));
+        if (NWV == 1) return v;
+        if (lane == 0) partd[0][wave] = v;
+        __syncthreads();
+        v = partd[0][0];
+        for (int w = 1; w < NWV; ++w) v = fmax(v, partd[0][w]);
+        __syncthreads();
+        return v;
+    };
     auto block_sum = [&](double v, int which) {
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
@@ -693,6 +855,7 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
             }
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            if (REST && top == -INFINITY) top = 0.f;   // every item is on the list
 #pragma unroll
             for (int i = 0; i < DI_RANGES / 64; ++i) {
                 r[i] = lane + 64 * i < ranges ? __builtin_amdgcn_exp2f(r[i] - top) : 0.f;
@@ -700,12 +863,12 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
             }
             sum = wave_sum(sum);
 #pragma unroll
-            for (int i = 0; i < DI_RANGES / 64; ++i) range_w[lane + 64 * i] = ldexpf(r[i] / sum, -sy);
+            for (int i = 0; i < DI_RANGES / 64; ++i) range_w[lane + 64 * i] = REST && sum == 0.f ? 0.f : ldexpf(r[i] / sum, -sy);
             if (lane == 0) {
                 row_ref = top;
                 row_mass = ldexpf(sum, -(int)DI_HEADROOM);
                 ref_out[b] = row_ref;
-                mass_out[b] = row_mass;
+                mass_out[b] = REST && sum == 0.f ? 1.f : row_mass;
             }
         }
         // The entries that count, the best of them, and whether two name the same item (a hash table, open addressing: at
@@ -721,7 +884,7 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
             const int e = tid + NT * i;
             my_id[i] = e < k ? ids[b * k + e] : -1;
             my_s[i] = e < k ? scores[b * k + e] : 0.f;
-            if (!(my_id[i] >= 0 && my_id[i] < m && my_s[i] > -FLT_MAX)) my_id[i] = -1;
+            if (!di_counts(my_id[i], my_s[i], m)) my_id[i] = -1;
             if (my_id[i] >= 0) top = fmaxf(top, my_s[i]);
             valid += my_id[i] >= 0 ? 1 : 0;
         }
@@ -769,10 +932,10 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
                 for (int c = tid; c < F; c += NT) base[b * F + c] = 0.f;
             continue;
         }
-        // log sum exp of the student's logits and of the teacher's
-        const double log_mass = (double)row_ref * 0.69314718055994531 + log((double)row_mass);
-        double teacher = 0.0;
-        if (teacher_lse) {
+        // log sum exp of the student's logits (of those off the list, with the class) and of the teacher's
+        const double log_rest = REST && row_mass == 0.f ? -INFINITY : (double)row_ref * 0.69314718055994531 + log((double)row_mass);
+        double log_mass = log_rest, teacher = 0.0;
+        if (REST) {
             teacher = (double)teacher_lse[b] - (double)top * inv_t;
         } else {
             double mass = 0.0;
@@ -846,66 +1009,100 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
             }
         }
         __syncthreads();
-        // The student's logits and probabilities on the list, and the items' sums under both distributions: a factor row is
-        // read once.
-        f32x2 sum_py[PIECES] = {}, sum_qy[PIECES] = {};
-        for (int e0 = group; e0 - group < merged; e0 += 4 * ROWS) {
-            f32x2 y[4][PIECES];
+        // f(e, whether it is an entry, this lane's pieces of the item's factors) for the entries of this group of lanes
+        auto each_entry = [&](auto&& f) {
+            for (int e0 = group; e0 - group < merged; e0 += 4 * ROWS) {
+                f32x2 y[4][PIECES];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int e = e0 + u * ROWS;
-                const float* v = Y + (int64_t)mid[e < merged ? e : 0] * F + 2 * sub;
+                for (int u = 0; u < 4; ++u) {
+                    const int e = e0 + u * ROWS;
+                    const float* v = Y + (int64_t)mid[e < merged ? e : 0] * F + 2 * sub;
 #pragma unroll
-                for (int i = 0; i < PIECES; ++i) y[u][i] = *reinterpret_cast<const f32x2*>(v + 32 * i);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int e = e0 + u * ROWS;
-                float z = 0.f;
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) {
-                    z = __builtin_fmaf(x[i][0], y[u][i][0], z);
-                    z = __builtin_fmaf(x[i][1], y[u][i][1], z);
+                    for (int i = 0; i < PIECES; ++i) y[u][i] = *reinterpret_cast<const f32x2*>(v + 32 * i);
                 }
 #pragma unroll
-                for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
-                const double lq = (double)z * inv_t - log_mass;
-                const float q = expf((float)lq), p = mp[e < merged ? e : 0];
-                if (e < merged) {
+                for (int u = 0; u < 4; ++u) f(e0 + u * ROWS, e0 + u * ROWS < merged, y[u]);
+            }
+        };
+        auto logit = [&](const f32x2 (&y)[PIECES]) -> float {
+            float z = 0.f;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                z = __builtin_fmaf(x[i][0], y[i][0], z);
+                z = __builtin_fmaf(x[i][1], y[i][1], z);
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+            return z;
+        };
+        f32x2 sum[PIECES] = {};   // of dX but for its weight: the list's part
+        auto add = [&](f32x2 (&to)[PIECES], float w, const f32x2 (&y)[PIECES]) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) to[i][j] = __builtin_fmaf(w, y[i][j], to[i][j]);
+        };
+        // The student's logits and probabilities on the list, and the sum of the list's items: a factor row is read once.  Without
+        // the class q is known from the mass of all items and is in their mean; with it a group of lanes holds its q relative
+        // to the largest it has met, until all of them complete the log-sum-exp.
+        if (!REST) {
+            each_entry([&](int e, bool real, const f32x2 (&y)[PIECES]) {
+                const float z = logit(y);
+                const float q = expf((float)((double)z * inv_t - log_mass)), p = mp[real ? e : 0];
+                if (real) {
                     if (sub == 0) {
                         mz[e] = z;
                         sp[e] = q;
                     }
+                    if (base) add(sum, -p, y);
+                }
+            });
+        } else {
+            f32x2 sum_q[PIECES] = {};
+            double group_top = -INFINITY, group_mass = 0.0;
+            each_entry([&](int e, bool real, const f32x2 (&y)[PIECES]) {
+                const float z = logit(y);
+                const double t = (double)z * inv_t;
+                const float p = mp[real ? e : 0];
+                if (real) {
+                    if (sub == 0) mz[e] = z;
+                    if (t > group_top) {
+                        const float back = expf((float)(group_top - t));
+                        group_mass *= (double)back;
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) sum_q[i] *= back;
+                        group_top = t;
+                    }
+                    const float q = expf((float)(t - group_top));
+                    group_mass += (double)q;
                     if (base) {
-#pragma unroll
-                        for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                sum_py[i][j] = __builtin_fmaf(p, y[u][i][j], sum_py[i][j]);
-                                if (teacher_lse) sum_qy[i][j] = __builtin_fmaf(q, y[u][i][j], sum_qy[i][j]);
-                            }
+                        add(sum, -p, y);
+                        add(sum_q, q, y);
                     }
                 }
-            }
+            });
+            const double top_log = block_max(fmax(group_top, log_rest));
+            const double list_mass = block_sum(sub == 0 ? group_mass * (double)expf((float)(group_top - top_log)) : 0.0, 1);
+            log_mass = top_log + log(list_mass + exp(log_rest - top_log));
+            const float scale = expf((float)(group_top - log_mass));
+            add(sum, scale, sum_q);
+            for (int e = tid; e < merged; e += NT) sp[e] = expf((float)((double)mz[e] * inv_t - log_mass));
         }
         __syncthreads();
-        double kl = 0.0, sum_p = 0.0, sum_q = 0.0;
+        double kl = 0.0, sum_p = 0.0;
         for (int e = tid; e < merged; e += NT) {
             const double logq = (double)mz[e] * inv_t - log_mass;
-            const float p = mp[e], q = sp[e];
+            const float p = mp[e];
             if (!(p <= 0.f)) kl += (double)p * ((double)mlogp[e] - logq);   // (a NaN probability stays in the sum)
             sum_p += (double)p;
-            sum_q += (double)q;
         }
         kl = block_sum(kl, 0);
-        float a = 1.f;
-        if (teacher_lse) {
+        float a = 1.f;   // what the mean counts for
+        if (REST) {
             const double pr = fmax(1.0 - block_sum(sum_p, 1), 0.0);
-            const double qr = fmax(1.0 - block_sum(sum_q, 0), 0x1p-24);
-            if (pr > 0.0) {
-                kl += pr * log(pr / qr);
-                a = (float)(1.0 - pr / qr);
-            }
+            const double log_qr = log_rest - log_mass, qr = exp(log_qr);   // bounded below by 2^-24 beside p_r
+            if (pr > 0.0) kl += pr * (log(pr) - fmax(log_qr, -24.0 * 0.69314718055994531));
+            a = (float)(qr - pr * fmin(qr * 0x1p24, 1.0));
         }
         if (tid == 0) {
             loss[b] = (float)((double)temperature * (double)temperature * kl);
@@ -917,12 +1114,7 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
             id_out[b * k + e] = mid[e];
             val_out[b * k + e] = sp[e] - mp[e];
         }
-        // dX but for its weight: (1 - A) sum q y - sum p y over the list, and A times the ranges' sums
-        f32x2 sum[PIECES];
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) sum[i][j] = __builtin_fmaf(1.f - a, sum_qy[i][j], -sum_py[i][j]);
+        // and the ranges' part
         for (int r0 = group; r0 - group < ranges; r0 += 4 * ROWS) {
             f32x2 y[4][PIECES];
             float w[4];
@@ -960,81 +1152,6 @@ __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? 4 : 2) void distill_list
             base[b * F + c] = v;
         }
     }
-}
-
-// One workgroup per tile of 32 rows: their merged lists' entries grouped by item tile, (row in the tile, column in the
-// item tile, q - p) each, and where every item tile's group begins.  A group's order does not matter: its entries are
-// different places of one 32 x 32 block.  Item tiles are counted in LDS, DI_BINS at a time.
-__device__ __forceinline__ void di_group(int64_t tile, const int32_t* __restrict__ count, const int32_t* __restrict__ list_id,
-                                         const float* __restrict__ list_val, int64_t n, int k, int64_t ytiles,
-                                         uint16_t* __restrict__ start, uint16_t* __restrict__ place, float* __restrict__ val) {
-    __shared__ int32_t bins[DI_BINS];
-    __shared__ int32_t part[DI_PREPARE_THREADS / 64];
-    constexpr int PER = DI_BINS / DI_PREPARE_THREADS;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row0 = tile * 32;
-    const int rows = (int)(n - row0 < 32 ? n - row0 : 32);
-    uint16_t* tile_start = start + tile * (ytiles + 1);
-    // this thread's entries: item tile (-1: not an entry), place in the 32 x 32 block, value
-    constexpr int HELD = 32 * DI_LIST / DI_PREPARE_THREADS;
-    int32_t in[HELD], spot[HELD];
-    float v[HELD];
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const int e = tid + i * DI_PREPARE_THREADS;
-        in[i] = -1;
-        if (e < rows * k) {
-            const int r = e / k;
-            const int32_t id = list_id[row0 * k + e];
-            v[i] = list_val[row0 * k + e];
-            spot[i] = r * 32 + (id & 31);
-            in[i] = e - r * k < count[row0 + r] ? id >> 5 : -1;
-        }
-    }
-    int base = 0;
-    for (int64_t t0 = 0; t0 < ytiles; t0 += DI_BINS) {
-        for (int i = tid; i < DI_BINS; i += DI_PREPARE_THREADS) bins[i] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int64_t t = in[i] - t0;
-            if (in[i] >= 0 && t >= 0 && t < DI_BINS) atomicAdd(&bins[t], 1);
-        }
-        __syncthreads();
-        int sum = 0;
-        for (int i = 0; i < PER; ++i) sum += bins[tid * PER + i];
-        int inc = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(inc, d, 64);
-            inc += lane >= d ? o : 0;
-        }
-        if (lane == 63) part[wave] = inc;
-        __syncthreads();
-        int at = base + inc - sum;
-        for (int w = 0; w < DI_PREPARE_THREADS / 64; ++w) {
-            at += w < wave ? part[w] : 0;
-            base += part[w];
-        }
-        for (int i = 0; i < PER; ++i) {
-            const int c = bins[tid * PER + i];
-            bins[tid * PER + i] = at;
-            if (t0 + tid * PER + i < ytiles) tile_start[t0 + tid * PER + i] = (uint16_t)at;
-            at += c;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int64_t t = in[i] - t0;
-            if (in[i] >= 0 && t >= 0 && t < DI_BINS) {
-                const int64_t to = row0 * k + atomicAdd(&bins[t], 1);
-                place[to] = (uint16_t)spot[i];
-                val[to] = v[i];
-            }
-        }
-        __syncthreads();
-    }
-    if (tid == 0) tile_start[ytiles] = (uint16_t)base;
 }
 
 // dX; and per tile of rows what they bring to the backward pass, 32 numbers each: minus the reference of a row's logits,
@@ -1088,12 +1205,12 @@ __global__ __launch_bounds__(DI_PREPARE_THREADS) void distill_prepare_kernel(
     const float* __restrict__ base, const float* __restrict__ grad, float temperature, int64_t n, int f, float* __restrict__ dX,
     const float* __restrict__ ref, const float* __restrict__ mass, const float* __restrict__ a, float* __restrict__ rows,
     uint32_t* __restrict__ parts, const int32_t* __restrict__ count, const int32_t* __restrict__ list_id,
-    const float* __restrict__ list_val, int k, int64_t ytiles, uint16_t* __restrict__ start, uint16_t* __restrict__ place,
+    const float* __restrict__ list_val, int64_t m, int k, int64_t ytiles, uint16_t* __restrict__ start, uint16_t* __restrict__ place,
     float* __restrict__ val) {
     if (blockIdx.x < DI_WEIGH_BLOCKS)
         di_weigh((int)blockIdx.x, base, grad, temperature, n, f, dX, ref, mass, a, rows, parts);
     else
-        di_group((int64_t)blockIdx.x - DI_WEIGH_BLOCKS, count, list_id, list_val, n, k, ytiles, start, place, val);
+        di_group<true>((int64_t)blockIdx.x - DI_WEIGH_BLOCKS, count, list_id, list_val, n, m, k, ytiles, start, place, val, nullptr);
 }
 
 __global__ __launch_bounds__(DI_THREADS) void distill_zero_kernel(float* __restrict__ out, int64_t cnt) {
@@ -1136,26 +1253,28 @@ static int distill_lds(const void* kernel, int bytes, OncePerDevice& once, const
     return MIREC_OK;
 }
 
-template <int F, bool GRAD>
+template <int F, bool GRAD, bool REST>
 static int launch_forward(const DistillWorkspace& L, char* w, const float* X, int64_t n, const float* Y, int64_t m,
                           const int32_t* ids, const float* scores, int k, float temperature, const float* teacher_lse,
                           float* loss, hipStream_t stream) {
     const float step = (float)(1.4426950408889634 / (double)temperature);
     static OncePerDevice once;
-    constexpr int LDS = DistillTile<F>::STAGES_FORWARD * (GRAD ? DistillTile<F>::BYTES : 2 * DistillTile<F>::PLANE);
-    if (const int rc = distill_lds((const void*)distill_forward_kernel<F, GRAD>, LDS, once, "mirec_distill_loss")) return rc;
+    constexpr int LDS = DistillTile<F>::STAGES_FORWARD * (GRAD ? DistillTile<F>::BYTES : 2 * DistillTile<F>::PLANE) +
+                        (REST ? DI_NW * 64 * 4 : 0);
+    if (const int rc = distill_lds((const void*)distill_forward_kernel<F, GRAD, REST>, LDS, once, "mirec_distill_loss")) return rc;
     uint32_t* parts = (uint32_t*)(w + L.max_off);
     hipLaunchKernelGGL((distill_image_kernel<F>), dim3((unsigned)(L.xtiles + L.ytiles)), dim3(DI_THREADS), 0, stream, X, n,
                        L.xtiles, w + L.ximg_off, Y, m, w + L.yimg_off, parts);
     MIREC_LAUNCH_CHECK();
     const int64_t blocks = (n + DI_OWN - 1) / DI_OWN, per = (L.ytiles + L.splits_x - 1) / L.splits_x;
     const int64_t ranges = (L.ytiles + per - 1) / per;
-    hipLaunchKernelGGL((distill_forward_kernel<F, GRAD>), dim3((unsigned)(blocks * ranges)), dim3(64 * DI_NW), LDS, stream,
-                       w + L.ximg_off, n, blocks, w + L.yimg_off, m, L.ytiles, per, step, parts, (float*)(w + L.pref_off),
-                       (float*)(w + L.pmass_off), (float*)(w + L.part_off));
+    hipLaunchKernelGGL((distill_forward_kernel<F, GRAD, REST>), dim3((unsigned)(blocks * ranges)), dim3(64 * DI_NW), LDS, stream,
+                       w + L.ximg_off, n, blocks, w + L.yimg_off, m, L.ytiles, per, step, parts, k, (const uint16_t*)(w + L.start_off),
+                       (const uint32_t*)(w + L.gval_off), (float*)(w + L.pref_off), (float*)(w + L.pmass_off),
+                       (float*)(w + L.part_off));
     MIREC_LAUNCH_CHECK();
     const int nt = n > DI_MANY_ROWS ? 64 : 256;
-    hipLaunchKernelGGL(nt == 64 ? (distill_list_kernel<F, 64>) : (distill_list_kernel<F, 256>),
+    hipLaunchKernelGGL(nt == 64 ? (distill_list_kernel<F, 64, REST>) : (distill_list_kernel<F, 256, REST>),
                        dim3((unsigned)(n < 262144 ? n : 262144)), dim3(nt), (size_t)((k + 63) & ~63) * 24, stream, X, n, Y, m,
                        ids, scores, k, temperature, teacher_lse, (int)ranges, (const float*)(w + L.pref_off),
                        (const float*)(w + L.pmass_off), (const float*)(w + L.part_off), parts, loss, (float*)(w + L.ref_off),
@@ -1163,6 +1282,15 @@ static int launch_forward(const DistillWorkspace& L, char* w, const float* X, in
                        (float*)(w + L.val_off), GRAD ? (float*)(w + L.base_off) : nullptr);
     MIREC_LAUNCH_CHECK();
     return MIREC_OK;
+}
+
+template <int F>
+static int launch_forward(bool grad, const DistillWorkspace& L, char* w, const float* X, int64_t n, const float* Y, int64_t m,
+                          const int32_t* ids, const float* scores, int k, float temperature, const float* teacher_lse,
+                          float* loss, hipStream_t stream) {
+    auto* launch = grad ? (teacher_lse ? launch_forward<F, true, true> : launch_forward<F, true, false>)
+                        : (teacher_lse ? launch_forward<F, false, true> : launch_forward<F, false, false>);
+    return launch(L, w, X, n, Y, m, ids, scores, k, temperature, teacher_lse, loss, stream);
 }
 
 template <int F>
@@ -1207,14 +1335,14 @@ extern "C" int mirec_distill_loss(const float* X, int64_t n, const float* Y, int
     const DistillWorkspace L = distill_layout(n, m, f, k);
     if (const int rc = distill_check_ws("mirec_distill_loss", ws, ws_bytes, L.bytes)) return rc;
     char* w = (char*)ws;
-    hipLaunchKernelGGL(distill_absmax_kernel, dim3(DI_PARTS, 2), dim3(DI_MAX_THREADS), 0, stream, X, n * f, Y, m * f,
-                       (uint32_t*)(w + L.max_off));
+    hipLaunchKernelGGL(distill_scan_kernel, dim3((unsigned)(2 * DI_PARTS + (teacher_lse ? L.xtiles : 0))), dim3(DI_MAX_THREADS), 0,
+                       stream, X, Y, f, (uint32_t*)(w + L.max_off), ids, scores, n, m, k, L.ytiles, (uint16_t*)(w + L.start_off),
+                       (uint32_t*)(w + L.gval_off));
     MIREC_LAUNCH_CHECK();
     switch (f) {
 #define MIREC_DISTILL_CASE(FW)                                                                                          \
     case FW:                                                                                                            \
-        return with_grad ? launch_forward<FW, true>(L, w, X, n, Y, m, ids, scores, k, temperature, teacher_lse, loss, stream) \
-                         : launch_forward<FW, false>(L, w, X, n, Y, m, ids, scores, k, temperature, teacher_lse, loss, stream);
+        return launch_forward<FW>(with_grad != 0, L, w, X, n, Y, m, ids, scores, k, temperature, teacher_lse, loss, stream);
         MIREC_DISTILL_WIDTHS(MIREC_DISTILL_CASE)
 #undef MIREC_DISTILL_CASE
     }
@@ -1245,7 +1373,7 @@ extern "C" int mirec_distill_grad(const float* X, int64_t n, const float* Y, int
                        stream, (const float*)(w + L.base_off), grad, temperature, n, f, dX, (const float*)(w + L.ref_off),
                        (const float*)(w + L.mass_off), (const float*)(w + L.a_off), (float*)(w + L.row_off),
                        (uint32_t*)(w + L.max_off) + 2 * DI_PARTS, (const int32_t*)(w + L.count_off),
-                       (const int32_t*)(w + L.id_off), (const float*)(w + L.val_off), k, L.ytiles, (uint16_t*)(w + L.start_off),
+                       (const int32_t*)(w + L.id_off), (const float*)(w + L.val_off), m, k, L.ytiles, (uint16_t*)(w + L.start_off),
                        (uint16_t*)(w + L.place_off), (float*)(w + L.gval_off));
     MIREC_LAUNCH_CHECK();
     if (!dY) return MIREC_OK;

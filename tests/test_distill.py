@@ -507,6 +507,110 @@ def test_items_beyond_32_bit_offsets(dev):
     assert torch.all((dY[zero.to(dev)].double().cpu() - (qz * x).sum(0)).abs() <= (rel + 16 * HALF) * (qz * x.abs()).sum(0) + tiny)
 
 
+def compare_with_rest(X, Y, ids, scores, T, tlse, grad, got):
+    """``compare`` for rows whose students leave little outside their lists.  A probability q (on the list or off it), and
+    with it the share q_r, is off by a factor 1 + rel: twice dz, the exponential and division, and 8 sqrt(m) 2^-24 for the
+    sums.  The teacher's p is fp32: its logarithm lp is rounded once (half a step, 2^-24 |lp|) and the exponential is within
+    4 of those steps; p_r = 1 - sum p carries the sum of these, dp.  Off the list the weight of an item is q - p_r q / q_r:
+    both terms' rel, and dp q / q_r.  The two fp16 numbers that hold a weight are off by 2^-32 of the row's largest
+    (dX, off the list), by 2^-39 of the largest T grad (dY)."""
+    loss, dX, dY, G, has = statement(X, Y, ids, scores, T, tlse, grad)
+    X, Y, ids, scores, grad = X.double().cpu(), Y.double().cpu(), ids.cpu(), scores.double().cpu(), grad.double().cpu()
+    n, f = X.shape
+    m = Y.shape[0]
+    logq = torch.log_softmax(X @ Y.T / T, 1)
+    p = torch.zeros(n, m, dtype=torch.float64)
+    on = torch.zeros(n, m, dtype=torch.bool)
+    for b in range(n):
+        for i, v in zip(ids[b].tolist(), scores[b].tolist()):
+            if 0 <= i < m and v > LOW:
+                p[b, i] += math.exp(v / T - float(tlse[b]))
+                on[b, i] = True
+    lp = torch.where(on, p.clamp(min=1e-300).log(), 0.0)
+    pr = (1.0 - p.sum(1)).clamp(min=0.0)
+    qr = torch.where(on, 0.0, logq.exp()).sum(1).clamp(min=2.0 ** -24)
+    dz = (8 * math.sqrt(f) * HALF + 2 * 2.0 ** -22) * float((X.abs() @ Y.abs().T).max()) / T
+    rel = 2 * dz + 16 * HALF + 8 * math.sqrt(m) * HALF
+    ep = p * (lp.abs() + 4) * HALF
+    dp = ep.sum(1)
+    q = logq.exp()
+    share = q / qr[:, None]
+    off = T * torch.where(on, rel * q + ep, rel * (q + pr[:, None] * share) + dp[:, None] * share) * has[:, None]
+    weigh = T * torch.where(on, 0.0, q + pr[:, None] * share).amax(1) * has
+    w = grad.abs()
+    tx = w[:, None] * (off @ Y.abs() + (8 * math.sqrt(m) + 16) * HALF * (G.abs() @ Y.abs()) + m * 2.0 ** -32 * weigh[:, None] * Y.abs().amax())
+    ty = (off * w[:, None]).T @ X.abs() + (8 * math.sqrt(n) + 16) * HALF * ((G.abs() * w[:, None]).T @ X.abs())
+    ty = ty + n * 2.0 ** -39 * T * w.max() * X.abs().amax()
+    part = torch.where(on, p * rel + ep * (lp - logq).abs(), 0.0).sum(1)
+    rest = torch.where(pr > 0, pr * rel + dp * (1 + (pr.clamp(min=1e-300) / qr).log().abs()), 0.0)
+    tl = T * T * (part + rest + 4 * HALF) + 4 * HALF * loss.abs()
+    for name, a, b, t in zip(("loss", "dX", "dY"), got, (loss, dX, dY), (tl, tx, ty)):
+        assert torch.all(torch.isfinite(a)), f"{name} is not finite"
+        over = (a.double().cpu() - b).abs() / t.clamp(min=1e-300)
+        assert torch.all(over <= 1), f"{name}: {float(over.max())} times the tolerance"
+
+
+def certain_student(seed, n, m, f, T, top, rest, noise, k=5):
+    """Logits (over T) of `top` for item 7, which is on every list, and about `rest` of the probability for all others
+    together, spread with a standard deviation of `noise`; half of the teacher's mass is off its list."""
+    g = torch.Generator().manual_seed(seed)
+    s = math.sqrt(noise * T / math.sqrt(f - 2))
+    X, Y = torch.randn(n, f, generator=g) * s, torch.randn(m, f, generator=g) * s
+    gap = math.log(m / rest) + noise * noise / 2
+    X[:, 0], Y[:, 0] = math.sqrt(T * gap), 0.0
+    Y[7, 0] = math.sqrt(T * gap)
+    common = T * (top - gap)
+    X[:, 1], Y[:, 1] = math.sqrt(abs(common)), math.copysign(math.sqrt(abs(common)), common)
+    ids = torch.stack([torch.cat([torch.tensor([7]), 8 + torch.randperm(m - 8, generator=g)[:k - 1]]) for _ in range(n)])
+    ids[::3, 1] = -1
+    scores = torch.randn(n, k, generator=g) * T
+    tlse = torch.logsumexp(torch.where(ids < 0, -math.inf, scores) / T, 1) + math.log(2.0)
+    return X, Y, ids.to(torch.int32), scores, tlse, 0.5 + torch.rand(n, generator=g)
+
+
+@gpu
+@pytest.mark.parametrize("f,T,noise", [(64, 1.0, 1.0), (64, 0.05, 3.0), (32, 1.0, 3.0), (160, 2.0, 1.0)])
+@pytest.mark.parametrize("rest", [1e-9, 1e-7, 1e-6, 1e-5, 1e-4, 1e-2])
+@pytest.mark.parametrize("top", [20.0, 48.0, 100.0])
+def test_a_student_certain_of_its_list(dev, top, rest, f, T, noise):
+    """What the student gives all items off the list is small beside what it gives the list, and its own sum."""
+    X, Y, ids, scores, tlse, grad = (v.to(dev) for v in certain_student(81, 70, 900, f, T, top, rest, noise))
+    got = E.distill(X, Y, ids, scores, temperature=T, teacher_lse=tlse, grad=grad)
+    compare_with_rest(X, Y, ids, scores, T, tlse, grad, got)
+    with torch.no_grad():
+        assert torch.equal(E.distill_loss(X, Y, ids, scores, T, tlse), got[0])
+
+
+@gpu
+@pytest.mark.parametrize("spread", [6.0, 8.0, 12.0])
+@pytest.mark.parametrize("n,m,f,k", [(1500, 900, 64, 50), (80, 5000, 128, 100), (40, 300, 96, 256)])
+def test_a_sharp_student_and_a_flat_teacher(dev, n, m, f, k, spread):
+    """Lists of the student's own best items, a teacher that hardly tells them apart and keeps up to a third or almost all of
+    its mass elsewhere; few and many rows, lists of every item of a tile."""
+    X, Y, _, _, _, grad = problem(82, n, m, f, 1, spread=spread)
+    g = torch.Generator().manual_seed(83)
+    ids = torch.topk(X @ Y.T, k, dim=1).indices
+    ids[1] = torch.arange(32, 32 + k)           # whole tiles of items
+    ids[2] = torch.arange(k).flip(0)
+    ids[3, k // 2:] = ids[3, :k - k // 2]       # items listed twice
+    ids[4] = -1
+    scores = torch.randn(n, k, generator=g)
+    tlse = torch.logsumexp(scores, 1) + 0.02 + 3 * torch.rand(n, generator=g)
+    X, Y, ids, scores, tlse, grad = (v.to(dev) for v in (X, Y, ids.to(torch.int32), scores, tlse, grad))
+    got = E.distill(X, Y, ids, scores, teacher_lse=tlse, grad=grad)
+    compare_with_rest(X, Y, ids, scores, 1.0, tlse, grad, got)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 32, 100, 256])
+def test_nothing_off_the_list(dev, m):
+    """Every item listed and mass of the teacher elsewhere: the student's share is taken to be 2^-24."""
+    X, Y, ids, scores, tlse, grad = problem(84, 40, m, 64, m, dev, tail=True)
+    tlse = tlse + 0.5
+    got = E.distill(X, Y, ids, scores, teacher_lse=tlse, grad=grad)
+    compare_with_rest(X, Y, ids, scores, 1.0, tlse, grad, got)
+
+
 @gpu
 @pytest.mark.parametrize("liked", [False, True])
 def test_a_model_learns_from_a_models_lists(dev, liked):
