@@ -208,6 +208,10 @@ __device__ __forceinline__ int di_scale_exponent(const uint32_t* __restrict__ pa
     return di_exponent_of(top);
 }
 
+// What takes a product of the scaled factors to the logit it stands for, in octaves.  It does not vanish, so that minus infinity
+// stays what it is: 2^-126 times the largest scaled logit (192 2^30) is nothing beside one, as the logit itself would be.
+__device__ __forceinline__ float di_logit_factor(float step, int exponent) { return fmaxf(ldexpf(step, -exponent), FLT_MIN); }
+
 // What an entry of a list must be to count.
 __device__ __forceinline__ bool di_counts(int32_t id, float score, int64_t m) { return id >= 0 && id < m && score > -FLT_MAX; }
 
@@ -482,7 +486,7 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_forward_kernel(
     const int64_t t1 = t0 + tiles_per_range < ytiles ? t0 + tiles_per_range : ytiles;
     const int64_t own0 = block * DI_OWN + wave * 32;
     const bool active = own0 < n;
-    const float c = ldexpf(step, -di_scale_exponent(parts) - di_scale_exponent(parts + DI_PARTS));
+    const float c = di_logit_factor(step, di_scale_exponent(parts) + di_scale_exponent(parts + DI_PARTS));
 
     u32x4 own[2][F / 16];
     if (active) di_load_own<F>(ximg + (own0 / 32) * D::BYTES, own);
@@ -610,7 +614,7 @@ __global__ __launch_bounds__(64 * DI_NW) void distill_backward_kernel(
     const int sx = di_scale_exponent(parts), sy = di_scale_exponent(parts + DI_PARTS);
     // the weights of the rows; |q - p| is at most 1, and so is |q_r - p_r| e / S: S sums the e off the list
     const int sg = di_scale_exponent(parts + 2 * DI_PARTS);
-    const float c = ldexpf(step, -sx - sy);
+    const float c = di_logit_factor(step, sx + sy);
 
     const float back = ldexpf(temperature, -sx - sg);
 

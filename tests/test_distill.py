@@ -279,6 +279,19 @@ def test_rows_and_items_of_very_different_size(dev):
 
 
 @gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("m", [900, 928, 5])
+@pytest.mark.parametrize("scale", [1e-15, 1e-20, 1e-25])
+def test_factors_whose_products_vanish(dev, scale, m, tail):
+    """Logits of 1e-30 and less, and of zero in fp32: a uniform softmax, and gradients of the factors' size."""
+    X, Y, ids, scores, _, grad = problem(18, 70, m, 64, 16, dev)
+    X, Y = X * scale, Y * scale
+    tlse = torch.logsumexp(scores, 1) + 0.5 if tail else None
+    got = E.distill(X, Y, ids, scores, teacher_lse=tlse, grad=grad)
+    compare(X, Y, ids, scores, 1.0, tlse, grad, got)
+
+
+@gpu
 def test_weights_of_very_different_size(dev):
     X, Y, ids, scores, _, grad = problem(13, 100, 600, 32, 12, dev)
     grad = grad * torch.logspace(-12, 0, 100, device=dev)
