@@ -276,7 +276,10 @@ int mirec_topk_ordered(const float* Q, int64_t nq, const float* Y, int64_t ni, i
  * MIREC_SAMPLE_MAX_MASKED_ITEMS items) and list positions with a negative id.
  * Weights are fixed-point numbers of S = min(51, 62 - ceil(log2 m)) fraction bits, so
  * the result does not depend on any order of summation; an item less likely than
- * 2^-(S+1) of the best one is never drawn.
+ * 2^-(S+1) of the best one is not drawn while that is there, nor kept by a min_p above 0.
+ * Without replacement the weights are formed anew, relative to the best item left of
+ * those the cuts kept, where their sum falls below 2^min(ceil(log2 m) + 23, S - 1) units:
+ * all of these items come before a -1, each with its probability among those left.
  *   scores       [n, m] of `dtype` (MIREC_F32 / F16 / BF16), row r at r * row_stride elements
  *   ids          int32 [n, m], row r at r * ids_stride elements, or null
  *   uniforms     fp32 [n, draws] in [0, 1); values outside are moved to its ends, NaN to 0

@@ -17,7 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "libmirec.so")
 SOURCES = ["core.hip", "gram.hip", "als_sweep.hip", "als_short.hip", "plan_sort.hip", "topk.hip", "topk_small.hip", "topk_order.hip", "topk_inst_0.hip", "topk_inst_1.hip",
-           "topk_inst_2.hip", "topk_inst_3.hip", "topk_inst_4.hip", "topk_inst_5.hip", "sample.hip", "distill.hip", "lightfm.hip", "lightfm_train.hip", "transpose.hip", "metrics.hip", "build_matrix.hip"]
+           "topk_inst_2.hip", "topk_inst_3.hip", "topk_inst_4.hip", "topk_inst_5.hip", "sample.hip", "sample_inst_with.hip", "sample_inst_without.hip", "distill.hip", "lightfm.hip", "lightfm_train.hip", "transpose.hip", "metrics.hip", "build_matrix.hip"]
 HEADERS = sorted(os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")) + [os.path.join(ROOT, "include", "mirec.h")]
 # No packed fp32 instructions: the compiler forms them by itself from ordinary float code, and some of their forms have
 # given wrong results on gfx950 now and then (the host pass warns that it does not know the feature: harmless).

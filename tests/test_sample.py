@@ -157,7 +157,7 @@ def waits_missing(source):
 
 
 def test_cross_lane_steps_keep_their_wait_states():
-    text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "sample.hip")).read()
+    text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "sample_kernel.h")).read()
     assert len(re.findall(r"#define SM_\w+_STEP", text)) == 2
     assert waits_missing(text) == []
     # what the check is for: a carry read directly behind its write, a move directly behind a write
@@ -437,6 +437,123 @@ def test_without_replacement_no_item_twice(dev, m):
         check(s, u, ids, lp, replacement=False)
         assert torch.equal(torch.sort(ids[:, :m], dim=1).values, torch.arange(m, dtype=torch.int32, device=dev).expand(3, m))
         assert torch.all(ids[:, m:] == -1)
+
+
+def check_leaving(scores, uniforms, got_ids, got_lp, ids=None, T=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws without replacement against the definition in logarithms, so that an item counts however unlikely it was beside
+    those that have left.  The device forms its weights anew once their sum is below 2^(ceil(log2 m) + 23) units (m up to
+    2^19): m roundings of half a unit are 2^-24 of it at most, the border error on top."""
+    low = float(torch.finfo(scores.dtype).min)
+    s, u = scores.double().cpu().numpy(), uniforms.double().cpu().numpy()
+    got_ids, got_lp = got_ids.cpu().numpy(), got_lp.cpu().numpy()
+    n, m = s.shape
+    tol = 2.0 ** -24 + border_error(m)
+    for r in range(n):
+        ok = s[r] > low
+        if ids is not None:
+            lid = ids[r].cpu().numpy()
+            ok &= lid >= 0
+        t = float(T[r]) if isinstance(T, torch.Tensor) else T
+        best = s[r][ok].max() if ok.any() else 0.0
+        d = (s[r] - best) / t
+        left = [i for i in sorted(np.flatnonzero(ok), key=lambda i: (-s[r][i], i))]
+        if top_k > 0:
+            left = left[:top_k]
+        if top_p < 1:
+            mass = np.exp(d[left])
+            before = np.concatenate([[0.0], np.cumsum(mass)[:-1]])
+            left = [i for j, i in enumerate(left) if j == 0 or before[j] < top_p * mass.sum()]
+        if min_p > 0:
+            left = [i for i in left if d[i] >= math.log(min_p)]
+        left = np.array(sorted(left), dtype=np.int64)
+        for j in range(u.shape[1]):
+            where = f"row {r} draw {j}"
+            if left.size == 0:
+                assert got_ids[r, j] == -1 and got_lp[r, j] == -np.inf, where
+                continue
+            i = got_ids[r, j]
+            if ids is not None:
+                i = np.flatnonzero(lid == i)[0]
+            at = np.flatnonzero(left == i)
+            assert at.size == 1, f"{where}: {i} is not there"
+            w = np.exp(d[left] - d[left].max())
+            hi = np.cumsum(w)[at[0]] / w.sum()
+            lo = hi - w[at[0]] / w.sum()
+            assert lo - tol <= u[r, j] < hi + tol, f"{where}: item {i} holds [{lo}, {hi}), drawn with {u[r, j]}"
+            lp = d[i] - d[left].max() - math.log(w.sum())
+            assert got_lp[r, j] <= 0 and abs(got_lp[r, j] - lp) <= 2.0 ** -24 * abs(lp) + 2 * tol, f"{where}: {got_lp[r, j]} {lp}"
+            left = np.delete(left, at[0])
+
+
+def stepped(seed, n, m, gap, T, dtype="f32", few=3):
+    """Scores (in units of T) of standard deviation one around 0, -gap and -2 gap: `few` items on each of the first two steps."""
+    g = torch.Generator().manual_seed(seed)
+    level = torch.full((n, m), 2.0)
+    for r in range(n):
+        at = torch.randperm(m, generator=g)
+        level[r, at[:few]], level[r, at[few:2 * few]] = 0.0, 1.0
+    return ((torch.randn(n, m, generator=g) - gap * level) * T).to(TORCH[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("gap", [10.0, 20.0, 34.0, 36.5, 50.0, 700.0])
+@pytest.mark.parametrize("m", [5, 40, 64, 100, 200, 257, 3001, 20000])
+@pytest.mark.parametrize("cut", [dict(), dict(top_k=30), dict(top_k=400), dict(min_p=1e-13), dict(T=0.02), dict(top_p=0.75, T=3.0)])
+def test_items_far_less_likely_follow_those_that_left(dev, m, gap, cut):
+    """Every kept item is drawn before -1, with its probability among those left."""
+    T, n = cut.get("T", 1.0), 5
+    s = stepped(m, n, m, gap, T).to(dev)
+    draws = min(m + 2, 70) if m <= 200 else 10
+    u = torch.rand(n, draws, generator=torch.Generator().manual_seed(m + 1)).to(dev)
+    kw = {{"T": "temperature"}.get(k, k): v for k, v in cut.items()}
+    ids, lp = E.sample_scores(s, u, replacement=False, **kw)
+    check_leaving(s, u, ids, lp, **cut)
+
+
+@gpu
+def test_a_step_between_every_two_items(dev):
+    """The weights are formed anew at every draw; rows of all kernels, and scores of all types."""
+    for m, dtype, cut in ((2, "f32", {}), (64, "f32", {}), (90, "bf16", {}), (256, "f16", {}), (300, "f32", {}), (300, "f32", {"top_k": 100}),
+                          (2000, "bf16", {"top_k": 100}), (9000, "f32", {}), (20000, "f32", {"top_p": 0.9})):
+        g = torch.Generator().manual_seed(m)
+        s = torch.stack([torch.randperm(m, generator=g) for _ in range(3)]).float() * (-250.0 / m if dtype == "f16" else -1.0)
+        s = s.to(TORCH[dtype]).to(dev)
+        u = torch.rand(3, min(m + 1, 40), generator=g).to(dev)
+        T = 250.0 / m / 60 if dtype == "f16" else 1 / 60
+        ids, lp = E.sample_scores(s, u, temperature=T, replacement=False, **cut)
+        check_leaving(s, u, ids, lp, T=T, **cut)
+
+
+@gpu
+@pytest.mark.parametrize("m", [30, 100, 200])
+def test_stepped_lists_that_share_a_wavefront(dev, m):
+    """Ranked lists with and without steps side by side: each draws what it draws alone."""
+    n = 30011
+    g = torch.Generator().manual_seed(m)
+    s = torch.randn(n, m, generator=g) - 45.0 * (torch.arange(m) >= torch.randint(1, m + 1, (n, 1), generator=g))
+    s = torch.where(torch.rand(n, 1, generator=g) < 0.8, torch.sort(s, dim=1, descending=True).values, s)
+    ids = (torch.randint(0, 1 << 20, (n, m), generator=g, dtype=torch.int32) * 1024 + torch.arange(m, dtype=torch.int32)).to(dev)
+    ids[::7, ::3] = -1
+    s, u = s.to(dev), torch.rand(n, 9, generator=g).to(dev)
+    T = (0.3 + torch.rand(n, generator=g)).to(dev)
+    got, lp = E.sample_scores(s, u, ids=ids, temperature=T, replacement=False)
+    for r in (0, 1, 2, 3, 777, 14976, 14977, n - 2, n - 1):
+        one = slice(r, r + 1)
+        alone = E.sample_scores(s[one], u[one], ids=ids[one], temperature=T[one], replacement=False)
+        assert torch.equal(got[one], alone[0]) and torch.equal(lp[one], alone[1]), r
+    at = torch.arange(0, n, 997).to(dev)
+    check_leaving(s[at], u[at], got[at], lp[at], ids=ids[at], T=T[at].cpu())
+
+
+@gpu
+def test_a_certain_draw_has_probability_one(dev):
+    """What is reported for an item that was sure to be drawn, after others have left and before."""
+    for s, T in (([1.0, 0.105], 0.025), ([0.0, -35.0], 1.0), ([1.2, 0.45, 0.44, 0.43, 0.42], 0.02), ([0.0, -36.2, -36.3], 1.0)):
+        s = torch.tensor([s], device=dev)
+        u = torch.full((1, s.shape[1] + 1), 0.4, device=dev)
+        ids, lp = E.sample_scores(s, u, temperature=T, replacement=False)
+        check_leaving(s, u, ids, lp, T=T)
+        assert lp[0, s.shape[1] - 1] == 0.0 and ids[0, -1] == -1
 
 
 @gpu
