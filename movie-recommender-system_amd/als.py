@@ -144,12 +144,14 @@ class AlternatingLeastSquares:
         self.dtype = np.dtype(np.float32)
         self._reset_caches()
 
-    def _start_factors(self, users: int, items: int) -> None:
-        rs = _random_state(self.random_state)
-        if self.user_factors is None:
-            self.user_factors = rs.rand(users, self.factors).astype(np.float32) * 0.01
-        if self.item_factors is None:
-            self.item_factors = rs.rand(items, self.factors).astype(np.float32) * 0.01
+    def _start_factors(self, users: int, items: int):
+        """The factors that training starts from: those that are set, or random ones (the model is left as it is)."""
+        rs, X, Y = _random_state(self.random_state), self.user_factors, self.item_factors
+        if X is None:
+            X = rs.rand(users, self.factors).astype(np.float32) * 0.01
+        if Y is None:
+            Y = rs.rand(items, self.factors).astype(np.float32) * 0.01
+        return X, Y
 
     # -------------------------------------------------------------------- fit
     def fit(self, user_items, show_progress: bool = True, callback=None) -> None:
@@ -162,7 +164,7 @@ class AlternatingLeastSquares:
         if Cui.nnz >= 2 ** 31:
             raise ValueError("more than 2^31 stored interactions in one matrix")
         dev = E.require_cuda(self.device)
-        self._start_factors(users, items)
+        self.user_factors, self.item_factors = self._start_factors(users, items)
         if self.user_factors.shape != (users, self.factors) or self.item_factors.shape != (items, self.factors):
             raise ValueError("user_factors / item_factors do not match the matrix shape")
         if not self.use_cg and Cui.nnz and float(np.abs(Cui.data).min()) * abs(self.alpha) < 1.0:
@@ -523,7 +525,8 @@ class AlternatingLeastSquares:
         per user T^2 KL(p || q), p the softmax of the teacher's ``N`` (at most 224) best scores over ``temperature`` (without the
         items of ``user_items``, where given) and q the softmax of this model's scores of all items.  ``epochs``
         passes over the users in batches, Adam steps on both sides; starts from the factors that are set (``fit``'s
-        start otherwise).  Returns the mean loss of every epoch."""
+        start otherwise).  A call that is refused or fails leaves the model as it was.  Returns the mean loss of every
+        epoch."""
         if teacher.user_factors is None or teacher.item_factors is None:
             raise ValueError("the teacher has not been fitted")
         users, items = teacher.user_factors.shape[0], teacher.item_factors.shape[0]
@@ -537,9 +540,9 @@ class AlternatingLeastSquares:
                 raise ValueError("user_items must have the teacher's users and items")
             if not mask.has_sorted_indices:
                 mask = mask.sorted_indices()
-        self._start_factors(users, items)
-        if self.user_factors.shape != (users, self.factors) or self.item_factors.shape != (items, self.factors):
-            raise ValueError("user_factors / item_factors do not match the teacher's users and items")
+        for P, rows in ((self.user_factors, users), (self.item_factors, items)):
+            if P is not None and P.shape != (rows, self.factors):
+                raise ValueError("user_factors / item_factors do not match the teacher's users and items")
         dev = E.require_cuda(self.device)
         W = E.factor_width(teacher.factors, for_scoring=True)
         F = E.factor_width(self.factors)
@@ -548,7 +551,7 @@ class AlternatingLeastSquares:
             dmask = None if mask is None else E.DeviceCSR.from_scipy(mask, dev)
             batches = [(a, min(a + int(batch), users)) for a in range(0, users, int(batch))]
             lists = [E.topk(XT[a:b], YT, N, None if dmask is None else dmask.rows(a, b)) for a, b in batches]
-            X, Y = E.pad_factors(self.user_factors, F, dev), E.pad_factors(self.item_factors, F, dev)
+            X, Y = (E.pad_factors(P, F, dev) for P in self._start_factors(users, items))
             mX, vX, mY, vY = (torch.zeros_like(P) for P in (X, X, Y, Y))
             need = max((int(_lib.require().mirec_distill_workspace_bytes(b - a, items, F, N)) for a, b in batches), default=0)
             ws = torch.empty(need, dtype=torch.uint8, device=dev)

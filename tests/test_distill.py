@@ -669,6 +669,37 @@ def test_a_model_learns_from_a_models_lists(dev, liked):
 
 
 @gpu
+def test_a_refused_distillation_leaves_the_model_as_it_was(dev):
+    from scipy import sparse as sp
+    from movie_recommender_system_amd.als import AlternatingLeastSquares
+    g = np.random.default_rng(62)
+    teacher = AlternatingLeastSquares(factors=16)
+    teacher.user_factors, teacher.item_factors = (g.normal(0, 0.5, (c, 16)).astype(np.float32) for c in (30, 400))
+    bad = [dict(N=300), dict(temperature=0.0), dict(temperature=float("nan")), dict(N=0), dict(learning_rate=-1.0),
+           dict(user_items=sp.csr_matrix((30, 399), dtype=np.float32))]
+    new = AlternatingLeastSquares(factors=8, random_state=3)
+    old = AlternatingLeastSquares(factors=8, random_state=3)
+    x, y = (g.normal(0, 0.5, (c, 8)).astype(np.float32) for c in (30, 400))
+    old.user_factors, old.item_factors = x, y
+    half = AlternatingLeastSquares(factors=8, random_state=3)
+    half.item_factors = np.zeros((7, 8), np.float32)     # not the teacher's items
+    for kw in bad:
+        for model in (new, old, half):
+            with pytest.raises((ValueError, _lib.MirecError)):
+                model.distill(teacher, **kw)
+        assert new.user_factors is None and new.item_factors is None
+        assert old.user_factors is x and old.item_factors is y and half.user_factors is None
+    with pytest.raises(ValueError):
+        half.distill(teacher)
+    with pytest.raises(ValueError):                      # still a model that was never fitted
+        new.sample(0, None, filter_already_liked_items=False)
+    with pytest.raises(_lib.MirecError):                 # wider than the kernels
+        wide = AlternatingLeastSquares(factors=200)
+        wide.distill(teacher)
+    assert wide.user_factors is None and wide.item_factors is None
+
+
+@gpu
 def test_the_list_of_the_best_items_to_draws(dev):
     """The operators together, as they are used: a teacher's top-K lists, a student's step, its own lists, draws."""
     g = torch.Generator().manual_seed(3)
