@@ -265,7 +265,8 @@ int mirec_topk_ordered(const float* Q, int64_t nq, const float* Y, int64_t ni, i
  *   w_i >= min_p * max w; a temperature below 1e-37 keeps the best item;
  *   draw d takes the first index i whose running sum of kept weights, in ascending
  *   index order, exceeds uniforms[row, d] * total.
- * replacement = 0: a drawn item leaves the row before its next draw.
+ * replacement = 0: a drawn entry leaves the row before its next draw (an item that a
+ * list names twice has two entries).
  * out_ids int32[n, draws]: the item (ids[row, i] where ids are given, else i), or -1
  * where nothing is left; out_logprob fp32[n, draws]: the natural logarithm of the
  * probability the item was drawn with (-inf with id -1).

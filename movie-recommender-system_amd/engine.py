@@ -550,8 +550,8 @@ def sample_scores(scores: torch.Tensor, uniforms: torch.Tensor, ids: Optional[to
 
     ``ids`` (int32 [n, m]): the rows are ranked lists as ``topk`` returns them, the drawn list entries' ids come
     back and entries with a negative id or the score -FLT_MAX are never drawn; without it the rows are dense and
-    ``mask`` may hold one row of filtered items per row, as in ``topk``.  ``replacement=False``: an item is drawn
-    at most once per row.
+    ``mask`` may hold one row of filtered items per row, as in ``topk``.  ``replacement=False``: an entry
+    of a row is drawn at most once (an item that a list names twice has two), and those the cuts kept all come before a -1.
 
     Returns (ids int32 [n, draws], logprob fp32 [n, draws]): the items and the logarithms of the probabilities they
     were drawn with; (-1, -inf) where nothing is left to draw.  The same inputs give the same bits on every call."""

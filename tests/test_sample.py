@@ -557,6 +557,23 @@ def test_a_certain_draw_has_probability_one(dev):
 
 
 @gpu
+@pytest.mark.parametrize("m", [3, 70, 130, 300])
+def test_an_item_listed_twice_has_two_entries(dev, m):
+    """Its entries are drawn apart, each with the probability of its own score."""
+    g = torch.Generator().manual_seed(m)
+    s = torch.randn(4, m, generator=g)
+    s[2:] = torch.sort(s[2:], dim=1, descending=True).values
+    u = torch.rand(4, m + 1, generator=g)
+    one = torch.arange(m, dtype=torch.int32).expand(4, m).contiguous()
+    for replacement in (True, False):
+        a, la = E.sample_scores(s.to(dev), u.to(dev), ids=one.to(dev), replacement=replacement)
+        b, lb = E.sample_scores(s.to(dev), u.to(dev), ids=(one // 2).to(dev), replacement=replacement)
+        assert torch.equal(torch.where(a < 0, a, a // 2), b) and torch.equal(la, lb)
+        if not replacement:
+            assert torch.equal(torch.sort(a[:, :m], dim=1).values.cpu(), one) and torch.all(b[:, m] == -1)
+
+
+@gpu
 @pytest.mark.parametrize("m", [90, 2000])
 def test_parameters_per_row(dev, m):
     n = 24
