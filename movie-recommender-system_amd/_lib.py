@@ -65,7 +65,7 @@ SIGNATURES = {
     "mirec_ranking_hits": (_int, [_vp, _i64, _int, _vp, _vp, _vp, _vp, _vp]),
 }
 
-ABI_VERSION = 102   # mirec_version() of the library these signatures belong to
+ABI_VERSION = 102   # the oldest mirec_version() with these signatures (103 adds entry points)
 
 _lib = None
 _lock = threading.Lock()
@@ -90,7 +90,7 @@ def load(path: str = LIB_PATH):
             have = lib.mirec_version()
             if have < ABI_VERSION:
                 # entry points have changed their parameters: an older build would be called with shifted arguments
-                raise MirecError(f"{path} is version {have}, this package binds version {ABI_VERSION}: rebuild it "
+                raise MirecError(f"{path} is version {have}, this package binds version {ABI_VERSION} or later: rebuild it "
                                  "with `python __graft_entry__.py`")
             for name, (res, args) in SIGNATURES.items():
                 fn = getattr(lib, name, None)

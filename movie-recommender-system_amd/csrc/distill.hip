@@ -25,13 +25,14 @@
 // (below) and no logit passes through LDS or memory.
 //   distill_forward_kernel   owns rows of X, streams Y: running maximum, mass and mean of the items (dX's dense part); with
 //                            the class the listed items' logits become minus infinity, found by the lists' entries
-//                            grouped by (row tile, item tile) before the pass (4096 x 27000 at 128, lists of 100: 164 us
-//                            without, 179 with; grouping 6 us beside the largest magnitudes)
+//                            grouped by (row tile, item tile) before the pass (4096 x 27000 at 128, lists of 100: a step
+//                            takes 414 us with all this, 391 without)
 //   distill_backward_kernel  owns rows of Y, streams X: dY; the logits are formed a second time (three of twelve
 //                            matrix products) because keeping them would write and read n m of them
-// What bounds them: the matrix cores from 128 columns on (2048 x 200000 at 128: 0.53 and 0.62 ms, 1.10 PFLOP/s of plane
-// products, 96 % of what a large fp16 product of the library reaches here; 4096 x 27000: 0.15 and 0.19 ms); below, the
-// exponentials and conversions of a logit beside few products (1024 x 27000 at 64: 28 and 43 us, 0.6 PFLOP/s).
+// What bounds them: the matrix cores from 128 columns on (2048 x 200000 at 128: 0.51 and 0.57 ms, from run to run 1.08 to 1.16
+// PFLOP/s of plane products; a large fp16 product of the library reaches 1.15 here; 4096 x 27000 with the class: 0.17 and
+// 0.20 ms); below, the exponentials and conversions of a logit beside few products (1024 x 27000 at 64: 27 and 42 us, 0.6
+// PFLOP/s).
 //
 // fp32 on the fp16 matrix cores: an operand is two fp16 planes, hi = fp16(v), mid = fp16(v - hi), of the value scaled
 // by a power of two that puts its matrix's largest entry just below 2^15, and a product is hi hi + hi mid + mid hi in
@@ -787,8 +788,8 @@ __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* _
 // group of lanes in flight, and what does not depend on each other is asked for at once.  NT threads: 256 finish a row
 // soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) more rows than run at once with 256
 // (DI_MANY_ROWS: 1024 lists of 50 at 64 columns 12 and 16 us, 1500 of 200 at 192 columns 52 and 40).  4096 lists of 100 at 128
-// columns with the class 48 us, of which the factor rows, 0.2 GB from L2, are a third.  REST: two sums of the list's items in
-// registers, three wavefronts per SIMD from 96 columns on (four spill: 50 us).
+// columns with the class 45 us, of which the factor rows, 0.2 GB from L2, are a third.  REST: two sums of the list's items in
+// registers, three wavefronts per SIMD from 96 columns on (four spill and gain nothing).
 template <int F, int NT, bool REST>
 __global__ __launch_bounds__(NT, NT == 64 && F <= 128 ? (REST && F > 64 ? 3 : 4) : 2) void distill_list_kernel(
     const float* __restrict__ X, int64_t n, const float* __restrict__ Y, int64_t m, const int32_t* __restrict__ ids,
@@ -1246,7 +1247,7 @@ static int distill_check_ws(const char* who, const void* ws, size_t ws_bytes, si
     return MIREC_OK;
 }
 
-// Dynamic LDS of the two passes (two tiles) needs an attribute once per kernel and device.
+// Dynamic LDS of the two passes (two to four tiles) needs an attribute once per kernel and device.
 static int distill_lds(const void* kernel, int bytes, OncePerDevice& once, const char* who) {
     bool* done = once.slot();
     MIREC_REQUIRE(done, MIREC_E_HIP, "%s: cannot read the current device", who);

@@ -231,8 +231,8 @@ __device__ __forceinline__ float sm_logprob(float score, double best, double ste
 // the other, and keep their draws, one each, until all lanes have one: logarithms and stores are then one for all.
 // AGAIN: drawn items come back.
 // What bounds it is the number of vector instructions per row; most of them are for the row, not for its items, so that two
-// rows of up to 128 items share them.  Measured: 262144 lists of 100 under top_p and min_p 107 us (2 TB/s of scores and ids;
-// the bytes alone 53 us), of 50 76 us, one list 3.4 us.
+// rows of up to 128 items share them.  Measured: 262144 lists of 100 under top_p and min_p 104 us (2 TB/s of scores and ids;
+// the bytes alone 53 us), of 50 76 us, one list 3.4 us; ten draws without replacement under top_p 412 us.
 template <int DT, int E, int R, bool AGAIN>
 __global__ __launch_bounds__(256) void sample_short_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int m, int64_t stride, const int32_t* __restrict__ ids,
@@ -563,8 +563,8 @@ struct Chunk {
 // What bounds it: where the rows in flight exceed L2 each pass reads them at the rate of memory (two passes over 4096 x 27000
 // in 186 us, 4.75 TB/s), and a weight is 21 instructions (nine of them its polynomial); under top_p both take about 280 of
 // the 340 us of those rows.  Hence as few passes as possible, and four rows of 256 threads side by side on a compute unit, or
-// fewer of more threads where there are fewer rows.  Measured: 1024 x 27000 under top_p 104 us, 512 x 200000 bf16 uncut,
-// 8 draws, 149 us, one row of 27000 under top_k 17 us.
+// fewer of more threads where there are fewer rows.  Measured: 1024 x 27000 under top_p 105 us, 512 x 200000 bf16 uncut,
+// 8 draws, 144 us, one row of 27000 under top_k 17 us.
 // Registers: few rows, of 1024 threads, run one or two workgroups to a compute unit and are faster with more registers
 // (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6).  512 threads ask for 6; of 256 threads LDS
 // admits four rows, and a fifth (histogram, list and draws in one place) gains under top_p what it loses under top_k.  Without
