@@ -49,7 +49,7 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     for src in sources:
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ_DIR, src.replace(".hip", ".o"))
-        if force or _stale(o, [s] + HEADERS):
+        if force or _stale(o, [s, os.path.abspath(__file__)] + HEADERS):   # (this file holds the flags)
             jobs.append((s, o))
 
     def compile_one(job):

@@ -407,3 +407,37 @@ def test_optional_arguments_are_checked_before_any_device_call():
         model.recommend(0, row, N=2, items=[1, 5])
     with pytest.raises(ValueError, match="recalculate_user needs user_items"):
         model.recommend(0, None, N=2, recalculate_user=True)
+
+
+def test_the_library_is_built_again_where_its_flags_changed(monkeypatch, tmp_path):
+    """build_lib compiles what is older than its source, a header or the file that holds the compiler's flags (no compiler
+    is run here)."""
+    import subprocess
+    from movie_recommender_system_amd import build
+    made = []
+
+    def run(cmd, **kw):
+        out = cmd[cmd.index("-o") + 1]
+        made.append(os.path.basename(out))
+        open(out, "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "OBJ_DIR", str(tmp_path))
+    monkeypatch.setattr(build, "LIB_PATH", str(tmp_path / "lib.so"))
+    everything = sorted([s.replace(".hip", ".o") for s in build.SOURCES] + ["lib.so"])
+    build.build_lib()
+    assert sorted(made) == everything
+    made.clear()
+    build.build_lib()
+    assert made == []
+    flags, real = os.path.getmtime(os.path.abspath(build.__file__)), os.path.getmtime
+
+    def age(path):   # built after the sources, before the flags
+        if path.startswith(build.CSRC) or path.endswith("mirec.h"):
+            return flags - 2
+        return flags - 1 if path.startswith(str(tmp_path)) else real(path)
+
+    monkeypatch.setattr(build.os.path, "getmtime", age)
+    build.build_lib()
+    assert sorted(made) == everything
