@@ -441,3 +441,14 @@ def test_the_library_is_built_again_where_its_flags_changed(monkeypatch, tmp_pat
     monkeypatch.setattr(build.os.path, "getmtime", age)
     build.build_lib()
     assert sorted(made) == everything
+
+
+def test_the_build_entry_point_compiles_what_is_built_already(monkeypatch):
+    import __graft_entry__
+    import oracle
+    from movie_recommender_system_amd import build
+    forced = []
+    monkeypatch.setattr(build, "build_lib", lambda force=False, verbose=False: forced.append(force) or build.LIB_PATH)
+    monkeypatch.setattr(oracle, "build", lambda: "")
+    __graft_entry__.build()
+    assert forced == [True]
