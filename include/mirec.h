@@ -280,7 +280,8 @@ int mirec_topk_ordered(const float* Q, int64_t nq, const float* Y, int64_t ni, i
  * 2^-(S+1) of the best one is not drawn while that is there, nor kept by a min_p above 0.
  * Without replacement the weights are formed anew, relative to the best item left of
  * those the cuts kept, where their sum falls below 2^min(ceil(log2 m) + 23, S - 1) units:
- * all of these items come before a -1, each with its probability among those left.
+ * all of these items come before a -1, each with its probability among those left.  (A
+ * row of more than 256 items is read twice more each time, unless top_k is 128 or less.)
  *   scores       [n, m] of `dtype` (MIREC_F32 / F16 / BF16), row r at r * row_stride elements
  *   ids          int32 [n, m], row r at r * ids_stride elements, or null
  *   uniforms     fp32 [n, draws] in [0, 1); values outside are moved to its ends, NaN to 0

@@ -783,9 +783,9 @@ __global__ __launch_bounds__(DI_THREADS) void distill_join_kernel(const float* _
 
 // One workgroup per row: joins the row's partial results (REST: with teacher_lse, those of the items off the list); the list
 // without its excluded entries, entries that name the same item merged (their probabilities add); the row's loss; its dX
-// but for the weight.  Latency, not bandwidth, is
-// what a row costs (a chain of a dozen dependent steps): factor rows are read by sixteen lanes each, four rows of a
-// group of lanes in flight, and what does not depend on each other is asked for at once.  NT threads: 256 finish a row
+// but for the weight.  Latency, not bandwidth, is what a row costs (a chain of a dozen dependent steps): factor rows are
+// read by sixteen lanes each, four rows of a group of lanes in flight, and what does not depend on each other is asked for
+// at once.  NT threads: 256 finish a row
 // soonest, 64 (no barriers, sixteen rows in flight on a compute unit instead of four) more rows than run at once with 256
 // (DI_MANY_ROWS: 1024 lists of 50 at 64 columns 12 and 16 us, 1500 of 200 at 192 columns 52 and 40).  4096 lists of 100 at 128
 // columns with the class 45 us, of which the factor rows, 0.2 GB from L2, are a third.  REST: two sums of the list's items in

@@ -569,7 +569,8 @@ struct Chunk {
 // (one row of 27000: 22.3 -> 17.7 us with 4 wavefronts per SIMD in place of 6).  512 threads ask for 6; of 256 threads LDS
 // admits four rows, and a fifth (histogram, list and draws in one place) gains under top_p what it loses under top_k.  Without
 // AGAIN (drawn items come back) those of 256 have to be asked for the four: weights formed anew take more registers
-// (1024 x 27000 uncut, 5 draws: 78 us with three rows, 63 with four).
+// (1024 x 27000 uncut, 5 draws: 78 us with three rows, 63 with four).  Each time that weights are formed anew reads the row twice:
+// at a temperature of 0.02 of the scores' deviation, 10 draws of 1024 x 27000 take 392 us, at 0.5 of it 83.
 template <int DT, int NT, bool LISTS, bool AGAIN>
 __global__ __launch_bounds__(NT, NT == 1024 || (NT == 256 && !AGAIN) ? 4 : 6) void sample_long_kernel(
     const typename ScoreType<DT>::raw* __restrict__ scores, int64_t n, int64_t m, int64_t stride,

@@ -525,6 +525,47 @@ def test_a_step_between_every_two_items(dev):
 
 
 @gpu
+@pytest.mark.parametrize("m,dtype", [(300_007, "f32"), (524_288, "bf16"), (524_288, "f32")])
+@pytest.mark.parametrize("cut", [dict(), dict(top_k=60), dict(min_p=1e-12)])
+def test_steps_in_rows_of_more_than_1024_chunks(dev, m, dtype, cut):
+    s = stepped(m, 2, m, 45.0, 1.0, dtype, few=4).to(dev)
+    u = torch.rand(2, 12, generator=torch.Generator().manual_seed(m)).to(dev)
+    ids, lp = E.sample_scores(s, u, replacement=False, **cut)
+    check_leaving(s, u, ids, lp, **cut)
+
+
+@gpu
+def test_steps_beside_a_filter_and_in_a_replayed_graph(dev):
+    """Filtered items stay out of the weights that are formed anew; two captured calls give the eager draws on every replay."""
+    for n, m, cut in ((5, 150, {}), (4, 2000, {"top_k": 90}), (4, 5000, {})):
+        s = stepped(m, n, m, 50.0, 1.0).to(dev)
+        u = torch.rand(n, 10, generator=torch.Generator().manual_seed(m)).to(dev)
+        rows, csr = filter_rows(m, n, m, 0.5, dev)
+        call = lambda: E.sample_scores(s, u, mask=csr, replacement=False, **cut)
+        want = call()
+        inside = s.clone()
+        for r, out in enumerate(rows):
+            inside[r, torch.from_numpy(out).to(dev)] = torch.finfo(torch.float32).min
+        check_leaving(inside, u, *want, **cut)
+        torch.cuda.synchronize()
+        graphs, outs = [], []
+        for _ in range(2):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr):
+                outs.append(call())
+            graphs.append(gr)
+        for _ in range(3):
+            for gr, o in zip(graphs, outs):
+                o[0].fill_(7)
+                o[1].fill_(7.0)
+                gr.replay()
+            again = call()
+            torch.cuda.synchronize()
+            for o in outs + [again]:
+                assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
+
+
+@gpu
 @pytest.mark.parametrize("m", [30, 100, 200])
 def test_stepped_lists_that_share_a_wavefront(dev, m):
     """Ranked lists with and without steps side by side: each draws what it draws alone."""
